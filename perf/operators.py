@@ -170,11 +170,17 @@ def key_like(g, *shape):
     return x
 
 
+def scale_for(top):
+    """The smallest power of two s in [2^-100, 2^120] with 127 s >= top."""
+    m, e = torch.frexp(top)
+    e = torch.where(top > 0, e - 7 + (m > 0.9921875).int(), -100)
+    return torch.exp2(e.clamp(-100, 120).float())
+
+
 def quantised(x, block):
     """Codes and block scales of [..., tokens, d] values (tokens a multiple of block)."""
     b = x.unflatten(-2, (-1, block))
-    m, e = torch.frexp(b.abs().amax((-1, -2)))
-    s = torch.exp2((e - 7 + (m > 0.9921875).int()).clamp(-100, 120).float())
+    s = scale_for(b.abs().amax((-1, -2)))
     return torch.round(b / s[..., None, None]).to(torch.int8).flatten(-3, -2), s
 
 
@@ -334,8 +340,7 @@ def plain_appended(new, codes, scales, x, case):
     is_new = (at >= 0) & (at < count)
     row = (torch.arange(n, device="cuda")[:, None] * count + at.clamp(0, count - 1)).flatten()
     fresh = new.index_select(0, row).float().view(n, width, hk, d).transpose(1, 2) * is_new[:, None, :, None]
-    m, e = torch.frexp(fresh.unflatten(2, (-1, block)).abs().amax((-1, -2)))
-    s = torch.exp2((e - 7 + (m > 0.9921875).int()).clamp(-100, 120).float())
+    s = scale_for(fresh.unflatten(2, (-1, block)).abs().amax((-1, -2)))
     has_old = (slot[:, ::block] < x["lens"][:, None])[:, None]
     s_old = torch.where(has_old, s_old, torch.full_like(s_old, 2.0 ** -100))
     s = torch.maximum(s, s_old)
