@@ -350,6 +350,153 @@ int vg_flat_search_ip_noalloc(const float *db, size_t n, const float *queries,
                               void *stream, uint32_t *out_ids, float *out_dist,
                               uint32_t *out_count);
 
+/* ---- key/value cache held in 8 bits ------------------------------------
+ *
+ * No counterpart in the reference: the index's codes-and-queries scheme for
+ * the context of a language model served next to it.  Keys and values are
+ * kept as 8-bit codes with one scale per (sequence, head, block of tokens);
+ * queries stay in 16 bits; attention is the exhaustive inner-product scan
+ * with a softmax in place of the top-k.
+ *
+ * The functions of this section enqueue their work on `stream` (a cudaStream_t
+ * of the handle's device, NULL = legacy default stream) and return without
+ * waiting for it.  Tensors are device memory that stays valid until that work
+ * is done; counts, lengths and sequence lists are host memory, read before
+ * the call returns.  A vg_kv_cache is externally synchronised on the host;
+ * work on its contents is ordered by the handle, also across streams.  Its
+ * functions cannot be captured into a CUDA graph (lengths and launch shapes
+ * are host state): VG_ERR_UNSUPPORTED. */
+
+/* Element types of tensors. */
+enum { VG_F32 = 0, VG_F16 = 1, VG_BF16 = 2 };
+
+/* A device tensor [tokens][num_heads][dim] with the last dimension contiguous
+ * and the other two strided (in elements; 0 = broadcast, inputs only).  Any
+ * element-aligned address and stride works; multiples of 16 bytes are faster. */
+typedef struct vg_heads {
+  void *data;
+  uint64_t num_heads;
+  int64_t token_stride, head_stride;
+} vg_heads;
+
+/* Rotary positions.  Frequency i of dim/2 is base^(-2i/dim), then
+ *   VG_ROTARY_PLAIN     unchanged
+ *   VG_ROTARY_LINEAR    divided by factor
+ *   VG_ROTARY_BY_PARTS  f (g + (1 - g) / factor) with g rising linearly from
+ *                       0 to 1 as the turns original_length f / (2 pi) go
+ *                       from low_turns to high_turns
+ * Pairs are (i, i + dim/2), or (2i, 2i + 1) when interleaved. */
+enum { VG_ROTARY_PLAIN = 0, VG_ROTARY_LINEAR = 1, VG_ROTARY_BY_PARTS = 2 };
+typedef struct vg_rotary_params {
+  uint64_t dim;        /* rotated dimensions: even, 2..256 */
+  int32_t interleaved; /* 0: halves, 1: adjacent pairs */
+  int32_t scaling;     /* VG_ROTARY_* */
+  double base;         /* > 1, e.g. 10000 */
+  double factor;       /* >= 1 (VG_ROTARY_LINEAR, VG_ROTARY_BY_PARTS) */
+  double original_length, low_turns, high_turns; /* VG_ROTARY_BY_PARTS */
+  double magnitude;    /* every rotated pair is multiplied by it; usually 1 */
+} vg_rotary_params;
+typedef struct vg_rotary vg_rotary;
+
+/* A table of frequencies (host memory only). */
+int vg_rotary_create(const vg_rotary_params *params, vg_rotary **out);
+int vg_rotary_destroy(vg_rotary *r);
+/* The dim/2 frequencies, in radians per position. */
+int vg_rotary_frequencies(const vg_rotary *r, double *out);
+
+/* Rotate q and k (k nullable, with k_out) of `tokens` tokens at the given
+ * positions (device, int64): (a, b) -> m (a cos t - b sin t, a sin t + b cos t),
+ * t = position * frequency, reduced in 64 bits, the rest in f32, rounded once.
+ * Head dimensions from dim on are copied.  transpose: -sin, the transposed
+ * map, which takes the gradient of the outputs to that of the inputs.  An
+ * output is its input (same address and strides: in place) or does not
+ * overlap any other tensor.  Can be captured into a CUDA graph. */
+int vg_rotary_apply(const vg_rotary *r, int dtype, size_t head_dim, const int64_t *positions, size_t tokens,
+                    const vg_heads *q, const vg_heads *q_out, const vg_heads *k, const vg_heads *k_out,
+                    int transpose, int device, void *stream);
+
+typedef struct vg_kv_params {
+  uint64_t num_seqs;     /* sequences held */
+  uint64_t capacity;     /* tokens per sequence, at most 2^30 */
+  uint64_t num_kv_heads; /* at most 65535 */
+  uint64_t head_dim;     /* 32, 64, 96 or 128 */
+  uint64_t block_tokens; /* tokens that share a scale: 16, 32, 64 or 128 */
+} vg_kv_params;
+typedef struct vg_kv_info {
+  uint64_t num_seqs, capacity, num_kv_heads, head_dim, block_tokens;
+  uint64_t weight_stride; /* tokens between two (sequence, head) rows of the weights */
+  uint64_t device_bytes;
+  int32_t device, reserved;
+} vg_kv_info;
+typedef struct vg_kv_cache vg_kv_cache;
+
+/* An empty cache: 2 (head_dim + 4 / block_tokens) + 4 bytes per token, head
+ * and sequence of capacity. */
+int vg_kv_create(const vg_kv_params *params, int device, vg_kv_cache **out);
+int vg_kv_destroy(vg_kv_cache *kv);
+int vg_kv_get_info(const vg_kv_cache *kv, vg_kv_info *out);
+/* Tokens held by each sequence, [num_seqs]. */
+int vg_kv_lengths(const vg_kv_cache *kv, uint32_t *out);
+/* Drop the tokens of every sequence from lengths[s] on (at most the present
+ * length; 0 empties it).  Host only: no device work. */
+int vg_kv_truncate(vg_kv_cache *kv, const uint32_t *lengths);
+/* The accumulated weights, device f32 [num_seqs][num_kv_heads][weight_stride],
+ * owned by the cache. */
+int vg_kv_weights(const vg_kv_cache *kv, float **out);
+
+/* Append counts[s] tokens to every sequence s; k and v hold all sequences'
+ * tokens one after another, in sequence order.  A block's scale is the
+ * smallest power of two in [2^-100, 2^120] with 127 scale >= |x| for every x it was
+ * given; codes are round-half-even(x / scale), clamped to +-127.  While a
+ * block fills up its scale only grows, and its codes are then rounded to the
+ * new one.  A block given a value that is not finite reads as NaN from then
+ * on.  Weights of the new tokens are 0.  VG_ERR_INVALID_PARAMETER, with
+ * nothing appended, when a sequence would pass the capacity. */
+int vg_kv_append(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_heads *k, const vg_heads *v,
+                 void *stream);
+
+/* Attention of counts[s] queries per sequence s (packed as in vg_kv_append)
+ * over its cached tokens.  q.num_heads is a multiple g of num_kv_heads; query
+ * head h reads key/value head h / g.  Query j of n sees the first
+ * length - n + j + 1 tokens with VG_KV_CAUSAL (the queries are the last
+ * tokens appended), every token without; a query that sees none gives 0 and
+ * an lse of -inf.  out = softmax(scale q.K) V in `dtype` (VG_F16 or VG_BF16),
+ * lse (nullable, f32 [queries][q heads], contiguous) the natural log of the
+ * softmax's denominator.  VG_KV_ACCUMULATE adds to every cached token's
+ * weight (per key/value head) its probabilities summed over the call's
+ * queries and the heads that share it.  Results do not depend on the call's
+ * other sequences' contents, and are the same in every run. */
+enum { VG_KV_CAUSAL = 1, VG_KV_ACCUMULATE = 2 };
+int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_heads *q, const vg_heads *out,
+                 float *lse, float scale, int flags, void *stream);
+
+/* Cut sequence src[i] down to `budget` tokens into sequence dst[i] (i < n),
+ * replacing what dst[i] held; src[i] stays as it is.  Per head the `recent`
+ * (at most budget) newest tokens are kept, and of the others those of largest
+ * accumulated weight (ties: the older token), in their order; a sequence of
+ * at most budget tokens is copied.  A block of dst takes the largest scale of
+ * its tokens; codes of smaller scales are rounded to it.  kept (nullable,
+ * device i32 [n][num_kv_heads][budget]) gets the token's place in src, -1
+ * past the end; weights move along and are 0 up to `budget`.  No sequence
+ * may appear twice among src and dst. */
+int vg_kv_evict(vg_kv_cache *kv, size_t n, const uint32_t *src, const uint32_t *dst, size_t budget, size_t recent,
+                int32_t *kept, void *stream);
+
+/* The values (code * scale) of tokens [starts[s], starts[s] + counts[s]) of
+ * every sequence, packed in sequence order into k and v in `dtype`. */
+int vg_kv_read(vg_kv_cache *kv, const uint32_t *starts, const uint32_t *counts, int dtype, const vg_heads *k,
+               const vg_heads *v, void *stream);
+
+/* Set or copy out a whole sequence: codes int8 [num_kv_heads][length][head_dim],
+ * scales f32 [num_kv_heads][ceil(length / block_tokens)], weights (nullable)
+ * f32 [num_kv_heads][length]; host or device memory, contiguous.  `length`
+ * of an export is the sequence's.  Scales are powers of two (or NaN).  These
+ * return when the copy is done. */
+int vg_kv_load(vg_kv_cache *kv, size_t seq, size_t length, const int8_t *k_codes, const float *k_scales,
+               const int8_t *v_codes, const float *v_scales, const float *weights, void *stream);
+int vg_kv_export(vg_kv_cache *kv, size_t seq, int8_t *k_codes, float *k_scales, int8_t *v_codes, float *v_scales,
+                 float *weights, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

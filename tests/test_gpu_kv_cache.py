@@ -1,0 +1,608 @@
+"""Rotary positions and the 8-bit key/value cache on the GPU against the plain
+64-bit restatement in oracle/kv_cache.py.
+
+Stored codes, scales and evictions are exact (power-of-two scales), so they
+are compared bit for bit.  Bounds of the rest, with u = 2^-24 and u_out the
+output type's unit roundoff:
+  rotary     |err| <= u_out |out| + 8 u m (|a| + |b|): angle rounded to f32 as a
+             fraction of a turn, sine and cosine to 2 ulp, three roundings
+  scores     |err| <= e = (d + 16) u S, S = scale sum |q_i k_i|: f32 sums of exact
+             products in any order, one rounding of the factor
+  lse        |err| <= e + 16 u (1 + |lse|)
+  weights    |err| <= (2 e + 32 u (1 + |lse|)) w
+  out        |err| <= 1.01 u_out |out| + (2^-11 + 2 e + 32 u (1 + |lse|)) sum p |v| + n 2^-36 max |v|:
+             probabilities rounded to binary16 (2^-12, doubled), those of n tokens
+             below its range, 2^-38 of the largest, to 0
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from oracle import kv_cache as ref
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+U = 2.0 ** -24
+ROUND = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # bf16: 8 significant bits
+
+
+def _types():
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _rand(g, *shape, dtype="f32", scale=1.0):
+    x = torch.from_numpy((g.standard_normal(shape) * scale).astype(np.float32)).to(_types()[dtype])
+    return x.cuda()
+
+
+def _np(x):
+    return x.detach().double().cpu().numpy()
+
+
+# ---- rotary -----------------------------------------------------------------
+
+
+def _rotary_bound(x, want, freq, interleaved, m, dtype):
+    r = 2 * len(freq)
+    size, pairs = np.zeros_like(want), np.abs(_np(x))
+    ia, ib = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2), slice(r // 2, r))
+    size[..., ia] = size[..., ib] = pairs[..., ia] + pairs[..., ib]
+    tiny = 2.0 ** -25 if dtype == "f16" else 0.0  # half the smallest binary16
+    return 1.01 * ROUND[dtype] * np.abs(want) + 8 * U * m * size + tiny
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("tokens,hq,hk,d,rot", [(1, 1, 1, 32, 32), (5, 8, 2, 128, 128), (33, 3, 1, 96, 64),
+                                                (700, 12, 4, 64, 64), (7, 2, 2, 100, 50), (9, 1, 3, 10, 2),
+                                                (3, 2, 1, 256, 256)])
+def test_rotary(tokens, hq, hk, d, rot, layout, dtype):
+    from vicinity_b200 import Rotary
+
+    g = np.random.default_rng(tokens + d)
+    pos = g.integers(0, 1 << 20, tokens)
+    pos[0] = 0
+    pos[-1] = (1 << 31) + 5 if tokens > 1 else 0
+    q, k = _rand(g, tokens, hq, d, dtype=dtype), _rand(g, tokens, hk, d, dtype=dtype)
+    scaled = dict(scaling="by_parts", factor=8.0, original_length=4096.0, magnitude=1.25)
+    r = Rotary(rot, base=500.0, layout=layout, **scaled)
+    freq = ref.rotary_frequencies(rot, 500.0, "by_parts", 8.0, 4096.0)
+    assert np.allclose(r.frequencies(), freq, rtol=1e-14)
+    p = torch.from_numpy(pos).cuda()
+    for transpose in (False, True):
+        oq, ok = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+        r.apply(p, q, k, out_q=oq, out_k=ok, transpose=transpose)
+        for x, got in ((q, oq), (k, ok)):
+            want = ref.rotary(_np(x), pos, r.frequencies(), layout == "interleaved", 1.25, transpose)
+            err = np.abs(_np(got) - want)
+            assert (err <= _rotary_bound(x, want, freq, layout == "interleaved", 1.25, dtype)).all(), err.max()
+        # in place, and one tensor alone
+        qi = q.clone()
+        r.apply(p, qi, transpose=transpose)
+        assert torch.equal(qi, oq)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_strides_and_alignment(layout):
+    # head-major storage, an odd first element, a broadcast input: the same as contiguous copies
+    from vicinity_b200 import Rotary
+
+    g = np.random.default_rng(3)
+    t, h, d = 19, 4, 64
+    r = Rotary(d, layout=layout, scaling="linear", factor=2.0)
+    pos = torch.arange(100, 100 + t).cuda()
+    base = _rand(g, h, t, d, dtype="bf16").transpose(0, 1)
+    flat = _rand(g, t * h * d + 1, dtype="bf16")
+    odd = flat[1:].view(t, h, d)
+    wide = _rand(g, t, 1, d, dtype="bf16").expand(t, h, d)
+    for x in (base, odd, wide):
+        want, got = torch.empty(t, h, d, dtype=x.dtype, device="cuda"), torch.empty(h, t, d, dtype=x.dtype, device="cuda")
+        r.apply(pos, x.contiguous(), out_q=want)
+        r.apply(pos, x, out_q=got.transpose(0, 1))
+        assert torch.equal(got.transpose(0, 1), want)
+
+
+def test_rotary_gradient():
+    # the transposed map against differences of the map in 64 bits, and as the
+    # adjoint: <R x, y> = <x, R^T y>
+    from vicinity_b200 import Rotary
+
+    g = np.random.default_rng(8)
+    t, h, d, rot = 6, 2, 24, 16
+    r = Rotary(rot, layout="interleaved", magnitude=0.75)
+    pos = np.array([0, 1, 17, 300, 4000, 70000])
+    x, y = g.standard_normal((t, h, d)), g.standard_normal((t, h, d)).astype(np.float32)
+    dx = torch.empty(t, h, d, device="cuda")
+    r.apply(torch.from_numpy(pos).cuda(), torch.from_numpy(y).cuda(), out_q=dx, transpose=True)
+    freq, eps = r.frequencies(), 1e-3
+    for i in ((0, 0, 3), (2, 1, 0), (3, 1, 15), (5, 0, 8), (4, 1, 20)):
+        up, down = x.copy(), x.copy()
+        up[i] += eps
+        down[i] -= eps
+        f = [(ref.rotary(z, pos, freq, True, 0.75) * y).sum() for z in (up, down)]
+        # linear map: the difference quotient is exact up to rounding (~1e-11)
+        assert abs((f[0] - f[1]) / (2 * eps) - float(dx[i])) <= 1e-9 + 8 * U * 0.75 * 2 * np.abs(y).max()
+
+
+def test_rotary_in_a_captured_graph_and_on_a_stream():
+    from vicinity_b200 import Rotary
+
+    g = np.random.default_rng(4)
+    q = _rand(g, 8, 2, 32, dtype="f16")
+    pos, out, want = torch.arange(8).cuda(), torch.empty_like(q), torch.empty_like(q)
+    r = Rotary(32)
+    r.apply(pos, q, out_q=want)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        r.apply(pos, q, out_q=out, stream=torch.cuda.current_stream().cuda_stream)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+# ---- cache ------------------------------------------------------------------
+
+
+class Mirror:
+    """A KVCache and its restatement, driven together."""
+
+    def __init__(self, seqs, capacity, heads, d, block):
+        from vicinity_b200 import KVCache
+
+        self.cache = KVCache(seqs, capacity, heads, d, block_tokens=block)
+        self.heads, self.d, self.block, self.seqs = heads, d, block, seqs
+        self.k = [[ref.Head(d, block) for _ in range(heads)] for _ in range(seqs)]
+        self.v = [[ref.Head(d, block) for _ in range(heads)] for _ in range(seqs)]
+        self.w = [[np.zeros(0) for _ in range(heads)] for _ in range(seqs)]
+
+    def append(self, counts, k, v, stream=None):
+        self.cache.append(k, v, counts, stream=stream)
+        kn, vn, row = _np(k), _np(v), 0
+        for s, c in enumerate(counts):
+            for h in range(self.heads):
+                self.k[s][h].append(kn[row:row + c, h])
+                self.v[s][h].append(vn[row:row + c, h])
+                self.w[s][h] = np.concatenate([self.w[s][h], np.zeros(c)])
+            row += c
+
+    def fill(self, g, counts, dtype="bf16", scale=1.0):
+        n = sum(counts)
+        self.append(counts, _rand(g, n, self.heads, self.d, dtype=dtype, scale=scale),
+                    _rand(g, n, self.heads, self.d, dtype=dtype, scale=scale))
+
+    def truncate(self, lengths):
+        self.cache.truncate(lengths)
+        for s, n in enumerate(lengths):
+            for h in range(self.heads):
+                self.k[s][h].truncate(n)
+                self.v[s][h].truncate(n)
+                self.w[s][h] = self.w[s][h][:n]
+
+    def check(self):
+        torch.cuda.synchronize()
+        assert self.cache.lengths.tolist() == [len(h[0]) for h in self.k]
+        for s in range(self.seqs):
+            kc, ks, vc, vs, _ = self.cache.export(s)
+            for h in range(self.heads):
+                for codes, scales, want in ((kc, ks, self.k[s][h]), (vc, vs, self.v[s][h])):
+                    assert np.array_equal(scales[h], want.scales, equal_nan=True), (s, h)
+                    sound = ~np.isnan(np.repeat(want.scales, self.block)[:len(want)])
+                    assert np.array_equal(codes[h][sound], want.codes[sound]), (s, h)
+
+    def attend(self, counts, q, dtype, scale=None, causal=True, accumulate=False, out=None, stream=None):
+        n, hq = q.shape[0], q.shape[1]
+        g = hq // self.heads
+        out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda") if out is None else out
+        lse = torch.full((n, hq), 7.0, device="cuda")
+        self.cache.attend(q, counts, out, lse=lse, scale=scale, causal=causal, accumulate=accumulate, stream=stream)
+        torch.cuda.synchronize()
+        scale = self.d ** -0.5 if scale is None else scale
+        qn, on, ln, row = _np(q), _np(out), _np(lse), 0
+        weights = torch.as_tensor(self.cache.weights, device="cuda").double().cpu().numpy()
+        for s, c in enumerate(counts):
+            for h in range(self.heads if c else 0):
+                heads = slice(h * g, (h + 1) * g)
+                o, want_lse, w, size, top = ref.attention(qn[row:row + c, heads], self.k[s][h].values(),
+                                                          self.v[s][h].values(), c, scale, causal)
+                e = (self.d + 16) * U * top
+                soft = np.where(np.isfinite(want_lse), np.abs(want_lse), 0.0)
+                got, got_lse = on[row:row + c, heads], ln[row:row + c, heads]
+                fine = np.isfinite(want_lse)
+                assert np.array_equal(np.isnan(want_lse), np.isnan(got_lse))
+                assert np.array_equal(want_lse == -np.inf, got_lse == -np.inf)
+                err = np.abs(got_lse[fine] - want_lse[fine])
+                assert (err <= (e + 16 * U * (1 + soft))[fine]).all(), (s, h, err.max())
+                tol = 1.01 * ROUND[dtype] * np.abs(o) + (2.0 ** -11 + 2 * e + 32 * U * (1 + soft))[..., None] * size
+                tol += 2.0 ** -24 if dtype == "f16" else 0.0
+                tol += len(self.v[s][h]) * 2.0 ** -36 * np.nan_to_num(np.abs(self.v[s][h].values())).max(initial=0.0)
+                assert np.array_equal(np.isnan(o), np.isnan(got)), (s, h)
+                ok = ~np.isnan(o)
+                assert (np.abs(got - o)[ok] <= tol[ok]).all(), (s, h, np.nanmax(np.abs(got - o) / (tol + 1e-300)))
+                assert (got[want_lse == -np.inf] == 0).all()
+                if accumulate:
+                    rel = (2 * e + 32 * U * (1 + soft))[fine].max(initial=0.0)
+                    old, now = self.w[s][h], weights[s, h, :len(self.w[s][h])]
+                    assert np.array_equal(np.isnan(old + w), np.isnan(now)), (s, h)
+                    err = np.nan_to_num(np.abs(now - (old + w)))
+                    assert (err <= np.nan_to_num(rel * w + 4 * U * (old + w)) + 1e-12).all(), (s, h, err.max())
+                    # later steps and evictions start from what the cache holds
+                    self.w[s][h] = now.copy()
+            row += c
+        return out
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_append_and_read(block, d, dtype):
+    g = np.random.default_rng(block + d)
+    m = Mirror(4, 333, 3, d, block)
+    for step, counts in enumerate([[1, 0, 17, 200], [1, 0, block - 1, 1], [block, 0, 1, 3], [0, 0, 0, 0], [40, 0, 2, 129]]):
+        # growing magnitudes make the scales of blocks with tokens grow
+        m.fill(g, counts, dtype, scale=2.0 ** (step % 3) * 0.7)
+    m.check()
+    starts, counts = [0, 0, 5, 100], [43, 0, 1, 233]
+    n = sum(counts)
+    k, v = (torch.full((n, 3, d), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    m.cache.read(starts, counts, k, v)
+    row = 0
+    for s, c in enumerate(counts):
+        for h in range(3):
+            assert np.array_equal(_np(k)[row:row + c, h], m.k[s][h].values()[starts[s]:starts[s] + c])
+            assert np.array_equal(_np(v)[row:row + c, h], m.v[s][h].values()[starts[s]:starts[s] + c])
+        row += c
+
+
+def test_append_edges_of_the_scales():
+    # zeros, the powers of two where the scale steps, subnormals, the largest
+    # floats, infinities and NaN, each in a block of its own
+    rows = [[0.0], [127.0], [127.0 * (1 + 2.0 ** -20)], [128.0], [2.0 ** -140], [3.0e38, -3.4e38], [math.inf], [math.nan],
+            [1.0, -1.0], [0.5, 1.5, 2.5, 127.0, -0.5, -1.5, -2.5]]
+    x = np.zeros((16 * len(rows), 1, 32), np.float32)
+    for i, r in enumerate(rows):
+        x[16 * i, 0, :len(r)] = r
+    m = Mirror(1, 16 * len(rows) + 16, 1, 32, 16)
+    t = torch.from_numpy(x).cuda()
+    m.append([x.shape[0]], t, t.clone())
+    m.check()
+    # a block that was given NaN stays NaN until it starts afresh
+    m.append([1], torch.full((1, 1, 32), math.nan, device="cuda"), torch.ones(1, 1, 32, device="cuda"))
+    m.append([1], torch.ones(1, 1, 32, device="cuda"), torch.ones(1, 1, 32, device="cuda"))
+    m.check()
+    m.truncate([x.shape[0]])
+    m.append([3], torch.ones(3, 1, 32, device="cuda"), torch.ones(3, 1, 32, device="cuda"))
+    m.check()
+
+
+def test_append_strided_broadcast_and_unaligned():
+    g = np.random.default_rng(5)
+    for dtype in ("f32", "bf16"):
+        m = Mirror(2, 100, 4, 64, 32)
+        k = _rand(g, 4, 70, 64, dtype=dtype).transpose(0, 1)           # head-major
+        v = _rand(g, 70, 1, 64, dtype=dtype).expand(70, 4, 64)         # one head for all
+        m.append([30, 40], k, v)
+        flat = _rand(g, 20 * 4 * 65 + 1, dtype=dtype)
+        odd = flat[1:].view(20, 4, 65)[..., :64]                       # rows that start anywhere
+        m.append([20, 0], odd, odd)
+        m.check()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d,block,heads,group", [(32, 16, 1, 1), (64, 32, 2, 4), (96, 64, 3, 7), (128, 128, 2, 8),
+                                                 (128, 64, 1, 33), (64, 16, 5, 2)])
+def test_attend_single_tokens(d, block, heads, group, dtype):
+    g = np.random.default_rng(d + group)
+    m = Mirror(6, 700, heads, d, block)
+    m.fill(g, [1, 0, 15, 129, 700, 300], scale=1.5)
+    q = _rand(g, 6, heads * group, d, dtype=dtype, scale=2.0)
+    m.attend([1] * 6, q, dtype, accumulate=True)
+    m.attend([1] * 6, q, dtype, accumulate=True, scale=0.03)  # weights add up
+    m.attend([0, 0, 1, 0, 1, 0], q[:2], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d,block,heads,group,counts", [
+    (64, 32, 2, 2, [3, 2, 0, 5]), (128, 64, 1, 4, [40, 1, 33, 0]), (96, 16, 2, 3, [129, 0, 64, 7]),
+    (32, 128, 1, 8, [17, 16, 15, 1]), (128, 32, 2, 1, [257, 3, 0, 130])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_several_tokens(d, block, heads, group, counts, causal, dtype):
+    g = np.random.default_rng(d + group + sum(counts))
+    m = Mirror(4, 640, heads, d, block)
+    m.fill(g, [300, 2, 64, 0])        # the last sequence is empty but for its own queries
+    m.fill(g, counts)
+    q = _rand(g, sum(counts), heads * group, d, dtype=dtype, scale=2.0)
+    m.attend(counts, q, dtype, causal=causal, accumulate=True)
+
+
+def test_attend_rows_that_see_nothing():
+    # more queries than tokens: the first ones see none; an empty sequence
+    g = np.random.default_rng(2)
+    for counts in ([20, 3, 1], [150, 1, 140], [1, 300, 1]):
+        m = Mirror(3, 256, 2, 64, 16)
+        m.fill(g, [7, 0, 130])
+        q = _rand(g, sum(counts), 4, 64, dtype="bf16")
+        m.attend(counts, q, "bf16", accumulate=True)
+        m.attend(counts, q, "bf16", causal=False)
+
+
+def test_attend_does_not_see_what_is_masked():
+    # blocks that read as NaN, and stale tokens past a truncation, reach no
+    # query that does not see them
+    g = np.random.default_rng(6)
+    for counts in ([2, 1], [40, 33]):
+        m = Mirror(2, 256, 1, 64, 16)
+        m.fill(g, [100, 96])
+        bad = torch.full((60, 1, 64), math.nan, device="cuda")
+        m.append([30, 30], bad, bad)     # the first sequence's last block has 4 older tokens: they read as NaN
+        m.truncate([100, 96])
+        q = _rand(g, sum(counts), 2, 64, dtype="bf16")
+        m.attend(counts, q, "bf16", accumulate=True)
+        # ... and every query that sees them is NaN
+        m.append([0, 16], bad[:16], bad[:16])
+        m.attend([0, counts[1]], q[:counts[1]], "bf16")
+
+
+def test_attend_scores_far_apart():
+    # huge scores (one token takes all), equal scores, negative and zero scale
+    g = np.random.default_rng(7)
+    for n in (1, 48):
+        m = Mirror(1, 400, 2, 128, 64)
+        m.fill(g, [333], scale=8.0)
+        q = _rand(g, n, 4, 128, dtype="bf16", scale=8.0)
+        for scale in (1.0, -0.05, 0.0):
+            m.attend([n], q, "bf16", scale=scale, accumulate=True)
+        m.attend([n], q * 0, "bf16")
+        # values and keys of very different magnitudes from block to block
+        m.fill(g, [60], scale=2.0 ** -30)
+        m.fill(g, [3], scale=2.0 ** 20)
+        m.attend([n], (q.float() * 2.0 ** -24).to(q.dtype), "bf16")
+
+
+def test_attend_strides_and_streams():
+    g = np.random.default_rng(9)
+    m = Mirror(2, 300, 2, 64, 32)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    m.fill(g, [200, 131])
+    for n in (1, 20):
+        q = _rand(g, 4, 2 * n, 64, dtype="bf16").transpose(0, 1)
+        out = torch.empty(4, 2 * n, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+        torch.cuda.synchronize()
+        m.attend([n, n], q, "bf16", out=out, stream=s.cuda_stream)
+        flat = _rand(g, 2 * n * 4 * 67 + 1, dtype="f16")
+        odd = flat[1:].view(2 * n, 4, 67)[..., 1:65]
+        m.attend([n, n], odd, "f16", accumulate=True)
+
+
+def test_attend_is_the_same_in_every_run_and_ordered_across_streams():
+    g = np.random.default_rng(10)
+    m = Mirror(3, 4000, 2, 128, 64)
+    m.fill(g, [4000, 1, 777])
+    for n in (1, 100):
+        q = _rand(g, 3 * n, 8, 128, dtype="bf16")
+        out = [torch.empty_like(q) for _ in range(4)]
+        streams = [torch.cuda.Stream() for _ in out]
+        torch.cuda.synchronize()
+        for o, st in zip(out, streams):
+            m.cache.attend(q, [n] * 3, o, accumulate=True, stream=st.cuda_stream)
+        torch.cuda.synchronize()
+        for o in out[1:]:
+            assert torch.equal(o, out[0])
+
+
+def test_long_sequence_offsets_past_32_bits():
+    # the last sequence's codes lie beyond 4 GiB: [17][2][1_100_032][128]
+    from vicinity_b200 import KVCache
+
+    cap, d = 1_100_000, 128
+    cache = KVCache(17, cap, 2, d, block_tokens=64)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = cap - 3
+    k = torch.randn(n, 2, d, generator=g, device="cuda", dtype=torch.float32).to(torch.bfloat16)
+    v = torch.randn(n, 2, d, generator=g, device="cuda", dtype=torch.float32).to(torch.bfloat16)
+    counts = [0] * 16 + [n]
+    cache.append(k, v, counts)
+    kr, vr = torch.empty(500, 2, d, dtype=torch.bfloat16, device="cuda"), torch.empty(500, 2, d, dtype=torch.bfloat16, device="cuda")
+    cache.read([0] * 16 + [n - 500], [0] * 16 + [500], kr, vr)
+    tail = ref.Head(d, 64)
+    first = (n - 500) // 64 * 64
+    tail.append(_np(k[first:, 1]))
+    assert np.array_equal(_np(kr[:, 1]), tail.values()[n - 500 - first:])
+    q = torch.randn(1, 4, d, generator=g, device="cuda").to(torch.bfloat16)
+    out, lse = torch.empty_like(q), torch.empty(1, 4, device="cuda")
+    cache.attend(q, [0] * 16 + [1], out, lse=lse, accumulate=True)
+    # the same attention in 64 bits on the GPU, from the values read back
+    kk, vv = torch.empty(n, 2, d, dtype=torch.bfloat16, device="cuda"), torch.empty(n, 2, d, dtype=torch.bfloat16, device="cuda")
+    cache.read([0] * 17, counts, kk, vv)
+    for h in range(4):
+        s = (kk[:, h // 2].double() @ q[0, h].double()) / math.sqrt(d)
+        p = torch.softmax(s, 0)
+        o = p @ vv[:, h // 2].double()
+        size = p @ vv[:, h // 2].double().abs()
+        assert abs(float(lse[0, h]) - float(torch.logsumexp(s, 0))) <= 1e-4
+        assert ((out[0, h].double() - o).abs() <= 1.01 * 2.0 ** -8 * o.abs() + (2.0 ** -11 + 1e-4) * size).all()
+    w = torch.as_tensor(cache.weights, device="cuda")
+    assert abs(float(w[16].double().sum()) - 4.0) <= 1e-3 and float(w[:16].abs().sum()) == 0.0
+
+
+# ---- eviction ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("d,block,heads", [(32, 16, 1), (64, 64, 3), (96, 32, 2), (128, 128, 2)])
+@pytest.mark.parametrize("budget,recent", [(1, 0), (1, 1), (100, 0), (100, 33), (257, 257), (900, 5)])
+def test_evict(budget, recent, d, block, heads):
+    g = np.random.default_rng(budget + d)
+    lens = [0, 1, budget, min(budget + 1, 900), 900]
+    n = len(lens)
+    m = Mirror(2 * n, 900, heads, d, block)
+    for part in range(3):  # blocks of different scales
+        m.fill(g, [(x * (part + 1)) // 3 - (x * part) // 3 for x in lens] + [0] * n, scale=3.0 ** part)
+    m.fill(g, [0] * n + [37] * n)  # what the destinations held is replaced
+    weights = torch.as_tensor(m.cache.weights, device="cuda")
+    w = torch.from_numpy(g.exponential(size=(n, heads, 900)).astype(np.float32))
+    w[torch.from_numpy(g.random((n, heads, 900)) < 0.4)] = 0.0   # many ties
+    w[:, :, ::7] = 1.5
+    weights[:n] = w.cuda()
+    kept = torch.full((n, heads, budget), 7, dtype=torch.int32, device="cuda")
+    m.cache.evict(list(range(n)), list(range(n, 2 * n)), budget, recent, kept=kept)
+    torch.cuda.synchronize()
+    for s, length in enumerate(lens):
+        for h in range(heads):
+            at = ref.keep(w[s, h].numpy(), length, budget, recent)
+            assert np.array_equal(kept[s, h].cpu().numpy(), np.pad(at, (0, budget - len(at)), constant_values=-1))
+            m.k[n + s][h], m.v[n + s][h] = m.k[s][h].kept(at), m.v[s][h].kept(at)
+            want = np.pad(w[s, h].numpy()[at], (0, budget - len(at)))
+            assert np.array_equal(weights[n + s, h, :budget].cpu().numpy(), want)
+    m.check()
+    # what is left is attended to and appended to
+    m.fill(g, [0] * n + [min(2, 900 - min(x, budget)) for x in lens])
+    q = _rand(g, n, heads, d, dtype="bf16")
+    m.attend([0] * n + [1] * n, q, "bf16")
+
+
+def test_evict_long_rows_and_special_weights():
+    g = np.random.default_rng(12)
+    m = Mirror(2, 40_000, 2, 32, 64)
+    m.fill(g, [40_000, 0])
+    weights = torch.as_tensor(m.cache.weights, device="cuda")
+    w = g.random((2, 40_000)).astype(np.float32)
+    w[0] = 0.25                                # all equal: the oldest stay
+    w[1, 1000:3000] = np.inf
+    w[1, 3000] = np.nan                        # counts as the largest
+    w[1, 5000:9000] = 1e-42                    # subnormals keep their order
+    w[1, 9000:30_000] = -0.0                   # as 0
+    weights[0, :, :40_000] = torch.from_numpy(w).cuda()
+    for budget, recent in ((5_000, 100), (39_999, 0), (2_500, 2_400)):
+        kept = torch.empty(1, 2, budget, dtype=torch.int32, device="cuda")
+        m.cache.evict([0], [1], budget, recent, kept=kept)
+        order = np.where(np.isnan(w), np.inf, w).astype(np.float64)
+        order[np.isnan(w)] = 1e308
+        order[np.isinf(w)] = 1e307
+        for h in range(2):
+            assert np.array_equal(kept[0, h].cpu().numpy(), ref.keep(order[h], 40_000, budget, recent))
+
+
+def test_evict_poisoned_blocks():
+    g = np.random.default_rng(13)
+    m = Mirror(2, 128, 1, 32, 16)
+    m.fill(g, [40, 0])
+    bad = torch.full((1, 1, 32), math.inf, device="cuda")
+    m.append([1, 0], bad, torch.ones_like(bad))
+    m.fill(g, [40, 0])
+    m.cache.evict([0], [1], 30, 10)
+    at = ref.keep(np.zeros(81), 81, 30, 10)
+    m.k[1][0], m.v[1][0] = m.k[0][0].kept(at), m.v[0][0].kept(at)
+    m.check()
+
+
+# ---- whole sequences ---------------------------------------------------------
+
+
+def test_load_and_export_round_trip():
+    from vicinity_b200 import KVCache
+
+    g = np.random.default_rng(14)
+    m = Mirror(3, 200, 2, 96, 32)
+    m.fill(g, [150, 0, 31])
+    m.attend([1, 0, 1], _rand(g, 2, 4, 96, dtype="bf16"), "bf16", accumulate=True)
+    other = KVCache(4, 333, 2, 96, block_tokens=32)
+    for s in range(3):
+        state = m.cache.export(s)
+        if state[0].shape[1]:
+            other.load(3 - s, *state)                                           # host arrays
+            other.load(3 - s, *[torch.from_numpy(a).cuda() for a in state])     # device arrays
+            for a, b in zip(state, other.export(3 - s)):
+                assert np.array_equal(a, b)
+    assert other.lengths.tolist() == [0, 31, 0, 150]
+
+
+# ---- refusals ----------------------------------------------------------------
+
+
+def test_refusals():
+    from vicinity_b200 import KVCache, Rotary
+
+    c = KVCache(2, 100, 2, 64, block_tokens=16)
+    bf = dict(dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(5, 2, 64, **bf)
+    q = torch.zeros(5, 4, 64, **bf)
+    with pytest.raises(ValueError, match="capacity"):
+        c.append(torch.zeros(101, 2, 64, **bf), torch.zeros(101, 2, 64, **bf), [101, 0])
+    assert c.lengths.tolist() == [0, 0]
+    with pytest.raises(ValueError, match="one entry"):
+        c.append(k, k, [5])
+    with pytest.raises(ValueError, match="must not be negative"):
+        c.append(k, k, [6, -1])
+    with pytest.raises(ValueError, match=r"k must be \[4"):
+        c.append(k, k, [4, 0])
+    with pytest.raises(ValueError, match="key/value heads"):
+        c.append(torch.zeros(5, 1, 64, **bf), torch.zeros(5, 1, 64, **bf), [5, 0])
+    with pytest.raises(ValueError, match="element type"):
+        c.append(k, k.half(), [5, 0])
+    with pytest.raises(ValueError, match="device memory"):
+        c.append(k.cpu(), k.cpu(), [5, 0])
+    with pytest.raises(ValueError, match="contiguous in its last"):
+        c.append(torch.zeros(5, 2, 128, **bf)[..., ::2], k, [5, 0])
+    c.append(k, k, [5, 0])
+    with pytest.raises(ValueError, match="truncated"):
+        c.truncate([6, 0])
+    with pytest.raises(ValueError, match="multiple"):
+        c.attend(torch.zeros(1, 3, 64, **bf), [1, 0], torch.zeros(1, 3, 64, **bf))
+    with pytest.raises(ValueError, match="unsupported"):
+        c.attend(q.float(), [5, 0], q.float())
+    with pytest.raises(ValueError, match="heads of q"):
+        c.attend(q, [5, 0], torch.zeros(5, 2, 64, **bf))
+    with pytest.raises(ValueError, match="must not overlap"):
+        c.attend(q, [5, 0], torch.zeros(5, 1, 64, **bf).expand(5, 4, 64))
+    with pytest.raises(ValueError, match="finite"):
+        c.attend(q, [5, 0], q.clone(), scale=math.inf)
+    with pytest.raises(ValueError, match="lse"):
+        c.attend(q, [5, 0], q.clone(), lse=torch.zeros(5, 3, device="cuda"))
+    with pytest.raises(ValueError, match="twice"):
+        c.evict([0], [0], 4, 1)
+    with pytest.raises(ValueError, match="budget"):
+        c.evict([0], [1], 101, 1)
+    with pytest.raises(ValueError, match="recent"):
+        c.evict([0], [1], 4, 5)
+    with pytest.raises(ValueError, match="below 2"):
+        c.evict([0], [2], 4, 1)
+    with pytest.raises(ValueError, match="holds only"):
+        c.read([3, 0], [3, 0], k[:3].clone(), k[:3].clone())
+    with pytest.raises(ValueError, match="kept"):
+        c.evict([0], [1], 4, 1, kept=torch.zeros(1, 2, 3, dtype=torch.int32, device="cuda"))
+    r = Rotary(32)
+    with pytest.raises(ValueError, match="at least the rotated"):
+        r.apply(torch.arange(5).cuda(), torch.zeros(5, 2, 16, **bf))
+    with pytest.raises(ValueError, match="int64"):
+        r.apply(torch.arange(5, dtype=torch.int32).cuda(), q)
+    with pytest.raises(ValueError, match="out_k without k"):
+        r.apply(torch.arange(5).cuda(), q, out_k=k)
+    with pytest.raises(ValueError, match="heads of its input"):
+        r.apply(torch.arange(5).cuda(), q, out_q=torch.zeros(5, 2, 64, **bf))
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="captured"):
+        with torch.cuda.graph(graph, stream=s):
+            c.attend(q, [5, 0], q.clone(), stream=torch.cuda.current_stream().cuda_stream)
+    # nothing above changed the cache
+    assert c.lengths.tolist() == [5, 0]
+
+
+def test_empty_calls():
+    from vicinity_b200 import KVCache, Rotary
+
+    c = KVCache(2, 100, 2, 64)
+    none = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    c.append(none, none, [0, 0])
+    c.attend(none, [0, 0], none)
+    c.read([0, 0], [0, 0], none, none)
+    c.evict([], [], 4, 1)
+    c.evict([0], [1], 4, 1)
+    Rotary(64).apply(torch.zeros(0, dtype=torch.int64, device="cuda"), none)
+    assert c.lengths.tolist() == [0, 0]

@@ -19,11 +19,14 @@ from .ivf_pq import (
     shard_assign_lists,
     verify_generation,
 )
+from .kv_cache import KVCache, Rotary
 
 __all__ = [
     "FlatIndex",
     "IVFPQFileSearcher",
     "IVFPQIndex",
+    "KVCache",
+    "Rotary",
     "current_generation",
     "MISSING_DISTANCE",
     "MISSING_LABEL",

@@ -27,6 +27,13 @@ VG_ERR_OUT_OF_MEMORY = -12
 VG_ERR_OTHER = -13
 VG_ERR_NOT_FOUND = -14
 
+F32, F16, BF16 = 0, 1, 2
+
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BY_PARTS = 0, 1, 2
+
+KV_CAUSAL = 1
+KV_ACCUMULATE = 2
+
 EXPORT_CENTROIDS = 0
 EXPORT_CODEBOOKS = 1
 EXPORT_ASSIGNMENTS = 2
@@ -109,9 +116,54 @@ class VgProfile(C.Structure):
     ]
 
 
+class VgHeads(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("num_heads", C.c_uint64),
+        ("token_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+    ]
+
+
+class VgRotaryParams(C.Structure):
+    _fields_ = [
+        ("dim", C.c_uint64),
+        ("interleaved", C.c_int32),
+        ("scaling", C.c_int32),
+        ("base", C.c_double),
+        ("factor", C.c_double),
+        ("original_length", C.c_double),
+        ("low_turns", C.c_double),
+        ("high_turns", C.c_double),
+        ("magnitude", C.c_double),
+    ]
+
+
+class VgKvParams(C.Structure):
+    _fields_ = [
+        (name, C.c_uint64) for name in ("num_seqs", "capacity", "num_kv_heads", "head_dim", "block_tokens")
+    ]
+
+
+class VgKvInfo(C.Structure):
+    _fields_ = [
+        (name, C.c_uint64)
+        for name in (
+            "num_seqs",
+            "capacity",
+            "num_kv_heads",
+            "head_dim",
+            "block_tokens",
+            "weight_stride",
+            "device_bytes",
+        )
+    ] + [("device", C.c_int32), ("reserved", C.c_int32)]
+
+
 _vp = C.c_void_p
 _sz = C.c_size_t
 _i = C.c_int
+_hp = C.POINTER(VgHeads)
 
 # name -> (restype, argtypes); every declaration of include/vicinity_gpu.h.
 SIGNATURES = {
@@ -156,6 +208,25 @@ SIGNATURES = {
     "vg_ivfpq_load_generation": (_i, [C.c_char_p, C.c_int, C.POINTER(_vp)]),
     "vg_generation_current": (_i, [C.c_char_p, C.c_char_p, _sz]),
     "vg_verify_generation": (_i, [C.c_char_p]),
+    "vg_rotary_create": (_i, [C.POINTER(VgRotaryParams), C.POINTER(_vp)]),
+    "vg_rotary_destroy": (_i, [_vp]),
+    "vg_rotary_frequencies": (_i, [_vp, _vp]),
+    "vg_rotary_apply": (
+        _i,
+        [_vp, _i, _sz, _vp, _sz, _hp, _hp, _hp, _hp, _i, _i, _vp],
+    ),
+    "vg_kv_create": (_i, [C.POINTER(VgKvParams), _i, C.POINTER(_vp)]),
+    "vg_kv_destroy": (_i, [_vp]),
+    "vg_kv_get_info": (_i, [_vp, C.POINTER(VgKvInfo)]),
+    "vg_kv_lengths": (_i, [_vp, _vp]),
+    "vg_kv_truncate": (_i, [_vp, _vp]),
+    "vg_kv_weights": (_i, [_vp, C.POINTER(_vp)]),
+    "vg_kv_append": (_i, [_vp, _vp, _i, _hp, _hp, _vp]),
+    "vg_kv_attend": (_i, [_vp, _vp, _i, _hp, _hp, _vp, C.c_float, _i, _vp]),
+    "vg_kv_evict": (_i, [_vp, _sz, _vp, _vp, _sz, _sz, _vp, _vp]),
+    "vg_kv_read": (_i, [_vp, _vp, _vp, _i, _hp, _hp, _vp]),
+    "vg_kv_load": (_i, [_vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "vg_kv_export": (_i, [_vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vg_flat_search_ip_noalloc": (_i, [_vp, _sz, _vp, _sz, _sz, _sz, _i, _vp, _vp, _vp, _vp]),
 }
 

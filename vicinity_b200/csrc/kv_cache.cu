@@ -1,0 +1,433 @@
+// C ABI of the key/value cache (include/vicinity_gpu.h): the handle, its
+// device memory, the launch plans made from host-side lengths, and checks.
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <string>
+#include <vector>
+
+#include "kv_cache.h"
+#include "kv_host.h"
+
+using namespace vg;
+
+struct vg_kv_cache {
+  int device = 0;
+  vg_kv_params params{};
+  KvView view{};
+  DevBuf codes[2], scales[2], weights;
+  std::vector<uint32_t> len;  // tokens of each sequence once all enqueued work is done
+  DevBuf ws_lse, ws_kept;
+  // Work is ordered across streams: each call's stream first waits for the
+  // event recorded after the last call's work.
+  cudaEvent_t done = nullptr;
+
+  ~vg_kv_cache() {
+    if (done) {
+      cudaEventSynchronize(done);
+      cudaEventDestroy(done);
+    }
+  }
+};
+
+namespace {
+
+// The device work of one call, between begin() and the end of the scope.
+class Work {
+ public:
+  Work(vg_kv_cache *kv, void *stream) : kv_(kv), s_(static_cast<cudaStream_t>(stream)) {}
+  ~Work() {  // also after a failed launch: what was enqueued before it is ordered
+    if (begun_) cudaEventRecord(kv_->done, s_);
+  }
+  int begin() {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    VG_CU(cudaStreamIsCapturing(s_, &cap));
+    if (cap != cudaStreamCaptureStatusNone)
+      return fail(VG_ERR_UNSUPPORTED, "unsupported: key/value cache calls cannot be captured into a CUDA graph");
+    VG_CU(cudaStreamWaitEvent(s_, kv_->done, 0));
+    begun_ = true;
+    return VG_OK;
+  }
+
+ private:
+  vg_kv_cache *kv_;
+  cudaStream_t s_;
+  bool begun_ = false;
+};
+
+uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+
+// Rows of all sequences; refuses totals that do not fit the packed row index.
+int total_rows(const vg_kv_cache *kv, const uint32_t *counts, size_t *out) {
+  size_t n = 0;
+  for (size_t s = 0; s < kv->params.num_seqs; ++s) n += counts[s];
+  if (n > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "at most 2^31 - 1 tokens per call");
+  *out = n;
+  return VG_OK;
+}
+
+// Calls launch(plan) for the sequences with a count, kPlanSeqs at a time.
+// entry(seq, PlanSeq&) fills in len and count and returns the entry's units.
+template <class Entry, class Launch>
+int for_plans(const vg_kv_cache *kv, const uint32_t *counts, Entry &&entry, Launch &&launch) {
+  Plan plan;
+  plan.n = plan.units = 0;
+  uint32_t row = 0;
+  uint64_t units = 0;
+  const size_t ns = kv->params.num_seqs;
+  for (size_t s = 0; s < ns; ++s) {
+    if (counts[s]) {
+      PlanSeq &e = plan.s[plan.n++];
+      e.seq = static_cast<uint32_t>(s);
+      e.len = kv->len[s];
+      e.count = counts[s];
+      e.row0 = row;
+      e.unit0 = static_cast<uint32_t>(units);
+      units += entry(s, e);
+      if (units > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "too many tokens in one call");
+      row += counts[s];
+    }
+    if (plan.n == kPlanSeqs || (s + 1 == ns && plan.n)) {
+      plan.units = static_cast<uint32_t>(units);
+      VG_CU(launch(plan));
+      plan.n = 0;
+      units = 0;
+    }
+  }
+  return VG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vg_kv_create(const vg_kv_params *params, int device, vg_kv_cache **out) {
+  return guarded([&]() -> int {
+    if (!params || !out) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    *out = nullptr;
+    const vg_kv_params &p = *params;
+    if (p.num_seqs == 0 || p.num_kv_heads == 0 || p.num_kv_heads > 65535 || p.capacity == 0 ||
+        p.capacity > (1ull << 30))
+      return fail(VG_ERR_INVALID_CONFIG,
+                  "invalid config: num_seqs >= 1, num_kv_heads 1 to 65535 and capacity 1 to 2^30 are needed");
+    if (p.head_dim != 32 && p.head_dim != 64 && p.head_dim != 96 && p.head_dim != 128)
+      return fail(VG_ERR_INVALID_CONFIG, "invalid config `head_dim`: must be 32, 64, 96 or 128");
+    if (p.block_tokens != 16 && p.block_tokens != 32 && p.block_tokens != 64 && p.block_tokens != 128)
+      return fail(VG_ERR_INVALID_CONFIG, "invalid config `block_tokens`: must be 16, 32, 64 or 128");
+    if (p.num_seqs > (1ull << 31) / p.num_kv_heads)
+      return fail(VG_ERR_INVALID_CONFIG, "invalid config: num_seqs * num_kv_heads must be at most 2^31");
+    VG_TRY(check_device(device));
+    DeviceGuard g(device);
+    auto kv = std::make_unique<vg_kv_cache>();
+    kv->device = device;
+    kv->params = p;
+    kv->len.assign(p.num_seqs, 0);
+    const size_t stride = (p.capacity + kKvPad - 1) / kKvPad * kKvPad;
+    const size_t rows = p.num_seqs * p.num_kv_heads;
+    if (rows > (size_t(1) << 50) / (stride * p.head_dim))
+      return fail(VG_ERR_OUT_OF_MEMORY, "the cache does not fit any device");
+    for (int i = 0; i < 2; ++i) {
+      VG_CU(kv->codes[i].reserve(rows * stride * p.head_dim));
+      VG_CU(kv->scales[i].reserve(rows * (stride / p.block_tokens) * sizeof(float)));
+      kv->view.codes[i] = kv->codes[i].as<int8_t>();
+      kv->view.scales[i] = kv->scales[i].as<float>();
+    }
+    VG_CU(kv->weights.reserve(rows * stride * sizeof(float)));
+    VG_CU(cudaMemsetAsync(kv->weights.p, 0, rows * stride * sizeof(float), nullptr));
+    VG_CU(cudaStreamSynchronize(nullptr));
+    VG_CU(cudaEventCreateWithFlags(&kv->done, cudaEventDisableTiming));
+    kv->view.weights = kv->weights.as<float>();
+    kv->view.heads = static_cast<uint32_t>(p.num_kv_heads);
+    kv->view.dim = static_cast<uint32_t>(p.head_dim);
+    kv->view.block = static_cast<uint32_t>(p.block_tokens);
+    kv->view.block_shift = p.block_tokens == 16 ? 4 : p.block_tokens == 32 ? 5 : p.block_tokens == 64 ? 6 : 7;
+    kv->view.stride = static_cast<uint32_t>(stride);
+    *out = kv.release();
+    return VG_OK;
+  });
+}
+
+int vg_kv_destroy(vg_kv_cache *kv) {
+  if (!kv) return VG_OK;
+  DeviceGuard g(kv->device);
+  delete kv;
+  return VG_OK;
+}
+
+int vg_kv_get_info(const vg_kv_cache *kv, vg_kv_info *out) {
+  return guarded([&]() -> int {
+    if (!kv || !out) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    *out = vg_kv_info{};
+    out->num_seqs = kv->params.num_seqs;
+    out->capacity = kv->params.capacity;
+    out->num_kv_heads = kv->params.num_kv_heads;
+    out->head_dim = kv->params.head_dim;
+    out->block_tokens = kv->params.block_tokens;
+    out->weight_stride = kv->view.stride;
+    out->device_bytes = kv->codes[0].cap + kv->codes[1].cap + kv->scales[0].cap + kv->scales[1].cap + kv->weights.cap +
+                        kv->ws_lse.cap + kv->ws_kept.cap;
+    out->device = kv->device;
+    return VG_OK;
+  });
+}
+
+int vg_kv_lengths(const vg_kv_cache *kv, uint32_t *out) {
+  return guarded([&]() -> int {
+    if (!kv || !out) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    std::copy(kv->len.begin(), kv->len.end(), out);
+    return VG_OK;
+  });
+}
+
+int vg_kv_truncate(vg_kv_cache *kv, const uint32_t *lengths) {
+  return guarded([&]() -> int {
+    if (!kv || !lengths) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    for (size_t s = 0; s < kv->len.size(); ++s)
+      if (lengths[s] > kv->len[s])
+        return fail(VG_ERR_INVALID_PARAMETER, "sequence " + std::to_string(s) + " holds " +
+                                                  std::to_string(kv->len[s]) + " tokens: cannot be truncated to " +
+                                                  std::to_string(lengths[s]));
+    std::copy(lengths, lengths + kv->len.size(), kv->len.begin());
+    return VG_OK;
+  });
+}
+
+int vg_kv_weights(const vg_kv_cache *kv, float **out) {
+  return guarded([&]() -> int {
+    if (!kv || !out) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    *out = kv->view.weights;
+    return VG_OK;
+  });
+}
+
+int vg_kv_append(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_heads *k, const vg_heads *v,
+                 void *stream) {
+  return guarded([&]() -> int {
+    if (!kv || !counts) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    VG_TRY(check_dtype(dtype));
+    size_t rows = 0;
+    VG_TRY(total_rows(kv, counts, &rows));
+    for (size_t s = 0; s < kv->len.size(); ++s)
+      if (counts[s] > kv->params.capacity - kv->len[s])
+        return fail(VG_ERR_INVALID_PARAMETER, "sequence " + std::to_string(s) + " would pass its capacity of " +
+                                                  std::to_string(kv->params.capacity) + " tokens");
+    if (rows == 0) return VG_OK;
+    DeviceGuard g(kv->device);
+    VG_TRY(check_heads(k, "k", rows, kv->params.head_dim, dtype, kv->device, false));
+    VG_TRY(check_heads(v, "v", rows, kv->params.head_dim, dtype, kv->device, false));
+    if (k->num_heads != kv->params.num_kv_heads || v->num_heads != kv->params.num_kv_heads)
+      return fail(VG_ERR_DIMENSION_MISMATCH, "k and v must have the cache's key/value heads");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Work work(kv, stream);
+    VG_TRY(work.begin());
+    const uint32_t sh = kv->view.block_shift;
+    VG_TRY(for_plans(
+        kv, counts,
+        [&](size_t, PlanSeq &e) { return ((e.len + e.count - 1) >> sh) - (e.len >> sh) + 1; },
+        [&](const Plan &plan) { return launch_kv_append(kv->view, plan, dtype, strided(*k), strided(*v), s); }));
+    for (size_t i = 0; i < kv->len.size(); ++i) kv->len[i] += counts[i];
+    return VG_OK;
+  });
+}
+
+int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_heads *q, const vg_heads *out,
+                 float *lse, float scale, int flags, void *stream) {
+  return guarded([&]() -> int {
+    if (!kv || !counts) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    VG_TRY(check_dtype(dtype));
+    if (dtype == VG_F32) return fail(VG_ERR_UNSUPPORTED, "unsupported: queries are VG_F16 or VG_BF16");
+    if (!std::isfinite(scale)) return fail(VG_ERR_INVALID_PARAMETER, "scale must be finite");
+    if (flags & ~(VG_KV_CAUSAL | VG_KV_ACCUMULATE)) return fail(VG_ERR_INVALID_PARAMETER, "unknown flags");
+    size_t rows = 0;
+    VG_TRY(total_rows(kv, counts, &rows));
+    if (rows == 0) return VG_OK;
+    DeviceGuard g(kv->device);
+    VG_TRY(check_heads(q, "q", rows, kv->params.head_dim, dtype, kv->device, false));
+    VG_TRY(check_heads(out, "out", rows, kv->params.head_dim, dtype, kv->device, true));
+    if (q->num_heads % kv->params.num_kv_heads)
+      return fail(VG_ERR_DIMENSION_MISMATCH, "the query heads must be a multiple of the cache's key/value heads");
+    if (out->num_heads != q->num_heads) return fail(VG_ERR_DIMENSION_MISMATCH, "out must have the heads of q");
+    if (lse) VG_TRY(check_device_memory(lse, kv->device, "lse"));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Work work(kv, stream);
+    VG_TRY(work.begin());
+    AttendArgs a{};
+    a.kv = kv->view;
+    a.dtype = dtype;
+    a.q = strided(*q);
+    a.out = strided(*out);
+    a.q_heads = static_cast<uint32_t>(q->num_heads);
+    a.group = a.q_heads / kv->view.heads;
+    a.scale = scale;
+    a.causal = (flags & VG_KV_CAUSAL) != 0;
+    if (!lse) {
+      VG_CU(kv->ws_lse.reserve(rows * a.q_heads * sizeof(float)));
+      lse = kv->ws_lse.as<float>();
+    }
+    a.lse = lse;
+    VG_TRY(for_plans(
+        kv, counts, [&](size_t, PlanSeq &e) { return e.count; },
+        [&](const Plan &plan) { return launch_kv_attend_rows(a, plan, s); }));
+    if (flags & VG_KV_ACCUMULATE)
+      VG_TRY(for_plans(
+          kv, counts, [&](size_t, PlanSeq &e) { return ceil_div(e.len, 4); },
+          [&](const Plan &plan) { return launch_kv_weigh_rows(a, plan, s); }));
+    return VG_OK;
+  });
+}
+
+int vg_kv_evict(vg_kv_cache *kv, size_t n, const uint32_t *src, const uint32_t *dst, size_t budget, size_t recent,
+                int32_t *kept, void *stream) {
+  return guarded([&]() -> int {
+    if (!kv || (n && (!src || !dst))) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    if (budget == 0 || budget > kv->params.capacity)
+      return fail(VG_ERR_INVALID_PARAMETER, "budget must be 1 to the capacity");
+    if (recent > budget) return fail(VG_ERR_INVALID_PARAMETER, "recent must be at most budget");
+    std::vector<char> seen(kv->len.size(), 0);
+    for (size_t i = 0; i < n; ++i)
+      for (uint32_t s : {src[i], dst[i]}) {
+        if (s >= kv->len.size()) return fail(VG_ERR_INVALID_PARAMETER, "no sequence " + std::to_string(s));
+        if (seen[s]) return fail(VG_ERR_INVALID_PARAMETER, "sequence " + std::to_string(s) + " appears twice");
+        seen[s] = 1;
+      }
+    if (n == 0) return VG_OK;
+    DeviceGuard g(kv->device);
+    if (kept) VG_TRY(check_device_memory(kept, kv->device, "kept"));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Work work(kv, stream);
+    VG_TRY(work.begin());
+    const size_t row = kv->params.num_kv_heads * budget;
+    if (!kept) {
+      VG_CU(kv->ws_kept.reserve(n * row * sizeof(int32_t)));
+      kept = kv->ws_kept.as<int32_t>();
+    }
+    Plan plan;
+    for (size_t i0 = 0; i0 < n; i0 += kPlanSeqs) {
+      plan.n = static_cast<uint32_t>(std::min<size_t>(n - i0, kPlanSeqs));
+      uint64_t units = 0;
+      for (uint32_t i = 0; i < plan.n; ++i) {
+        PlanSeq &e = plan.s[i];
+        e.seq = src[i0 + i];
+        e.len = kv->len[e.seq];
+        e.count = static_cast<uint32_t>(budget);
+        e.row0 = dst[i0 + i];
+        e.unit0 = static_cast<uint32_t>(units);
+        units += ceil_div(std::min(e.len, e.count), kv->view.block);
+      }
+      if (units > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "too many tokens in one call");
+      plan.units = static_cast<uint32_t>(units);
+      VG_CU(launch_kv_select(kv->view, plan, static_cast<uint32_t>(budget), static_cast<uint32_t>(recent),
+                             kept + i0 * row, s));
+      VG_CU(launch_kv_gather(kv->view, plan, static_cast<uint32_t>(budget), kept + i0 * row, s));
+    }
+    for (size_t i = 0; i < n; ++i) kv->len[dst[i]] = std::min(kv->len[src[i]], static_cast<uint32_t>(budget));
+    return VG_OK;
+  });
+}
+
+int vg_kv_read(vg_kv_cache *kv, const uint32_t *starts, const uint32_t *counts, int dtype, const vg_heads *k,
+               const vg_heads *v, void *stream) {
+  return guarded([&]() -> int {
+    if (!kv || !starts || !counts) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    VG_TRY(check_dtype(dtype));
+    size_t rows = 0;
+    VG_TRY(total_rows(kv, counts, &rows));
+    for (size_t s = 0; s < kv->len.size(); ++s)
+      if (counts[s] && (starts[s] > kv->len[s] || counts[s] > kv->len[s] - starts[s]))
+        return fail(VG_ERR_INVALID_PARAMETER, "sequence " + std::to_string(s) + " holds only " +
+                                                  std::to_string(kv->len[s]) + " tokens");
+    if (rows == 0) return VG_OK;
+    DeviceGuard g(kv->device);
+    VG_TRY(check_heads(k, "k", rows, kv->params.head_dim, dtype, kv->device, true));
+    VG_TRY(check_heads(v, "v", rows, kv->params.head_dim, dtype, kv->device, true));
+    if (k->num_heads != kv->params.num_kv_heads || v->num_heads != kv->params.num_kv_heads)
+      return fail(VG_ERR_DIMENSION_MISMATCH, "k and v must have the cache's key/value heads");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Work work(kv, stream);
+    VG_TRY(work.begin());
+    VG_TRY(for_plans(
+        kv, counts,
+        [&](size_t seq, PlanSeq &e) {
+          e.len = starts[seq];
+          return ceil_div(e.count, kReadTile);
+        },
+        [&](const Plan &plan) { return launch_kv_read(kv->view, plan, dtype, strided(*k), strided(*v), s); }));
+    return VG_OK;
+  });
+}
+
+}  // extern "C"
+
+namespace {
+
+// One row of a host or device array to or from the cache.
+int copy_row(void *dst, const void *src, size_t bytes, cudaStream_t s) {
+  VG_CU(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDefault, s));
+  return VG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vg_kv_load(vg_kv_cache *kv, size_t seq, size_t length, const int8_t *k_codes, const float *k_scales,
+               const int8_t *v_codes, const float *v_scales, const float *weights, void *stream) {
+  return guarded([&]() -> int {
+    if (!kv) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    if (seq >= kv->len.size()) return fail(VG_ERR_INVALID_PARAMETER, "no sequence " + std::to_string(seq));
+    if (length > kv->params.capacity) return fail(VG_ERR_INVALID_PARAMETER, "length is over the capacity");
+    if (length && (!k_codes || !k_scales || !v_codes || !v_scales))
+      return fail(VG_ERR_INVALID_PARAMETER, "null codes or scales");
+    DeviceGuard g(kv->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Work work(kv, stream);
+    VG_TRY(work.begin());
+    const KvView &w = kv->view;
+    const int8_t *codes[2] = {k_codes, v_codes};
+    const float *scales[2] = {k_scales, v_scales};
+    const size_t nb = w.stride >> w.block_shift, used = (length + w.block - 1) >> w.block_shift;
+    for (size_t h = 0; length && h < w.heads; ++h) {
+      const size_t r = seq * w.heads + h;
+      for (int i = 0; i < 2; ++i) {
+        VG_TRY(copy_row(w.codes[i] + r * w.stride * w.dim, codes[i] + h * length * w.dim, length * w.dim, s));
+        VG_TRY(copy_row(w.scales[i] + r * nb, scales[i] + h * used, used * sizeof(float), s));
+      }
+      if (weights) VG_TRY(copy_row(w.weights + r * w.stride, weights + h * length, length * sizeof(float), s));
+      else VG_CU(cudaMemsetAsync(w.weights + r * w.stride, 0, length * sizeof(float), s));
+    }
+    VG_CU(cudaStreamSynchronize(s));
+    kv->len[seq] = static_cast<uint32_t>(length);
+    return VG_OK;
+  });
+}
+
+int vg_kv_export(vg_kv_cache *kv, size_t seq, int8_t *k_codes, float *k_scales, int8_t *v_codes, float *v_scales,
+                 float *weights, void *stream) {
+  return guarded([&]() -> int {
+    if (!kv) return fail(VG_ERR_INVALID_PARAMETER, "null argument");
+    if (seq >= kv->len.size()) return fail(VG_ERR_INVALID_PARAMETER, "no sequence " + std::to_string(seq));
+    const size_t length = kv->len[seq];
+    if (length && (!k_codes || !k_scales || !v_codes || !v_scales))
+      return fail(VG_ERR_INVALID_PARAMETER, "null codes or scales");
+    DeviceGuard g(kv->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Work work(kv, stream);
+    VG_TRY(work.begin());
+    const KvView &w = kv->view;
+    int8_t *codes[2] = {k_codes, v_codes};
+    float *scales[2] = {k_scales, v_scales};
+    const size_t nb = w.stride >> w.block_shift, used = (length + w.block - 1) >> w.block_shift;
+    for (size_t h = 0; length && h < w.heads; ++h) {
+      const size_t r = seq * w.heads + h;
+      for (int i = 0; i < 2; ++i) {
+        VG_TRY(copy_row(codes[i] + h * length * w.dim, w.codes[i] + r * w.stride * w.dim, length * w.dim, s));
+        VG_TRY(copy_row(scales[i] + h * used, w.scales[i] + r * nb, used * sizeof(float), s));
+      }
+      if (weights) VG_TRY(copy_row(weights + h * length, w.weights + r * w.stride, length * sizeof(float), s));
+    }
+    VG_CU(cudaStreamSynchronize(s));
+    return VG_OK;
+  });
+}
+
+}  // extern "C"

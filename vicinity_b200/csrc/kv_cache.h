@@ -1,0 +1,101 @@
+// Device-side view of a key/value cache and the launchers of its kernels
+// (rotary.cu, kv_store.cu, kv_attend.cu, kv_attend_tc.cu).
+//
+// Layout, per (sequence, key/value head) row r = seq * heads + head:
+//   codes   int8 [2: K, V][rows][stride][dim]   token-major
+//   scales  f32  [2][rows][stride / block]      powers of two
+//   weights f32  [rows][stride]
+// stride is the capacity rounded up to kKvPad tokens, so a tile of up to
+// kKvPad tokens that starts on a multiple of its size is one contiguous range
+// inside the row, whatever the sequence's length.  Memory past a sequence's
+// length holds finite codes but any scale: readers select, never multiply,
+// it away.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace vg {
+
+constexpr uint32_t kKvPad = 128;
+constexpr int kPlanSeqs = 256;  // sequences per launch: the plan travels as a kernel argument (8 KB)
+
+struct KvView {
+  int8_t *codes[2];
+  float *scales[2];
+  float *weights;
+  uint32_t heads, dim, block, block_shift, stride;
+};
+
+// One sequence of a launch.  unit0: the first of the launch's work units that
+// belongs to it (what a unit is, the kernel says).
+struct PlanSeq {
+  uint32_t seq;    // slot in the cache
+  uint32_t len;    // tokens cached when the kernel runs
+  uint32_t count;  // tokens of this call
+  uint32_t row0;   // first of them in the packed tensors
+  uint32_t unit0;
+};
+struct Plan {
+  uint32_t n, units;
+  PlanSeq s[kPlanSeqs];
+};
+
+struct Strided {
+  void *p;
+  int64_t token, head;  // strides in elements
+};
+
+// Entry of the plan that work unit u belongs to (entries without units are skipped).
+__device__ __forceinline__ uint32_t plan_find(const Plan &plan, uint32_t u) {
+  uint32_t lo = 0, hi = plan.n;  // last entry with unit0 <= u
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (plan.s[mid].unit0 <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// ---- rotary.cu ----
+struct RotaryTable {
+  double turns[128];  // frequency / (2 pi)
+  uint32_t pairs;
+  int interleaved;
+  float magnitude;
+};
+cudaError_t launch_rotary(const RotaryTable &t, int dtype, uint32_t dim, const int64_t *pos, size_t tokens,
+                          const Strided &q, const Strided &qo, uint32_t q_heads, const Strided &k, const Strided &ko,
+                          uint32_t k_heads, bool transpose, cudaStream_t s);
+
+// ---- kv_store.cu ----
+// Units: the blocks that a sequence's new tokens touch (len: before the append).
+cudaError_t launch_kv_append(const KvView &kv, const Plan &plan, int dtype, const Strided &k, const Strided &v,
+                             cudaStream_t s);
+// Units: tiles of kReadTile tokens of [len, len + count) -- len is the first token read.
+constexpr uint32_t kReadTile = 32;
+cudaError_t launch_kv_read(const KvView &kv, const Plan &plan, int dtype, const Strided &k, const Strided &v,
+                           cudaStream_t s);
+// Selection: entry i keeps min(len, count = budget) tokens of sequence seq;
+// kept i32 [entries][heads][budget].  row0 is the destination sequence.
+cudaError_t launch_kv_select(const KvView &kv, const Plan &plan, uint32_t budget, uint32_t recent, int32_t *kept,
+                             cudaStream_t s);
+// Units: blocks of the destination.
+cudaError_t launch_kv_gather(const KvView &kv, const Plan &plan, uint32_t budget, const int32_t *kept,
+                             cudaStream_t s);
+
+// ---- kv_attend.cu ----
+struct AttendArgs {
+  KvView kv;
+  int dtype;
+  Strided q, out;
+  uint32_t q_heads, group;
+  float scale;      // softmax scale
+  bool causal;
+  float *lse;       // [rows][q_heads]
+};
+cudaError_t launch_kv_attend_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+cudaError_t launch_kv_weigh_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+
+}  // namespace vg
