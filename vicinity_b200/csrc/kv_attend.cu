@@ -1,11 +1,410 @@
 // Attention over a key/value cache held in 8 bits.
+//
+// Scores are x = log2(e) scale q.k and the reference of a row's exponentials is
+// the running maximum of x + log2(value scale): with P = 2^(x + log2 vs - mu) the
+// sum of P times the value codes needs no other factor, and the denominator is
+// the sum of P / vs (powers of two: exact).  Codes are exact in binary16, and a
+// query row is scaled by a power of two into its range, so both products run on
+// the tensor cores in binary16 with f32 sums; only P is rounded, to 11 bits.
 #include "common.cuh"
 #include "elements.cuh"
+#include "kv_attend.cuh"
 #include "kv_cache.h"
 
 namespace vg {
 
 namespace {
+
+// ---- up to 16 query rows per key/value head ----------------------------------
+//
+// One token of decoding, or a few: bound by reading the codes once.  A CTA of
+// four warps takes (sequence, head, chunk of tokens); each warp walks its own
+// 16-token steps, which it copies into its own shared-memory ring (cp.async,
+// kStages steps ahead, no barrier between warps), converts to binary16 in
+// registers and multiplies with mma.sync m16n8k16, the rows' 16 being all that
+// there is.  The order of the dimensions inside a product is free, so a lane
+// takes whole words of a row: dim / 4 consecutive key dimensions, dim / 8
+// consecutive value dimensions.
+constexpr int kDecWarps = 4;
+constexpr int kStages = 4;
+constexpr int kStep = 16;  // tokens per step: one scale each for keys and values (blocks are multiples of 16)
+
+// byte offset of (token, byte of its row) in a stage: 16-byte chunks XORed so
+// that the lanes of one load phase hit different banks
+template <int D>
+__device__ __forceinline__ uint32_t swz(uint32_t tok, uint32_t byte) {
+  if (D == 128) return tok * D + (byte ^ ((tok & 7u) << 4));
+  if (D == 64) return tok * D + (byte ^ (((tok >> 1) & 3u) << 4));
+  return tok * D + byte;
+}
+
+// N words at byte offset `at` (a multiple of their size) of a row's chunk
+template <int D, int N>
+__device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint32_t at, uint32_t (&w)[N]) {
+  if (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(st + swz<D>(tok, at + 16 * i));
+      w[4 * i] = x.x;
+      w[4 * i + 1] = x.y;
+      w[4 * i + 2] = x.z;
+      w[4 * i + 3] = x.w;
+    }
+  } else if (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 x = *reinterpret_cast<const uint2 *>(st + swz<D>(tok, at + 8 * i));
+      w[2 * i] = x.x;
+      w[2 * i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t *>(st + swz<D>(tok, at + 4 * i));
+  }
+}
+
+// The result of one row from its sums: 8 dimensions from c on, and the lse.
+template <class T>
+__device__ __forceinline__ void finish_row(const AttendArgs &a, size_t token, uint32_t hq, uint32_t c, bool ovec,
+                                           float mu, float sum, float (&y)[8]) {
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no token seen: 0
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] *= inv;
+  store8(static_cast<T *>(a.out.p) + static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head +
+             c,
+         ovec, y);
+  if (c == 0) {
+    const float lse2 = sum == 0.0f ? -VG_INF : mu - kPShift + log2f(sum);
+    if (a.lse) a.lse[token * a.q_heads + hq] = lse2 * kLn2;
+    if (a.lse2) a.lse2[token * a.q_heads + hq] = lse2;
+  }
+}
+
+template <class T, int D, bool kScores>
+__global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const __grid_constant__ AttendArgs a,
+                                                                          const __grid_constant__ Plan plan,
+                                                                          const bool qvec, const bool ovec) {
+  constexpr int kPlane = kStep * D;                    // bytes of one step's keys (or values)
+  constexpr int kStage = 2 * kPlane + 16;              // and the two scales
+  constexpr int kK = D / 16;                           // key words per lane and token = k-steps
+  constexpr int kV = D / 32;                           // value words per lane and token
+  extern __shared__ __align__(16) uint8_t dec_smem[];
+  const int warp = threadIdx.x >> 5, lane = lane_id(), n = lane >> 2, j = lane & 3;
+  uint8_t *ring = dec_smem + warp * (kStages * kStage);
+  const KvView &kv = a.kv;
+  const uint32_t unit = blockIdx.x, entry = plan_find(plan, unit), head = blockIdx.y;
+  const PlanSeq &ps = plan.s[entry];
+  const uint32_t t0 = (unit - ps.unit0) * a.chunk, t1 = min(ps.len, t0 + a.chunk);
+  const size_t r = static_cast<size_t>(ps.seq) * kv.heads + head;
+  const int8_t *kc = kv.codes[0] + r * kv.stride * D, *vc = kv.codes[1] + r * kv.stride * D;
+  const size_t nb = kv.stride >> kv.block_shift;
+  const float *ks = kv.scales[0] + r * nb, *vs = kv.scales[1] + r * nb;
+
+  const uint32_t steps = t1 > t0 ? (t1 - t0 + kStep - 1) / kStep : 0;
+  auto fetch = [&](uint32_t step, uint32_t slot) {  // always one group, empty past the end
+    if (step < steps) {
+      uint8_t *st = ring + slot * kStage;
+      const uint32_t t = t0 + step * kStep;
+      const int8_t *sk = kc + static_cast<size_t>(t) * D, *sv = vc + static_cast<size_t>(t) * D;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint32_t c = lane + 32 * i, tok = c / (D / 16), byte = (c % (D / 16)) * 16;
+        cp_async16(st + swz<D>(tok, byte), sk + c * 16);
+        cp_async16(st + kPlane + swz<D>(tok, byte), sv + c * 16);
+      }
+      if (lane < 2) cp_async4(st + 2 * kPlane + lane * 4, (lane ? vs : ks) + (t >> kv.block_shift));
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(warp + i * kDecWarps, i);
+
+  // the lane's two rows: their limits, and the query as A fragments
+  const uint32_t rows = ps.count * a.group;
+  const uint32_t score_stride = (ps.len + kStep - 1) / kStep * kStep;
+  float *scores = a.scores + ps.aux + static_cast<size_t>(head) * rows * score_stride;
+  uint32_t lim[2];
+  float qs[2];
+  uint32_t qa[kK][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t row = n + 8 * h;
+    float x[D / 4];
+    lim[h] = 0;
+    if (row < rows) {
+      const uint32_t qi = row / a.group;
+      lim[h] = tokens_seen(ps, qi, a.causal);
+      const T *q = static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + qi) * a.q.token +
+                   static_cast<int64_t>(head * a.group + row - qi * a.group) * a.q.head + j * (D / 4);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) load8(q + 8 * i, qvec, *reinterpret_cast<float(*)[8]>(x + 8 * i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor_sync(VG_FULL_MASK, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(VG_FULL_MASK, top, 2));
+    float inv;
+    row_scale(top, qs[h], inv);
+    qs[h] *= a.scale * kLog2e;
+#pragma unroll
+    for (int s = 0; s < kK; ++s) {
+      qa[s][h] = pack_half2(x[4 * s] * inv, x[4 * s + 1] * inv);
+      qa[s][2 + h] = pack_half2(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
+    }
+  }
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float mu[2] = {-VG_INF, -VG_INF}, l[2] = {0.0f, 0.0f};
+  const uint32_t all_see = __reduce_min_sync(VG_FULL_MASK, min(n < rows ? lim[0] : t1, n + 8 < rows ? lim[1] : t1));
+
+  for (uint32_t step = warp, i = 0; step < steps; step += kDecWarps, ++i) {
+    fetch(step + (kStages - 1) * kDecWarps, (i + kStages - 1) % kStages);
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint8_t *st = ring + (i % kStages) * kStage;
+    const uint32_t t = t0 + step * kStep;
+    float s[2][4] = {};
+    {
+      uint32_t w0[kK], w1[kK];
+      row_words<D>(st, n, j * (D / 4), w0);
+      row_words<D>(st, n + 8, j * (D / 4), w1);
+#pragma unroll
+      for (int c = 0; c < kK; ++c) {
+        const uint32_t x0 = w0[c] ^ 0x80808080u, x1 = w1[c] ^ 0x80808080u;
+        mma_f16(s[0], qa[c], half2_of<0x4140>(x0), half2_of<0x4342>(x0));
+        mma_f16(s[1], qa[c], half2_of<0x4140>(x1), half2_of<0x4342>(x1));
+      }
+    }
+    const float kscale = *reinterpret_cast<const float *>(st + 2 * kPlane);
+    const float vscale = *reinterpret_cast<const float *>(st + 2 * kPlane + 4);
+    const float lv = log2_scale(vscale);
+    float gm[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float f = kscale * qs[h];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c >> 1][2 * h + (c & 1)] *= f;
+    }
+    if (t + kStep > all_see) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (t + 2 * j + (c & 1) + 8 * (c >> 1) >= lim[h]) s[c >> 1][2 * h + (c & 1)] = -VG_INF;
+    }
+    if (kScores) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (n + 8 * h < rows) {
+          float *sc = scores + static_cast<size_t>(n + 8 * h) * score_stride + t + 2 * j;
+          *reinterpret_cast<float2 *>(sc) = make_float2(s[0][2 * h], s[0][2 * h + 1]);
+          *reinterpret_cast<float2 *>(sc + 8) = make_float2(s[1][2 * h], s[1][2 * h + 1]);
+        }
+    }
+    bool raise = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      gm[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])) + lv;
+      raise |= gm[h] > mu[h] + kLazy;
+    }
+    if (__any_sync(VG_FULL_MASK, raise)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        gm[h] = fmaxf(gm[h], __shfl_xor_sync(VG_FULL_MASK, gm[h], 1));
+        gm[h] = fmaxf(gm[h], __shfl_xor_sync(VG_FULL_MASK, gm[h], 2));
+        const float m = fmaxf(mu[h], gm[h]);
+        const float c = m == -VG_INF ? 1.0f : exp2_approx(mu[h] - m);
+        mu[h] = m;
+        l[h] *= c;
+#pragma unroll
+        for (int i2 = 0; i2 < D / 8; ++i2) {
+          o[i2][2 * h] *= c;
+          o[i2][2 * h + 1] *= c;
+        }
+      }
+    }
+    uint32_t pa[4];
+    const float per_v = inverse_scale(vscale);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float ref = lv + kPShift - (mu[h] == -VG_INF ? 0.0f : mu[h]);
+      float p[4], sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        p[c] = exp2_approx(s[c >> 1][2 * h + (c & 1)] + ref);
+        sum += p[c];
+      }
+      l[h] += sum * per_v;
+      if (vscale != vscale) {  // the values read as NaN: so does every row that sees one of them
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (t + 2 * j + (c & 1) + 8 * (c >> 1) < lim[h]) p[c] = vscale;
+      }
+      pa[h] = pack_half2(p[0], p[1]);
+      pa[2 + h] = pack_half2(p[2], p[3]);
+    }
+    {
+      uint32_t w[4][kV];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        row_words<D>(st + kPlane, 2 * j + (c & 1) + 8 * (c >> 1), n * (D / 8), w[c]);
+#pragma unroll
+      for (int c = 0; c < kV; ++c) {
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+          const uint32_t sel = hi ? 0x7362u : 0x5140u;
+          const uint32_t x0 = __byte_perm(w[0][c], w[1][c], sel) ^ 0x80808080u;
+          const uint32_t x1 = __byte_perm(w[2][c], w[3][c], sel) ^ 0x80808080u;
+          mma_f16(o[4 * c + 2 * hi], pa, half2_of<0x4140>(x0), half2_of<0x4140>(x1));
+          mma_f16(o[4 * c + 2 * hi + 1], pa, half2_of<0x4342>(x0), half2_of<0x4342>(x1));
+        }
+      }
+    }
+    __syncwarp();  // the slot is free for the next fetch
+  }
+
+  // join the four warps, then write the rows out or, one chunk of several, as partial sums
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(VG_FULL_MASK, l[h], 1);
+    l[h] += __shfl_xor_sync(VG_FULL_MASK, l[h], 2);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  float *so = reinterpret_cast<float *>(dec_smem);                       // [warp][16][D]
+  float2 *sml = reinterpret_cast<float2 *>(so + kDecWarps * kDecodeRows * D);  // [warp][16]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float *row = so + (warp * kDecodeRows + n + 8 * h) * D + 2 * j * (D / 8);
+#pragma unroll
+    for (int i = 0; i < D / 8; i += 4) {
+      *reinterpret_cast<float4 *>(row + i) =
+          make_float4(o[i][2 * h], o[i + 1][2 * h], o[i + 2][2 * h], o[i + 3][2 * h]);
+      *reinterpret_cast<float4 *>(row + D / 8 + i) =
+          make_float4(o[i][2 * h + 1], o[i + 1][2 * h + 1], o[i + 2][2 * h + 1], o[i + 3][2 * h + 1]);
+    }
+    if (j == 0) sml[warp * kDecodeRows + n + 8 * h] = make_float2(mu[h], l[h]);
+  }
+  __syncthreads();
+  const bool whole = ps.len <= a.chunk;
+  for (uint32_t e = threadIdx.x; e < rows * (D / 8); e += kDecWarps * 32) {
+    const uint32_t row = e / (D / 8), c = e % (D / 8) * 8;
+    float m = -VG_INF, sum = 0.0f, y[8] = {};
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, sml[w * kDecodeRows + row].x);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float2 ml = sml[w * kDecodeRows + row];
+      const float f = ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
+      sum += f * ml.y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kDecodeRows + row) * D + c + i];
+    }
+    if (whole) {
+      const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
+      finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
+    } else {
+      const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kDecodeRows + row;
+      float *dst = a.part_o + at * D + c;
+      *reinterpret_cast<float4 *>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4 *>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
+      if (c == 0) a.part_ml[at] = make_float2(m, sum);
+    }
+  }
+}
+
+// ---- joining the chunks of a sequence -------------------------------------------
+
+// One CTA per (sequence, head, row): 16-byte slices of the row's partial sums,
+// groups of threads taking every kGroups-th chunk.
+constexpr int kJoinThreads = 256;
+
+template <class T>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendArgs a,
+                                                                   const __grid_constant__ Plan plan,
+                                                                   const uint32_t part_rows, const bool ovec) {
+  __shared__ float weight[kMaxSplits];
+  __shared__ float red[kJoinThreads / 32];
+  __shared__ float acc[kJoinThreads * 8];
+  const PlanSeq &ps = plan.s[blockIdx.x];
+  const uint32_t head = blockIdx.y, row = blockIdx.z, D = a.kv.dim;
+  if (ps.len <= a.chunk || row >= ps.count * a.group) return;
+  const uint32_t ns = (ps.len + a.chunk - 1) / a.chunk;
+  const size_t step = static_cast<size_t>(a.kv.heads) * part_rows;
+  const size_t first = (static_cast<size_t>(ps.unit0) * a.kv.heads + head) * part_rows + row;
+  const int warp = threadIdx.x >> 5;
+  float m = -VG_INF;
+  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) m = fmaxf(m, a.part_ml[first + i * step].x);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
+  if (lane_id() == 0) red[warp] = m;
+  __syncthreads();
+  for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, red[w]);
+  __syncthreads();
+  float sum = 0.0f;
+  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
+    const float2 ml = a.part_ml[first + i * step];
+    const float f = ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
+    weight[i] = f;
+    sum += f * ml.y;
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(VG_FULL_MASK, sum, w);
+  if (lane_id() == 0) red[warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[w];
+  const uint32_t per = D / 8, groups = kJoinThreads / per, g = threadIdx.x / per, c = threadIdx.x % per * 8;
+  float y[8] = {};
+  if (g < groups) {
+#pragma unroll 2
+    for (uint32_t i = g; i < ns; i += groups) {
+      const float4 *src = reinterpret_cast<const float4 *>(a.part_o + (first + i * step) * D + c);
+      const float4 u = src[0], v = src[1];
+      const float f = weight[i];
+      y[0] += f * u.x, y[1] += f * u.y, y[2] += f * u.z, y[3] += f * u.w;
+      y[4] += f * v.x, y[5] += f * v.y, y[6] += f * v.z, y[7] += f * v.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[threadIdx.x * 8 + i] = y[i];
+  __syncthreads();
+  if (g == 0) {
+    for (uint32_t w = 1; w < groups; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += acc[(w * per + threadIdx.x) * 8 + i];
+    const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
+    finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
+  }
+}
+
+// Weights from stored scores: a thread takes one token of one head.
+__global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_constant__ AttendArgs a,
+                                                                  const __grid_constant__ Plan plan) {
+  const PlanSeq &ps = plan.s[plan_find(plan, blockIdx.x)];
+  const uint32_t t = (blockIdx.x - ps.unit0) * kWeighTile + threadIdx.x, head = blockIdx.y;
+  if (t >= ps.len) return;
+  const uint32_t rows = ps.count * a.group, stride = (ps.len + kStep - 1) / kStep * kStep;
+  const float *sc = a.scores + ps.aux + static_cast<size_t>(head) * rows * stride + t;
+  const float *lse = a.lse2 + static_cast<size_t>(ps.row0) * a.q_heads + head * a.group;
+  float sum = 0.0f;
+  for (uint32_t row = 0; row < rows; ++row) {
+    const uint32_t qi = row / a.group;
+    const float x = sc[static_cast<size_t>(row) * stride];
+    const float p = exp2_approx(x - lse[static_cast<size_t>(qi) * a.q_heads + row - qi * a.group]);
+    sum += x == -VG_INF ? 0.0f : p;  // not seen
+  }
+  float *w = a.kv.weights + (static_cast<size_t>(ps.seq) * a.kv.heads + head) * a.kv.stride + t;
+  *w += sum;
+}
+
+// ---- more rows -----------------------------------------------------------------
 
 constexpr int kRowWarps = 4;
 
@@ -48,7 +447,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const __gri
   T *out = static_cast<T *>(a.out.p) + static_cast<int64_t>(ps.row0 + j) * a.out.token +
            static_cast<int64_t>(h) * a.out.head;
   for (uint32_t i = 0; i < per; ++i) out[lane + 32 * i] = from_f32<T>(sees ? o[i] / l : 0.0f);
-  if (lane == 0) a.lse[static_cast<size_t>(ps.row0 + j) * a.q_heads + h] = m + logf(l);
+  if (lane == 0) {
+    const size_t at = static_cast<size_t>(ps.row0 + j) * a.q_heads + h;
+    if (a.lse) a.lse[at] = m + logf(l);
+    if (a.lse2) a.lse2[at] = (m + logf(l)) * kLog2e;
+  }
 }
 
 // One warp per (cached token, key/value head): its probabilities, recomputed
@@ -77,13 +480,54 @@ __global__ void __launch_bounds__(kRowWarps * 32) weigh_rows_kernel(const __grid
       for (uint32_t i = 0; i < per; ++i) d += to_f32(q[lane + 32 * i]) * kvv[i];
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(VG_FULL_MASK, d, w);
-      sum += expf(d - a.lse[static_cast<size_t>(ps.row0 + j) * a.q_heads + h]);
+      sum += exp2f(d * kLog2e - a.lse2[static_cast<size_t>(ps.row0 + j) * a.q_heads + h]);
     }
   }
   if (lane == 0) kv.weights[r * kv.stride + t] += sum;
 }
 
+template <class T, int D>
+cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  auto *kern = a.scores ? attend_decode_kernel<T, D, true> : attend_decode_kernel<T, D, false>;
+  const int smem = kDecWarps * kStages * (2 * kStep * D + 16);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<dim3(plan.units, a.kv.heads), kDecWarps * 32, smem, s>>>(a, plan, rows_aligned(a.q, sizeof(T)),
+                                                                  rows_aligned(a.out, sizeof(T)));
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t decode_dim(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  switch (a.kv.dim) {
+    case 32: return decode<T, 32>(a, plan, s);
+    case 64: return decode<T, 64>(a, plan, s);
+    case 96: return decode<T, 96>(a, plan, s);
+    default: return decode<T, 128>(a, plan, s);
+  }
+}
+
 }  // namespace
+
+cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  if (plan.units == 0) return cudaSuccess;
+  return a.dtype == VG_F16 ? decode_dim<__half>(a, plan, s) : decode_dim<__nv_bfloat16>(a, plan, s);
+}
+
+cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, int part_rows, uint32_t max_rows,
+                                  cudaStream_t s) {
+  const dim3 grid(plan.n, a.kv.heads, max_rows);
+  const bool vec = rows_aligned(a.out, 2);
+  if (a.dtype == VG_F16) attend_join_kernel<__half><<<grid, kJoinThreads, 0, s>>>(a, plan, part_rows, vec);
+  else attend_join_kernel<__nv_bfloat16><<<grid, kJoinThreads, 0, s>>>(a, plan, part_rows, vec);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_weigh_scores(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  if (plan.units == 0) return cudaSuccess;
+  weigh_scores_kernel<<<dim3(plan.units, a.kv.heads), kWeighTile, 0, s>>>(a, plan);
+  return cudaGetLastError();
+}
 
 cudaError_t launch_kv_attend_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;

@@ -1,0 +1,87 @@
+// Device helpers shared by the attention kernels of the 8-bit cache.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <stdint.h>
+
+#include "kv_cache.h"
+#include "pipeline.cuh"
+
+namespace vg {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+#define VG_INF __int_as_float(0x7f800000)
+
+// Probabilities are held as 2^(x - mu + kPShift) in binary16: mu may lag the
+// running maximum by kLazy (fewer rescalings), so they are at most 2^15 and
+// vanish below 2^-38 of the largest.
+constexpr float kPShift = 13.0f, kLazy = 2.0f;
+
+__device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; 2^-inf = 0
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Two of the code bytes c of x (biased by 128), picked by the selector, as a
+// binary16 pair: 0x6400 | u is 1024 + u.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t half2_of(uint32_t x) {
+  const uint32_t m = __byte_perm(x, 0x64646464u, kSel), bias = 0x64806480u;  // 1152
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&m), *reinterpret_cast<const __half2 *>(&bias));
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// c += a b: A 16 x 16 and B 16 x 8 in binary16, C in f32
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The power of two s (and 1 / s) that brings a row of largest magnitude `top`
+// to [1, 2) (below 4 at the very end of the range); 1 where there is none.
+__device__ __forceinline__ void row_scale(float top, float &s, float &inv) {
+  const uint32_t e = __float_as_uint(top) >> 23;
+  const uint32_t c = top == 0.0f || e >= 255u ? 127u : min(max(e, 1u), 253u);
+  s = __uint_as_float(c << 23);
+  inv = __uint_as_float((254u - c) << 23);
+}
+
+// log2 and reciprocal of a value scale (a power of two); a scale that is NaN
+// counts as 1 here: the probabilities it meets are made NaN instead, so that
+// the denominators stay what they are
+__device__ __forceinline__ float log2_scale(float s) {
+  return s == s ? static_cast<float>(static_cast<int>(__float_as_uint(s) >> 23) - 127) : 0.0f;
+}
+__device__ __forceinline__ float inverse_scale(float s) {
+  return s == s ? __uint_as_float(0x7f000000u - __float_as_uint(s)) : 1.0f;
+}
+
+// Cached tokens that query qi of a sequence sees.
+__device__ __forceinline__ uint32_t tokens_seen(const PlanSeq &ps, uint32_t qi, bool causal) {
+  const uint32_t behind = ps.count - 1 - qi;
+  return !causal ? ps.len : ps.len > behind ? ps.len - behind : 0;
+}
+
+}  // namespace vg

@@ -17,7 +17,7 @@ struct vg_kv_cache {
   KvView view{};
   DevBuf codes[2], scales[2], weights;
   std::vector<uint32_t> len;  // tokens of each sequence once all enqueued work is done
-  DevBuf ws_lse, ws_kept;
+  DevBuf ws_lse, ws_kept, ws_part, ws_scores;
   // Work is ordered across streams: each call's stream first waits for the
   // event recorded after the last call's work.
   cudaEvent_t done = nullptr;
@@ -68,15 +68,16 @@ int total_rows(const vg_kv_cache *kv, const uint32_t *counts, size_t *out) {
 
 // Calls launch(plan) for the sequences with a count, kPlanSeqs at a time.
 // entry(seq, PlanSeq&) fills in len and count and returns the entry's units.
-template <class Entry, class Launch>
-int for_plans(const vg_kv_cache *kv, const uint32_t *counts, Entry &&entry, Launch &&launch) {
+// Sequences that `take` refuses are passed over.
+template <class Take, class Entry, class Launch>
+int for_plans_of(const vg_kv_cache *kv, const uint32_t *counts, Take &&take, Entry &&entry, Launch &&launch) {
   Plan plan;
   plan.n = plan.units = 0;
   uint32_t row = 0;
   uint64_t units = 0;
   const size_t ns = kv->params.num_seqs;
   for (size_t s = 0; s < ns; ++s) {
-    if (counts[s]) {
+    if (counts[s] && take(counts[s])) {
       PlanSeq &e = plan.s[plan.n++];
       e.seq = static_cast<uint32_t>(s);
       e.len = kv->len[s];
@@ -85,14 +86,105 @@ int for_plans(const vg_kv_cache *kv, const uint32_t *counts, Entry &&entry, Laun
       e.unit0 = static_cast<uint32_t>(units);
       units += entry(s, e);
       if (units > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "too many tokens in one call");
-      row += counts[s];
     }
+    row += counts[s];
     if (plan.n == kPlanSeqs || (s + 1 == ns && plan.n)) {
       plan.units = static_cast<uint32_t>(units);
-      VG_CU(launch(plan));
+      VG_TRY(launch(plan));
       plan.n = 0;
       units = 0;
     }
+  }
+  return VG_OK;
+}
+
+template <class Entry, class Launch>
+int for_plans(const vg_kv_cache *kv, const uint32_t *counts, Entry &&entry, Launch &&launch) {
+  return for_plans_of(kv, counts, [](uint32_t) { return true; }, entry, [&](Plan &plan) -> int {
+    VG_CU(launch(plan));
+    return VG_OK;
+  });
+}
+
+// Re-counts a plan's units: units_of(entry) each.
+template <class Units>
+int set_units(Plan &plan, Units &&units_of) {
+  uint64_t units = 0;
+  for (uint32_t i = 0; i < plan.n; ++i) {
+    plan.s[i].unit0 = static_cast<uint32_t>(units);
+    units += units_of(plan.s[i]);
+    if (units > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "too many tokens in one call");
+  }
+  plan.units = static_cast<uint32_t>(units);
+  return VG_OK;
+}
+
+// Tokens per work unit when every (sequence, head) is cut into chunks: the
+// smallest multiple of `quantum` that gives at most `slots` units, what the
+// GPU runs at once, or -- where the uncut sequences alone come near that --
+// four times as many, so that the last wave is a short one.
+uint32_t pick_chunk(const Plan &plan, uint64_t per_chunk, uint64_t slots, uint32_t quantum) {
+  uint32_t longest = 1;
+  for (uint32_t i = 0; i < plan.n; ++i) longest = std::max(longest, plan.s[i].len);
+  const uint64_t most = plan.n * per_chunk * 2 <= slots ? slots : 4 * slots;
+  uint32_t lo = std::max(1u, ceil_div(ceil_div(longest, kMaxSplits), quantum)), hi = std::max(lo, ceil_div(longest, quantum));
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    uint64_t units = 0;
+    for (uint32_t i = 0; i < plan.n; ++i) units += std::max(1u, ceil_div(plan.s[i].len, mid * quantum)) * per_chunk;
+    if (units <= most) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo * quantum;
+}
+
+constexpr size_t kScoreBytes = size_t(1) << 30;  // stored scores of one launch, at most
+constexpr uint64_t kDecodeSlots = 148 * 3;       // CTAs of the decoding kernel that run at once
+constexpr uint32_t kDecodeQuantum = 64;          // 4 warps of 16 tokens
+
+// Sequences of at most kDecodeRows rows per key/value head.
+int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
+  a.chunk = pick_chunk(plan, kv->view.heads, kDecodeSlots, kDecodeQuantum);
+  uint32_t max_rows = 0;
+  bool split = false;
+  size_t scores = 0;
+  for (uint32_t i = 0; i < plan.n; ++i) {
+    PlanSeq &e = plan.s[i];
+    max_rows = std::max(max_rows, e.count * a.group);
+    split |= e.len > a.chunk;
+    e.aux = scores;
+    scores += static_cast<size_t>(kv->view.heads) * e.count * a.group * (static_cast<size_t>(ceil_div(e.len, 16)) * 16);
+  }
+  VG_TRY(set_units(plan, [&](const PlanSeq &e) { return std::max(1u, ceil_div(e.len, a.chunk)); }));
+  if (split) {
+    const size_t rows = static_cast<size_t>(plan.units) * kv->view.heads * kDecodeRows;
+    VG_CU(kv->ws_part.reserve(rows * (kv->view.dim * sizeof(float) + sizeof(float2))));
+    a.part_o = kv->ws_part.as<float>();
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * kv->view.dim);
+  }
+  const bool keep = a.lse2 && scores * sizeof(float) <= kScoreBytes;
+  if (keep) {
+    VG_CU(kv->ws_scores.reserve(std::max<size_t>(scores, 1) * sizeof(float)));
+    a.scores = kv->ws_scores.as<float>();
+  }
+  VG_CU(launch_kv_attend_decode(a, plan, s));
+  if (split) VG_CU(launch_kv_attend_join(a, plan, kDecodeRows, max_rows, s));
+  if (keep) {
+    VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, kWeighTile); }));
+    VG_CU(launch_kv_weigh_scores(a, plan, s));
+  } else if (a.lse2) {
+    VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, 4); }));
+    VG_CU(launch_kv_weigh_rows(a, plan, s));
+  }
+  return VG_OK;
+}
+
+int attend_rows(vg_kv_cache *, const AttendArgs &a, Plan &plan, cudaStream_t s) {
+  VG_TRY(set_units(plan, [](const PlanSeq &e) { return e.count; }));
+  VG_CU(launch_kv_attend_rows(a, plan, s));
+  if (a.lse2) {
+    VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, 4); }));
+    VG_CU(launch_kv_weigh_rows(a, plan, s));
   }
   return VG_OK;
 }
@@ -165,7 +257,7 @@ int vg_kv_get_info(const vg_kv_cache *kv, vg_kv_info *out) {
     out->block_tokens = kv->params.block_tokens;
     out->weight_stride = kv->view.stride;
     out->device_bytes = kv->codes[0].cap + kv->codes[1].cap + kv->scales[0].cap + kv->scales[1].cap + kv->weights.cap +
-                        kv->ws_lse.cap + kv->ws_kept.cap;
+                        kv->ws_lse.cap + kv->ws_kept.cap + kv->ws_part.cap + kv->ws_scores.cap;
     out->device = kv->device;
     return VG_OK;
   });
@@ -260,18 +352,16 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     a.group = a.q_heads / kv->view.heads;
     a.scale = scale;
     a.causal = (flags & VG_KV_CAUSAL) != 0;
-    if (!lse) {
-      VG_CU(kv->ws_lse.reserve(rows * a.q_heads * sizeof(float)));
-      lse = kv->ws_lse.as<float>();
-    }
     a.lse = lse;
-    VG_TRY(for_plans(
-        kv, counts, [&](size_t, PlanSeq &e) { return e.count; },
-        [&](const Plan &plan) { return launch_kv_attend_rows(a, plan, s); }));
-    if (flags & VG_KV_ACCUMULATE)
-      VG_TRY(for_plans(
-          kv, counts, [&](size_t, PlanSeq &e) { return ceil_div(e.len, 4); },
-          [&](const Plan &plan) { return launch_kv_weigh_rows(a, plan, s); }));
+    if (flags & VG_KV_ACCUMULATE) {
+      VG_CU(kv->ws_lse.reserve(rows * a.q_heads * sizeof(float)));
+      a.lse2 = kv->ws_lse.as<float>();
+    }
+    const auto few = [&](uint32_t count) { return count <= kDecodeRows / a.group; };
+    const auto no_units = [](size_t, PlanSeq &) { return 0u; };
+    VG_TRY(for_plans_of(kv, counts, few, no_units, [&](Plan &plan) { return attend_decode(kv, a, plan, s); }));
+    VG_TRY(for_plans_of(kv, counts, [&](uint32_t c) { return !few(c); }, no_units,
+                        [&](Plan &plan) { return attend_rows(kv, a, plan, s); }));
     return VG_OK;
   });
 }

@@ -36,6 +36,8 @@ struct PlanSeq {
   uint32_t count;  // tokens of this call
   uint32_t row0;   // first of them in the packed tensors
   uint32_t unit0;
+  uint32_t pad;
+  uint64_t aux;    // offset of its scores
 };
 struct Plan {
   uint32_t n, units;
@@ -86,6 +88,8 @@ cudaError_t launch_kv_gather(const KvView &kv, const Plan &plan, uint32_t budget
                              cudaStream_t s);
 
 // ---- kv_attend.cu ----
+constexpr int kDecodeRows = 16;      // rows (queries x heads that share a key/value head) of the decoding kernel
+constexpr uint32_t kMaxSplits = 512;  // chunks of one sequence that are joined
 struct AttendArgs {
   KvView kv;
   int dtype;
@@ -93,8 +97,26 @@ struct AttendArgs {
   uint32_t q_heads, group;
   float scale;      // softmax scale
   bool causal;
-  float *lse;       // [rows][q_heads]
+  float *lse;       // [rows][q_heads] natural log (nullable)
+  float *lse2;      // [rows][q_heads] log2, for the weights (nullable)
+  // Splitting over the tokens: a unit takes `chunk` tokens; a sequence of more
+  // than one unit leaves [unit][head][row of 16 or 128] partial sums
+  uint32_t chunk;
+  float *part_o;    // [..][dim]
+  float2 *part_ml;  // [..] (reference mu, denominator)
+  // Scores x of the call's rows, for the weights (nullable): entry e has
+  // [heads][rows][len rounded up to 16] from scores + plan.s[e].aux
+  float *scores;
 };
+// Sequences of at most kDecodeRows rows per key/value head.  Units: chunks (at least one per sequence).
+cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+// Joins the partial sums of sequences that have more than one unit.
+cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, int part_rows, uint32_t max_rows,
+                                  cudaStream_t s);
+// Adds the probabilities of stored scores to the weights.  Units: kWeighTile tokens.
+constexpr uint32_t kWeighTile = 256;
+cudaError_t launch_kv_weigh_scores(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+
 cudaError_t launch_kv_attend_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s);
 cudaError_t launch_kv_weigh_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s);
 
