@@ -63,23 +63,6 @@ __device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint3
   }
 }
 
-// The result of one row from its sums: 8 dimensions from c on, and the lse.
-template <class T>
-__device__ __forceinline__ void finish_row(const AttendArgs &a, size_t token, uint32_t hq, uint32_t c, bool ovec,
-                                           float mu, float sum, float (&y)[8]) {
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no token seen: 0
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] *= inv;
-  store8(static_cast<T *>(a.out.p) + static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head +
-             c,
-         ovec, y);
-  if (c == 0) {
-    const float lse2 = sum == 0.0f ? -VG_INF : mu - kPShift + log2f(sum);
-    if (a.lse) a.lse[token * a.q_heads + hq] = lse2 * kLn2;
-    if (a.lse2) a.lse2[token * a.q_heads + hq] = lse2;
-  }
-}
-
 template <class T, int D, bool kScores>
 __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const __grid_constant__ AttendArgs a,
                                                                           const __grid_constant__ Plan plan,
@@ -321,7 +304,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
 
 // ---- joining the chunks of a sequence -------------------------------------------
 
-// One CTA per (sequence, head, row): 16-byte slices of the row's partial sums,
+// One CTA per (row, head, sequence): 32-byte slices of the row's partial sums,
 // groups of threads taking every kGroups-th chunk.
 constexpr int kJoinThreads = 256;
 
@@ -332,12 +315,15 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   __shared__ float weight[kMaxSplits];
   __shared__ float red[kJoinThreads / 32];
   __shared__ float acc[kJoinThreads * 8];
-  const PlanSeq &ps = plan.s[blockIdx.x];
-  const uint32_t head = blockIdx.y, row = blockIdx.z, D = a.kv.dim;
-  if (ps.len <= a.chunk || row >= ps.count * a.group) return;
+  const PlanSeq &ps = plan.s[blockIdx.z];
+  const uint32_t head = blockIdx.y, row = blockIdx.x, D = a.kv.dim, rows = ps.count * a.group;
+  if (ps.len <= a.chunk || row >= rows) return;
   const uint32_t ns = (ps.len + a.chunk - 1) / a.chunk;
   const size_t step = static_cast<size_t>(a.kv.heads) * part_rows;
-  const size_t first = (static_cast<size_t>(ps.unit0) * a.kv.heads + head) * part_rows + row;
+  // a sequence's units: its row blocks, the last one first, and the chunks of each
+  const uint32_t block = (rows + part_rows - 1) / part_rows - 1 - row / part_rows;
+  const size_t first =
+      ((static_cast<size_t>(ps.unit0) + block * ns) * a.kv.heads + head) * part_rows + row % part_rows;
   const int warp = threadIdx.x >> 5;
   float m = -VG_INF;
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) m = fmaxf(m, a.part_ml[first + i * step].x);
@@ -404,88 +390,6 @@ __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_c
   *w += sum;
 }
 
-// ---- more rows -----------------------------------------------------------------
-
-constexpr int kRowWarps = 4;
-
-// First version: one warp per (query row, head), the tokens one after another
-// with a running maximum and sum; a lane holds dim / 32 dimensions.
-template <class T>
-__global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const __grid_constant__ AttendArgs a,
-                                                                     const __grid_constant__ Plan plan) {
-  const PlanSeq &ps = plan.s[plan_find(plan, blockIdx.x)];
-  const uint32_t j = blockIdx.x - ps.unit0, h = blockIdx.y * kRowWarps + (threadIdx.x >> 5);
-  if (h >= a.q_heads) return;
-  const int lane = lane_id();
-  const KvView &kv = a.kv;
-  const size_t r = static_cast<size_t>(ps.seq) * kv.heads + h / a.group;
-  const uint32_t per = kv.dim / 32;
-  const T *q = static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + j) * a.q.token +
-               static_cast<int64_t>(h) * a.q.head;
-  float qv[4], o[4] = {};
-  for (uint32_t i = 0; i < 4; ++i) qv[i] = i < per ? to_f32(q[lane + 32 * i]) * a.scale : 0.0f;
-  const uint32_t behind = ps.count - 1 - j;
-  const uint32_t sees = a.causal ? (ps.len > behind ? ps.len - behind : 0) : ps.len;
-  const size_t nb = kv.stride >> kv.block_shift;
-  const int8_t *kc = kv.codes[0] + r * kv.stride * kv.dim, *vc = kv.codes[1] + r * kv.stride * kv.dim;
-  const float *ks = kv.scales[0] + r * nb, *vs = kv.scales[1] + r * nb;
-  float m = -__int_as_float(0x7f800000), l = 0.0f;
-  for (uint32_t t = 0; t < sees; ++t) {
-    float d = 0.0f;
-    for (uint32_t i = 0; i < per; ++i) d += qv[i] * static_cast<float>(kc[static_cast<size_t>(t) * kv.dim + lane + 32 * i]);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(VG_FULL_MASK, d, w);
-    const float s = d * ks[t >> kv.block_shift];
-    const float mn = s > m || s != s ? s : m;
-    const float c = expf(m - mn), p = expf(s - mn);
-    l = l * c + p;
-    const float pv = p * vs[t >> kv.block_shift];
-    for (uint32_t i = 0; i < per; ++i)
-      o[i] = o[i] * c + pv * static_cast<float>(vc[static_cast<size_t>(t) * kv.dim + lane + 32 * i]);
-    m = mn;
-  }
-  T *out = static_cast<T *>(a.out.p) + static_cast<int64_t>(ps.row0 + j) * a.out.token +
-           static_cast<int64_t>(h) * a.out.head;
-  for (uint32_t i = 0; i < per; ++i) out[lane + 32 * i] = from_f32<T>(sees ? o[i] / l : 0.0f);
-  if (lane == 0) {
-    const size_t at = static_cast<size_t>(ps.row0 + j) * a.q_heads + h;
-    if (a.lse) a.lse[at] = m + logf(l);
-    if (a.lse2) a.lse2[at] = (m + logf(l)) * kLog2e;
-  }
-}
-
-// One warp per (cached token, key/value head): its probabilities, recomputed
-// from the rows' lse, summed over the queries and heads that share it.
-template <class T>
-__global__ void __launch_bounds__(kRowWarps * 32) weigh_rows_kernel(const __grid_constant__ AttendArgs a,
-                                                                    const __grid_constant__ Plan plan) {
-  const PlanSeq &ps = plan.s[plan_find(plan, blockIdx.x)];
-  const uint32_t t = (blockIdx.x - ps.unit0) * kRowWarps + (threadIdx.x >> 5), g = blockIdx.y;
-  if (t >= ps.len) return;
-  const int lane = lane_id();
-  const KvView &kv = a.kv;
-  const size_t r = static_cast<size_t>(ps.seq) * kv.heads + g;
-  const uint32_t per = kv.dim / 32;
-  const float ks = kv.scales[0][r * (kv.stride >> kv.block_shift) + (t >> kv.block_shift)] * a.scale;
-  float kvv[4];
-  for (uint32_t i = 0; i < 4; ++i)
-    kvv[i] = i < per ? ks * static_cast<float>(kv.codes[0][(r * kv.stride + t) * kv.dim + lane + 32 * i]) : 0.0f;
-  float sum = 0.0f;
-  for (uint32_t j = 0; j < ps.count; ++j) {
-    if (a.causal && t + (ps.count - 1 - j) >= ps.len) continue;
-    for (uint32_t h = g * a.group; h < (g + 1) * a.group; ++h) {
-      const T *q = static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + j) * a.q.token +
-                   static_cast<int64_t>(h) * a.q.head;
-      float d = 0.0f;
-      for (uint32_t i = 0; i < per; ++i) d += to_f32(q[lane + 32 * i]) * kvv[i];
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(VG_FULL_MASK, d, w);
-      sum += exp2f(d * kLog2e - a.lse2[static_cast<size_t>(ps.row0 + j) * a.q_heads + h]);
-    }
-  }
-  if (lane == 0) kv.weights[r * kv.stride + t] += sum;
-}
-
 template <class T, int D>
 cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   auto *kern = a.scores ? attend_decode_kernel<T, D, true> : attend_decode_kernel<T, D, false>;
@@ -514,9 +418,9 @@ cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, cudaS
   return a.dtype == VG_F16 ? decode_dim<__half>(a, plan, s) : decode_dim<__nv_bfloat16>(a, plan, s);
 }
 
-cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, int part_rows, uint32_t max_rows,
+cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, uint32_t part_rows, uint32_t max_rows,
                                   cudaStream_t s) {
-  const dim3 grid(plan.n, a.kv.heads, max_rows);
+  const dim3 grid(max_rows, a.kv.heads, plan.n);
   const bool vec = rows_aligned(a.out, 2);
   if (a.dtype == VG_F16) attend_join_kernel<__half><<<grid, kJoinThreads, 0, s>>>(a, plan, part_rows, vec);
   else attend_join_kernel<__nv_bfloat16><<<grid, kJoinThreads, 0, s>>>(a, plan, part_rows, vec);
@@ -526,22 +430,6 @@ cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, int par
 cudaError_t launch_kv_weigh_scores(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
   weigh_scores_kernel<<<dim3(plan.units, a.kv.heads), kWeighTile, 0, s>>>(a, plan);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_kv_attend_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  if (plan.units == 0) return cudaSuccess;
-  const dim3 grid(plan.units, (a.q_heads + kRowWarps - 1) / kRowWarps);
-  if (a.dtype == VG_F16) attend_rows_kernel<__half><<<grid, kRowWarps * 32, 0, s>>>(a, plan);
-  else attend_rows_kernel<__nv_bfloat16><<<grid, kRowWarps * 32, 0, s>>>(a, plan);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_kv_weigh_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  if (plan.units == 0) return cudaSuccess;
-  const dim3 grid(plan.units, a.kv.heads);
-  if (a.dtype == VG_F16) weigh_rows_kernel<__half><<<grid, kRowWarps * 32, 0, s>>>(a, plan);
-  else weigh_rows_kernel<__nv_bfloat16><<<grid, kRowWarps * 32, 0, s>>>(a, plan);
   return cudaGetLastError();
 }
 

@@ -1,0 +1,748 @@
+// Attention of many queries over the 8-bit cache on the 5th-generation tensor
+// cores (tcgen05), and the weights of its tokens.
+//
+// The rows of a key/value head are its queries times the query heads that share
+// it; a tile is 128 rows (the lanes of the TMEM accumulator) by 128 tokens.
+// Bound by the exponentials and the products: 4 dim multiply-adds' worth of
+// tensor work and one ex2 per (row, token), the codes being read from L2 by
+// every row block.  See kv_attend.cu for the scaling of scores and
+// probabilities.
+//
+// attend_tile_kernel, one CTA per (sequence, head, 128 rows, chunk of tokens),
+// two CTAs on an SM so that one's products fill the other's softmax:
+//   warps 0..3  softmax: one row per thread, S from TMEM, P back into its place
+//   warps 4..7  load codes, convert them to binary16 tiles in shared memory
+//               (keys as they are; values transposed: tokens are the
+//               contraction of the second product)
+//   warp 8      copies the query tile, issues S = Q K^T and O += P V
+// Every wait is bounded: a protocol error sets the error flag and the kernel
+// drains its copies and products, frees its TMEM and returns.
+#include "common.cuh"
+#include "elements.cuh"
+#include "f32x2.cuh"
+#include "kv_attend.cuh"
+#include "kv_cache.h"
+#include "umma.cuh"
+
+#include <algorithm>
+
+namespace vg {
+
+namespace {
+
+constexpr int kRows = kTileRows;              // 128
+constexpr uint32_t kTok = 128;                // tokens per tile
+constexpr uint32_t kKBlockBytes = kRows * 128;  // 64 binary16 columns of a 128-row tile
+constexpr int kThreads = 288;
+constexpr uint32_t kTmemColumns = 256;        // S (P in its first half) and O, or two S
+
+__device__ __forceinline__ uint32_t f16_idesc(uint32_t n) {  // D f32, A and B binary16 K-major, M = 128
+  return (1u << 4) | ((n >> 3) << 17) | ((kRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// A from TMEM: binary16 pairs, 8 columns per K-step of 16
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t *v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Byte of (row, 16-byte chunk c of 8 binary16 columns) in a K-major tile of 128-byte swizzled rows.
+__device__ __forceinline__ uint32_t tile_byte(uint32_t rows, uint32_t row, uint32_t c) {
+  return (c >> 3) * (rows * 128) + row * 128 + (((c & 7u) ^ (row & 7u)) << 4);
+}
+
+// ---- key tile: 128 tokens x D, as they lie -------------------------------------
+
+// 16 codes each: item = (token, 16-byte chunk)
+template <int D, int kWorkers>
+struct KeyTile {
+  static constexpr int kItems = kTok * (D / 16) / kWorkers;
+  uint4 w[kItems];
+  __device__ __forceinline__ void load(const int8_t *codes, uint32_t tid) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(codes) + tid + i * kWorkers);
+  }
+  __device__ __forceinline__ void store(uint8_t *tile, uint32_t tid) const {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t e = tid + i * kWorkers, tok = e / (D / 16), c = e % (D / 16);
+      const uint32_t x[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // the lanes of the second K-block store their halves in the other
+        // order: eight lanes of a token meet eight different bank groups
+        const uint32_t hh = (c & 4u) ? 1 - h : h;
+        const uint32_t a = hh ? x[2] : x[0], b = hh ? x[3] : x[1];
+        *reinterpret_cast<uint4 *>(tile + tile_byte(kTok, tok, 2 * c + hh)) =
+            make_uint4(half2_of<0x4140>(a), half2_of<0x4342>(a), half2_of<0x4140>(b), half2_of<0x4342>(b));
+      }
+    }
+  }
+};
+
+// ---- value tile: D x 128 tokens -------------------------------------------------
+
+// Item = (8 tokens, 4 dimensions): a word of each token, transposed in
+// registers.  Dimension 4 i + d is row d D/4 + i of the tile, so that
+// neighbouring lanes store neighbouring rows (no bank conflicts).
+template <int D>
+struct ValueTile {
+  static constexpr int kItems = (kTok / 8) * (D / 4) / 128;
+  uint32_t w[kItems][8];
+  __device__ __forceinline__ void load(const int8_t *codes, uint32_t tid) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t e = tid + i * 128, u = e / (D / 4), c = e % (D / 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[i][k] = __ldg(reinterpret_cast<const uint32_t *>(codes) + (u * 8 + k) * (D / 4) + c);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t *tile, uint32_t tid) const {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t e = tid + i * 128, u = e / (D / 4), c = e % (D / 4);
+      uint32_t out[4][4];  // [dimension][token pair]
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t a = __byte_perm(w[i][2 * k], w[i][2 * k + 1], 0x5140) ^ 0x80808080u;
+        const uint32_t b = __byte_perm(w[i][2 * k], w[i][2 * k + 1], 0x7362) ^ 0x80808080u;
+        out[0][k] = half2_of<0x4140>(a);
+        out[1][k] = half2_of<0x4342>(a);
+        out[2][k] = half2_of<0x4140>(b);
+        out[3][k] = half2_of<0x4342>(b);
+      }
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        *reinterpret_cast<uint4 *>(tile + tile_byte(D, d * (D / 4) + c, u)) =
+            make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
+    }
+  }
+};
+
+// ---- query tiles -----------------------------------------------------------------
+
+// Rows of a block of 128 as a binary16 tile, each scaled by a power of two
+// into the range (and by the sign of the softmax scale), with the factor that
+// turns its products with key codes times their scale into scores.
+constexpr int kImageThreads = 256;
+
+template <class T>
+__global__ void __launch_bounds__(kImageThreads) query_tiles_kernel(const __grid_constant__ AttendArgs a,
+                                                                    const __grid_constant__ Plan plan,
+                                                                    const uint32_t blocks, const bool qvec) {
+  const uint32_t D = a.kv.dim, head = blockIdx.y;
+  uint32_t lo = 0, hi = plan.n;  // the entry that row block blockIdx.x belongs to
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (plan.s[mid].block0 <= blockIdx.x) lo = mid;
+    else hi = mid;
+  }
+  const PlanSeq &ps = plan.s[lo];
+  const uint32_t rows = ps.count * a.group, c = threadIdx.x & 15, sub = threadIdx.x >> 4;
+  const size_t at = static_cast<size_t>(blockIdx.x) * a.kv.heads + head;
+  uint8_t *tile = a.q_tiles + at * ((D + 63) / 64) * kKBlockBytes;
+  float *qf = a.q_factor + at * kRows;
+  const bool neg = a.scale < 0.0f;
+  for (uint32_t r = sub; r < kRows; r += kImageThreads / 16) {
+    const uint32_t row = (blockIdx.x - ps.block0) * kRows + r;
+    float x[8] = {};
+    if (row < rows && c < D / 8) {
+      const uint32_t qi = row / a.group;
+      load8(static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + qi) * a.q.token +
+                static_cast<int64_t>(head * a.group + row - qi * a.group) * a.q.head + c * 8,
+            qvec, x);
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(VG_FULL_MASK, top, w));
+    float s, inv;
+    row_scale(top, s, inv);
+    if (neg) inv = -inv;
+    if (c < D / 8)
+      *reinterpret_cast<uint4 *>(tile + tile_byte(kRows, r, c)) =
+          make_uint4(pack_half2(x[0] * inv, x[1] * inv), pack_half2(x[2] * inv, x[3] * inv),
+                     pack_half2(x[4] * inv, x[5] * inv), pack_half2(x[6] * inv, x[7] * inv));
+    if (c == 0) qf[r] = row < rows ? s * fabsf(a.scale) * kLog2e : 0.0f;
+  }
+}
+
+// ---- attention ---------------------------------------------------------------------
+
+template <int D>
+constexpr size_t tile_smem() {
+  return 1024 + 2 * ((D + 63) / 64) * kKBlockBytes + 2 * D * 128 + 128;
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_constant__ AttendArgs a,
+                                                                  const __grid_constant__ Plan plan,
+                                                                  const bool ovec) {
+  extern __shared__ uint8_t tile_raw[];
+  const uint32_t raw = smem_u32(tile_raw);
+  uint8_t *sm = tile_raw + (((raw + 1023u) & ~1023u) - raw);  // swizzled tiles need 1024-byte alignment
+  constexpr uint32_t kQBytes = ((D + 63) / 64) * kKBlockBytes, kVBytes = 2 * D * 128;
+  uint8_t *sQ = sm, *sK = sm + kQBytes, *sV = sK + kQBytes;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sV + kVBytes);
+  uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 2, *vfull = bars + 3, *vempty = bars + 4,
+           *sfull = bars + 5, *pfull = bars + 6, *drain = bars + 7;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 8);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = lane_id();
+
+  const KvView &kv = a.kv;
+  const uint32_t unit = blockIdx.x, head = blockIdx.y;
+  const PlanSeq &ps = plan.s[plan_find(plan, unit)];
+  const uint32_t rows = ps.count * a.group, ns = max(1u, (ps.len + a.chunk - 1) / a.chunk);
+  const uint32_t nrb = (rows + kRows - 1) / kRows;
+  const uint32_t rb = nrb - 1 - (unit - ps.unit0) / ns, sp = (unit - ps.unit0) % ns;  // last rows, which see most, first
+  const uint32_t last = min(rows, (rb + 1) * kRows) - 1;
+  const uint32_t t0 = sp * a.chunk, t1 = min(tokens_seen(ps, last / a.group, a.causal), t0 + a.chunk);
+  const uint32_t tiles = t1 > t0 ? (t1 - t0 + kTok - 1) / kTok : 0;
+  const size_t r = static_cast<size_t>(ps.seq) * kv.heads + head, nb = kv.stride >> kv.block_shift;
+
+  if (threadIdx.x == 0) {
+    mbar_init(qfull, 1);
+    mbar_init(kfull, 4);
+    mbar_init(kempty, 1);
+    mbar_init(vfull, 4);
+    mbar_init(vempty, 1);
+    mbar_init(sfull, 1);
+    mbar_init(pfull, 4);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tS = tmem, tO = tmem + kTok;
+  auto give_up = [&](int code) {
+    *abort_flag = 1;
+    if (a.error) *reinterpret_cast<volatile int *>(a.error) = code;
+  };
+
+  if (warp == 8) {
+    // ---- query tile and products ----
+    if (lane == 0 && tiles) {
+      const size_t at = static_cast<size_t>(ps.block0 + rb) * kv.heads + head;
+      mbar_arrive_expect_tx(qfull, kQBytes);
+      bulk_copy_g2s(sQ, a.q_tiles + at * kQBytes, kQBytes, qfull);
+      bool ok = mbar_wait_sleep(qfull, 0);
+      const uint32_t bQ = smem_u32(sQ), bK = smem_u32(sK), bV = smem_u32(sV);
+      for (uint32_t i = 0; ok && i < tiles; ++i) {
+        // S: the keys are there, and the previous tile's P (in S's place) has been used
+        if (*abort_flag || !mbar_wait_sleep(kfull, i & 1) || (i && !mbar_wait_sleep(vempty, (i - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * kKBlockBytes + (k & 3) * 32;
+          umma_ss(tS, umma_desc(bQ + off), umma_desc(bK + off), f16_idesc(kTok), k != 0);
+        }
+        umma_commit(kempty);
+        umma_commit(sfull);
+        if (!mbar_wait_sleep(vfull, i & 1) || !mbar_wait_sleep(pfull, i & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < static_cast<int>(kTok) / 16; ++k)
+          umma_ts(tO, tS + k * 8, umma_desc(bV + (k >> 2) * (D * 128) + (k & 3) * 32), f16_idesc(D), i != 0 || k != 0);
+        umma_commit(vempty);
+      }
+      if (!ok) give_up(1);
+      umma_commit(drain);  // every product issued is complete before TMEM is released
+      mbar_wait(drain, 0);
+    }
+  } else if (warp >= 4) {
+    // ---- codes to binary16 tiles ----
+    const uint32_t tid = threadIdx.x - 128;
+    const int8_t *kc = kv.codes[0] + (r * kv.stride + t0) * D, *vc = kv.codes[1] + (r * kv.stride + t0) * D;
+    KeyTile<D, 128> key;
+    ValueTile<D> value;
+    if (tiles) key.load(kc, tid);
+    bool ok = true;
+    for (uint32_t i = 0; i < tiles; ++i) {
+      value.load(vc + static_cast<size_t>(i) * kTok * D, tid);
+      if (!__all_sync(VG_FULL_MASK, !i || mbar_wait_sleep(kempty, (i - 1) & 1))) {
+        ok = false;
+        break;
+      }
+      key.store(sK, tid);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kfull);
+      if (i + 1 < tiles) key.load(kc + static_cast<size_t>(i + 1) * kTok * D, tid);
+      if (!__all_sync(VG_FULL_MASK, !i || mbar_wait_sleep(vempty, (i - 1) & 1))) {
+        ok = false;
+        break;
+      }
+      value.store(sV, tid);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(vfull);
+    }
+    if (!ok) give_up(2);
+  } else {
+    // ---- softmax: thread = row = TMEM lane ----
+    const uint32_t row = rb * kRows + threadIdx.x;
+    const bool valid = row < rows;
+    const uint32_t qi = row / a.group;
+    const uint32_t lim = valid ? tokens_seen(ps, qi, a.causal) : 0xffffffffu;
+    const uint32_t warp_lim = __reduce_min_sync(VG_FULL_MASK, lim);
+    const float f_row =
+        a.q_factor[(static_cast<size_t>(ps.block0 + rb) * kv.heads + head) * kRows + threadIdx.x];
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t pS = tS + lane_base, pO = tO + lane_base;
+    // lanes 0..7 and 8..15 hold the key and value scales of a tile's eight 16-token groups
+    const float *scales = kv.scales[lane >> 3 & 1] + r * nb;
+    auto scale_at = [&](uint32_t t) {
+      const uint32_t at = t + (lane & 7) * 16;
+      return lane < 16 && at < ps.len ? __ldg(scales + (at >> kv.block_shift)) : 1.0f;
+    };
+    float next = tiles ? scale_at(t0) : 1.0f;
+    float mu = -VG_INF, l = 0.0f;
+    bool ok = true;
+    for (uint32_t i = 0; i < tiles; ++i) {
+      const uint32_t t = t0 + i * kTok;
+      const float sc = next;
+      if (i + 1 < tiles) next = scale_at(t + kTok);
+      if (!__all_sync(VG_FULL_MASK, mbar_wait_sleep(sfull, i & 1))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float m = -VG_INF;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld32_nowait(pS + c * 32, v);
+        tmem_wait_ld();
+        if (t + (c + 1) * 32 > warp_lim) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (t + c * 32 + k >= lim) v[k] = 0xff800000u;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float f = f_row * __shfl_sync(VG_FULL_MASK, sc, 2 * c + g);
+          const float lv = log2_scale(__shfl_sync(VG_FULL_MASK, sc, 8 + 2 * c + g));
+          float x = -VG_INF;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x = fmaxf(x, __uint_as_float(v[16 * g + k]));
+          m = fmaxf(m, x * f + lv);  // NaN (-inf times 0: nothing seen) is passed over
+        }
+      }
+      if (__any_sync(VG_FULL_MASK, m > mu + kLazy)) {
+        m = fmaxf(m, mu);
+        const float c = m == -VG_INF ? 1.0f : exp2_approx(mu - m);
+        mu = m;
+        l *= c;
+        if (i) {
+#pragma unroll 1
+          for (int b = 0; b < D; b += 16) {
+            uint32_t v[16];
+            tmem_ld8_nowait(pO + b, v);
+            tmem_ld8_nowait(pO + b + 8, v + 8);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * c);
+            tmem_st16(pO + b, v);
+          }
+        }
+      }
+      const float base = kPShift - (mu == -VG_INF ? 0.0f : mu);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32], p[16];
+        tmem_ld32_nowait(pS + c * 32, v);
+        tmem_wait_ld();
+        const bool edge = t + (c + 1) * 32 > warp_lim;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float f = f_row * __shfl_sync(VG_FULL_MASK, sc, 2 * c + g);
+          const float vscale = __shfl_sync(VG_FULL_MASK, sc, 8 + 2 * c + g);
+          const float ref = base + log2_scale(vscale);
+          const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
+          f32x2 sum2 = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int e = 16 * g + 2 * k;
+            float2 x = f2_unpack(
+                f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2, ref2));
+            x.x = exp2_approx(x.x);
+            x.y = exp2_approx(x.y);
+            if (edge) {
+              if (t + c * 32 + e >= lim) x.x = 0.0f;
+              if (t + c * 32 + e + 1 >= lim) x.y = 0.0f;
+            }
+            sum2 = f2_add(sum2, f2_pack(x.x, x.y));
+            p[8 * g + k] = pack_half2(x.x, x.y);
+          }
+          const float2 sum = f2_unpack(sum2);
+          l += (sum.x + sum.y) * inverse_scale(vscale);
+          if (vscale != vscale) {  // the values read as NaN: so does every row that sees one of them
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t col = t + c * 32 + 16 * g + 2 * k;
+              if (col < lim) p[8 * g + k] = (p[8 * g + k] & 0xffff0000u) | 0x7fffu;
+              if (col + 1 < lim) p[8 * g + k] |= 0x7fff0000u;
+            }
+          }
+        }
+        tmem_st16(pS + c * 16, p);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull);
+    }
+    if (ok && tiles) {
+      ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(vempty, (tiles - 1) & 1));
+      tc_fence_after();
+    }
+    if (ok) {
+      const bool whole = ps.len <= a.chunk;
+      const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kRows + threadIdx.x;
+#pragma unroll 1
+      for (int b = 0; b < D / 4; b += 8) {  // dimensions 4 b .. 4 b + 31
+        uint32_t v[4][8] = {};
+        if (tiles) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d) tmem_ld8_nowait(pO + d * (D / 4) + b, v[d]);
+          tmem_wait_ld();
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float y[8];
+#pragma unroll
+          for (int d = 0; d < 8; ++d) y[d] = __uint_as_float(v[d & 3][2 * k + (d >> 2)]);
+          const uint32_t c = 4 * b + 8 * k;
+          if (whole) {
+            finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, l, y);
+          } else {
+            float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D + c);
+            dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+            dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+          }
+        }
+      }
+      if (!whole && valid) a.part_ml[at] = make_float2(mu, l);
+    } else {
+      give_up(3);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+  }
+}
+
+// ---- weights -------------------------------------------------------------------------
+
+// One CTA per (sequence, head, 128 tokens): the scores of every row block
+// again, transposed (tokens in the lanes), and the sum of a token's
+// probabilities 2^(x - lse) in a register.
+//   warps 0..7  convert the key tile, then, alternating row blocks, one token
+//               per thread
+//   warp 8      copies query tiles (two in flight), issues K Q^T
+template <int D>
+constexpr size_t weigh_smem() {
+  return 1024 + 3 * ((D + 63) / 64) * kKBlockBytes + 2 * kRows * (8 + 4) + kTok * 4 + 128;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_constant__ AttendArgs a,
+                                                                 const __grid_constant__ Plan plan) {
+  extern __shared__ uint8_t weigh_raw[];
+  const uint32_t raw = smem_u32(weigh_raw);
+  uint8_t *sm = weigh_raw + (((raw + 1023u) & ~1023u) - raw);
+  constexpr uint32_t kQBytes = ((D + 63) / 64) * kKBlockBytes;
+  uint8_t *sK = sm, *sQ = sm + kQBytes;  // two query tiles
+  float4 *row_f = reinterpret_cast<float4 *>(sQ + 2 * kQBytes);      // [2][64] (factor, factor, -lse, -lse) of a row pair
+  uint32_t *row_lim = reinterpret_cast<uint32_t *>(row_f + 2 * 64);  // [2][128]
+  float *half = reinterpret_cast<float *>(row_lim + 2 * kRows);      // [128]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(half + kTok);
+  uint64_t *kfull = bars, *qfull = bars + 1, *qempty = bars + 3, *sfull = bars + 5, *sempty = bars + 7, *drain = bars + 9;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = lane_id();
+
+  const KvView &kv = a.kv;
+  const uint32_t unit = blockIdx.x, head = blockIdx.y;
+  const PlanSeq &ps = plan.s[plan_find(plan, unit)];
+  const uint32_t t0 = (unit - ps.unit0) * kTok;
+  const uint32_t rows = ps.count * a.group, nrb = (rows + kRows - 1) / kRows;
+  const size_t r = static_cast<size_t>(ps.seq) * kv.heads + head;
+  // the first row block with a row that sees the tile's first token
+  uint32_t rb0 = 0;
+  if (a.causal && ps.len > t0) {
+    const uint32_t after = ps.len - 1 - t0;                    // query qi sees t0 if count - 1 - qi <= after
+    if (ps.count - 1 > after) rb0 = (ps.count - 1 - after) * a.group / kRows;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(kfull, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(qfull + i, 1);
+      mbar_init(qempty + i, 1);
+      mbar_init(sfull + i, 1);
+      mbar_init(sempty + i, 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto give_up = [&](int code) {
+    *abort_flag = 1;
+    if (a.error) *reinterpret_cast<volatile int *>(a.error) = code;
+  };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const uint32_t bK = smem_u32(sK);
+      const uint32_t n = nrb - rb0;
+      auto copy = [&](uint32_t i) {  // row block rb0 + i into stage i & 1
+        const size_t at = static_cast<size_t>(ps.block0 + rb0 + i) * kv.heads + head;
+        mbar_arrive_expect_tx(qfull + (i & 1), kQBytes);
+        bulk_copy_g2s(sQ + (i & 1) * kQBytes, a.q_tiles + at * kQBytes, kQBytes, qfull + (i & 1));
+      };
+      uint32_t copied = 0;
+      for (; copied < min(n, 2u); ++copied) copy(copied);
+      bool ok = mbar_wait_sleep(kfull, 0);
+      uint32_t i = 0;
+      for (; ok && i < n; ++i) {
+        const uint32_t st = i & 1, ph = (i >> 1) & 1;
+        if (*abort_flag || !mbar_wait_sleep(qfull + st, ph) || (i >= 2 && !mbar_wait_sleep(sempty + st, ph ^ 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t bQ = smem_u32(sQ + st * kQBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * kKBlockBytes + (k & 3) * 32;
+          umma_ss(tmem + st * kRows, umma_desc(bK + off), umma_desc(bQ + off), f16_idesc(kRows), k != 0);
+        }
+        umma_commit(qempty + st);
+        umma_commit(sfull + st);
+        if (i + 2 < n) {
+          if (!mbar_wait_sleep(qempty + st, ph)) {
+            ok = false;
+            break;
+          }
+          copy(copied++);
+        }
+      }
+      if (!ok) {
+        give_up(4);
+        // copies still in flight land in shared memory: wait for them (bounded)
+        for (uint32_t c = copied > 2 ? copied - 2 : 0; c < copied; ++c) mbar_wait(qfull + (c & 1), (c >> 1) & 1);
+      }
+      umma_commit(drain);
+      mbar_wait(drain, 0);
+    }
+  } else {
+    {
+      KeyTile<D, 256> key;
+      key.load(kv.codes[0] + (r * kv.stride + t0) * D, threadIdx.x);
+      key.store(sK, threadIdx.x);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kfull);
+    }
+    const int eg = warp >> 2, wl = threadIdx.x & 127;  // row blocks of this parity; token = TMEM lane
+    const uint32_t t = t0 + wl;
+    const uint32_t pS = tmem + eg * kRows + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float ks = t < ps.len ? kv.scales[0][r * (kv.stride >> kv.block_shift) + (t >> kv.block_shift)] : 0.0f;
+    const f32x2 ks2 = f2_pack(ks, ks);
+    float *my_f = reinterpret_cast<float *>(row_f + eg * 64);
+    uint32_t *my_lim = row_lim + eg * kRows;
+    float total = 0.0f;
+    bool ok = true;
+    for (uint32_t i = eg; i < nrb - rb0; i += 2) {
+      const uint32_t b = rb0 + i;
+      {
+        const uint32_t row = b * kRows + wl, qi = row / a.group;
+        float lse = VG_INF;  // rows past the end, or that see nothing: probability 0
+        uint32_t lim = 0;
+        if (row < rows) {
+          lim = tokens_seen(ps, qi, a.causal);
+          lse = a.lse2[(static_cast<size_t>(ps.row0) + qi) * a.q_heads + head * a.group + row - qi * a.group];
+          if (lse == -VG_INF) lse = VG_INF;
+        }
+        const float f = a.q_factor[(static_cast<size_t>(ps.block0 + b) * kv.heads + head) * kRows + wl];
+        named_sync(1 + eg, 128);  // the previous block's have been read
+        my_f[(wl >> 1) * 4 + (wl & 1)] = f;
+        my_f[(wl >> 1) * 4 + 2 + (wl & 1)] = -lse;
+        my_lim[wl] = lim;
+        named_sync(1 + eg, 128);
+      }
+      // rows are in the order of their queries: the first one sees least
+      const bool edge = my_lim[0] < t0 + kTok;
+      // after a wait that gave up the loop goes on, without waits, to keep the barriers in step
+      if (ok) ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(sfull + eg, (i >> 1) & 1));
+      tc_fence_after();
+      f32x2 sum2 = 0;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld32_nowait(pS + c * 32, v);
+        tmem_wait_ld();
+        if (c == 3) {  // in registers: the accumulator is free
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty + eg);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float4 w = reinterpret_cast<const float4 *>(my_f)[c * 16 + k];
+          const f32x2 x = f2_mul(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), ks2);
+          float2 p = f2_unpack(f2_fma(x, f2_pack(w.x, w.y), f2_pack(w.z, w.w)));
+          p.x = exp2_approx(p.x);
+          p.y = exp2_approx(p.y);
+          if (edge) {
+            if (t >= my_lim[c * 32 + 2 * k]) p.x = 0.0f;
+            if (t >= my_lim[c * 32 + 2 * k + 1]) p.y = 0.0f;
+          }
+          sum2 = f2_add(sum2, f2_pack(p.x, p.y));
+        }
+      }
+      const float2 sum = f2_unpack(sum2);
+      total += sum.x + sum.y;
+    }
+    if (!ok) give_up(5);
+    if (eg) half[wl] = total;
+    named_sync(3, 256);
+    if (!eg && t < ps.len) kv.weights[r * kv.stride + t] += total + half[wl];
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------------
+
+// At most two CTAs may be on an SM: each holds half of its TMEM.
+constexpr size_t kTwoPerSm = 80 * 1024;
+
+template <class T, int D>
+cudaError_t tile(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  auto *kern = attend_tile_kernel<T, D>;
+  const size_t smem = std::max(tile_smem<D>(), kTwoPerSm);
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  kern<<<dim3(plan.units, a.kv.heads), kThreads, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
+  return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t tile_type(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  return a.dtype == VG_F16 ? tile<__half, D>(a, plan, s) : tile<__nv_bfloat16, D>(a, plan, s);
+}
+
+template <int D>
+cudaError_t weigh(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  auto *kern = weigh_tile_kernel<D>;
+  const size_t smem = std::max(weigh_smem<D>(), kTwoPerSm);
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  kern<<<dim3(plan.units, a.kv.heads), kThreads, smem, s>>>(a, plan);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t query_tile_bytes(uint32_t dim) { return ((dim + 63) / 64) * kKBlockBytes; }
+
+cudaError_t launch_kv_query_tiles(const AttendArgs &a, const Plan &plan, uint32_t blocks, cudaStream_t s) {
+  const dim3 grid(blocks, a.kv.heads);
+  const bool vec = rows_aligned(a.q, 2);
+  if (a.dtype == VG_F16) query_tiles_kernel<__half><<<grid, kImageThreads, 0, s>>>(a, plan, blocks, vec);
+  else query_tiles_kernel<__nv_bfloat16><<<grid, kImageThreads, 0, s>>>(a, plan, blocks, vec);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  if (plan.units == 0) return cudaSuccess;
+  switch (a.kv.dim) {
+    case 32: return tile_type<32>(a, plan, s);
+    case 64: return tile_type<64>(a, plan, s);
+    case 96: return tile_type<96>(a, plan, s);
+    default: return tile_type<128>(a, plan, s);
+  }
+}
+
+cudaError_t launch_kv_weigh_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+  if (plan.units == 0) return cudaSuccess;
+  switch (a.kv.dim) {
+    case 32: return weigh<32>(a, plan, s);
+    case 64: return weigh<64>(a, plan, s);
+    case 96: return weigh<96>(a, plan, s);
+    default: return weigh<128>(a, plan, s);
+  }
+}
+
+}  // namespace vg

@@ -17,7 +17,8 @@ struct vg_kv_cache {
   KvView view{};
   DevBuf codes[2], scales[2], weights;
   std::vector<uint32_t> len;  // tokens of each sequence once all enqueued work is done
-  DevBuf ws_lse, ws_kept, ws_part, ws_scores;
+  DevBuf ws_lse, ws_kept, ws_part, ws_scores, ws_tiles;
+  int *h_err = nullptr, *d_err = nullptr;  // error flag of bounded device waits, in mapped pinned host memory
   // Work is ordered across streams: each call's stream first waits for the
   // event recorded after the last call's work.
   cudaEvent_t done = nullptr;
@@ -27,6 +28,7 @@ struct vg_kv_cache {
       cudaEventSynchronize(done);
       cudaEventDestroy(done);
     }
+    if (h_err) cudaFreeHost(h_err);
   }
 };
 
@@ -44,6 +46,9 @@ class Work {
     VG_CU(cudaStreamIsCapturing(s_, &cap));
     if (cap != cudaStreamCaptureStatusNone)
       return fail(VG_ERR_UNSUPPORTED, "unsupported: key/value cache calls cannot be captured into a CUDA graph");
+    if (const int code = *reinterpret_cast<volatile int *>(kv_->h_err))
+      return fail(VG_ERR_CUDA, "an earlier attention call gave up a wait on the device (code " + std::to_string(code) +
+                                   "): its results are not valid");
     VG_CU(cudaStreamWaitEvent(s_, kv_->done, 0));
     begun_ = true;
     return VG_OK;
@@ -119,32 +124,77 @@ int set_units(Plan &plan, Units &&units_of) {
   return VG_OK;
 }
 
-// Tokens per work unit when every (sequence, head) is cut into chunks: the
-// smallest multiple of `quantum` that gives at most `slots` units, what the
-// GPU runs at once, or -- where the uncut sequences alone come near that --
-// four times as many, so that the last wave is a short one.
-uint32_t pick_chunk(const Plan &plan, uint64_t per_chunk, uint64_t slots, uint32_t quantum) {
+// Tokens per work unit when the tokens of every sequence are cut into chunks.
+// Units run `slots` at a time, so w waves of chunks of c tokens take about
+// w (c + overhead): of one to four full waves, and of leaving the sequences
+// whole, the cheapest.  per_chunk(entry): units of one chunk of it.
+template <class PerChunk>
+uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, uint32_t overhead, PerChunk &&per_chunk) {
   uint32_t longest = 1;
   for (uint32_t i = 0; i < plan.n; ++i) longest = std::max(longest, plan.s[i].len);
-  const uint64_t most = plan.n * per_chunk * 2 <= slots ? slots : 4 * slots;
-  uint32_t lo = std::max(1u, ceil_div(ceil_div(longest, kMaxSplits), quantum)), hi = std::max(lo, ceil_div(longest, quantum));
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    uint64_t units = 0;
-    for (uint32_t i = 0; i < plan.n; ++i) units += std::max(1u, ceil_div(plan.s[i].len, mid * quantum)) * per_chunk;
-    if (units <= most) hi = mid;
-    else lo = mid + 1;
+  const auto units = [&](uint32_t chunk) {
+    uint64_t n = 0;
+    for (uint32_t i = 0; i < plan.n; ++i) n += std::max(1u, ceil_div(plan.s[i].len, chunk)) * per_chunk(plan.s[i]);
+    return n;
+  };
+  const uint32_t least = std::max(1u, ceil_div(ceil_div(longest, kMaxSplits), quantum));
+  uint32_t best = std::max(least, ceil_div(longest, quantum));
+  uint64_t cost = (units(best * quantum) + slots - 1) / slots * (uint64_t(best) * quantum + overhead);
+  for (uint32_t w = 1; w <= 4; ++w) {
+    uint32_t lo = least, hi = best;  // the smallest chunk that makes at most w waves
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (units(mid * quantum) <= w * slots) hi = mid;
+      else lo = mid + 1;
+    }
+    const uint64_t c = (units(lo * quantum) + slots - 1) / slots * (uint64_t(lo) * quantum + overhead);
+    if (c < cost) {
+      cost = c;
+      best = lo;
+    }
   }
-  return lo * quantum;
+  return best * quantum;
 }
 
 constexpr size_t kScoreBytes = size_t(1) << 30;  // stored scores of one launch, at most
 constexpr uint64_t kDecodeSlots = 148 * 3;       // CTAs of the decoding kernel that run at once
 constexpr uint32_t kDecodeQuantum = 64;          // 4 warps of 16 tokens
+constexpr uint64_t kTileSlots = 148 * 2;         // CTAs of the tile kernel that run at once
+constexpr uint32_t kSplitOverhead = 128;         // of a unit, in tokens
+
+// Query tiles of a plan's rows, for the tile kernels.
+int query_tiles(vg_kv_cache *kv, AttendArgs &a, Plan &plan, cudaStream_t s) {
+  uint64_t blocks = 0;
+  for (uint32_t i = 0; i < plan.n; ++i) {
+    plan.s[i].block0 = static_cast<uint32_t>(blocks);
+    blocks += ceil_div(plan.s[i].count * a.group, kTileRows);
+  }
+  const size_t n = blocks * kv->view.heads, bytes = query_tile_bytes(kv->view.dim);
+  VG_CU(kv->ws_tiles.reserve(n * (bytes + kTileRows * sizeof(float))));
+  a.q_tiles = kv->ws_tiles.as<uint8_t>();
+  a.q_factor = reinterpret_cast<float *>(a.q_tiles + n * bytes);
+  VG_CU(launch_kv_query_tiles(a, plan, static_cast<uint32_t>(blocks), s));
+  return VG_OK;
+}
+
+int weigh_tiles(AttendArgs &a, Plan &plan, cudaStream_t s) {
+  VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, kWeighRows); }));
+  VG_CU(launch_kv_weigh_tiles(a, plan, s));
+  return VG_OK;
+}
+
+int reserve_parts(vg_kv_cache *kv, AttendArgs &a, const Plan &plan, uint32_t part_rows) {
+  const size_t rows = static_cast<size_t>(plan.units) * kv->view.heads * part_rows;
+  VG_CU(kv->ws_part.reserve(rows * (kv->view.dim * sizeof(float) + sizeof(float2))));
+  a.part_o = kv->ws_part.as<float>();
+  a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * kv->view.dim);
+  return VG_OK;
+}
 
 // Sequences of at most kDecodeRows rows per key/value head.
 int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
-  a.chunk = pick_chunk(plan, kv->view.heads, kDecodeSlots, kDecodeQuantum);
+  a.chunk = pick_chunk(plan, kDecodeSlots, kDecodeQuantum, kSplitOverhead,
+                       [&](const PlanSeq &) { return uint64_t(kv->view.heads); });
   uint32_t max_rows = 0;
   bool split = false;
   size_t scores = 0;
@@ -156,12 +206,7 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
     scores += static_cast<size_t>(kv->view.heads) * e.count * a.group * (static_cast<size_t>(ceil_div(e.len, 16)) * 16);
   }
   VG_TRY(set_units(plan, [&](const PlanSeq &e) { return std::max(1u, ceil_div(e.len, a.chunk)); }));
-  if (split) {
-    const size_t rows = static_cast<size_t>(plan.units) * kv->view.heads * kDecodeRows;
-    VG_CU(kv->ws_part.reserve(rows * (kv->view.dim * sizeof(float) + sizeof(float2))));
-    a.part_o = kv->ws_part.as<float>();
-    a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * kv->view.dim);
-  }
+  if (split) VG_TRY(reserve_parts(kv, a, plan, kDecodeRows));
   const bool keep = a.lse2 && scores * sizeof(float) <= kScoreBytes;
   if (keep) {
     VG_CU(kv->ws_scores.reserve(std::max<size_t>(scores, 1) * sizeof(float)));
@@ -173,19 +218,26 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
     VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, kWeighTile); }));
     VG_CU(launch_kv_weigh_scores(a, plan, s));
   } else if (a.lse2) {
-    VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, 4); }));
-    VG_CU(launch_kv_weigh_rows(a, plan, s));
+    VG_TRY(query_tiles(kv, a, plan, s));
+    VG_TRY(weigh_tiles(a, plan, s));
   }
   return VG_OK;
 }
 
-int attend_rows(vg_kv_cache *, const AttendArgs &a, Plan &plan, cudaStream_t s) {
-  VG_TRY(set_units(plan, [](const PlanSeq &e) { return e.count; }));
-  VG_CU(launch_kv_attend_rows(a, plan, s));
-  if (a.lse2) {
-    VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, 4); }));
-    VG_CU(launch_kv_weigh_rows(a, plan, s));
-  }
+// Sequences of more rows.
+int attend_tiles(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
+  const auto blocks = [&](const PlanSeq &e) { return ceil_div(e.count * a.group, kTileRows); };
+  VG_TRY(query_tiles(kv, a, plan, s));
+  a.chunk = pick_chunk(plan, kTileSlots, kTileRows, kSplitOverhead,
+                       [&](const PlanSeq &e) { return uint64_t(kv->view.heads) * blocks(e); });
+  VG_TRY(set_units(plan, [&](const PlanSeq &e) { return uint64_t(blocks(e)) * std::max(1u, ceil_div(e.len, a.chunk)); }));
+  uint32_t max_rows = 0;  // of the sequences that are cut
+  for (uint32_t i = 0; i < plan.n; ++i)
+    if (plan.s[i].len > a.chunk) max_rows = std::max(max_rows, plan.s[i].count * a.group);
+  if (max_rows) VG_TRY(reserve_parts(kv, a, plan, kTileRows));
+  VG_CU(launch_kv_attend_tiles(a, plan, s));
+  if (max_rows) VG_CU(launch_kv_attend_join(a, plan, kTileRows, max_rows, s));
+  if (a.lse2) VG_TRY(weigh_tiles(a, plan, s));
   return VG_OK;
 }
 
@@ -228,6 +280,9 @@ int vg_kv_create(const vg_kv_params *params, int device, vg_kv_cache **out) {
     VG_CU(cudaMemsetAsync(kv->weights.p, 0, rows * stride * sizeof(float), nullptr));
     VG_CU(cudaStreamSynchronize(nullptr));
     VG_CU(cudaEventCreateWithFlags(&kv->done, cudaEventDisableTiming));
+    VG_CU(cudaHostAlloc(reinterpret_cast<void **>(&kv->h_err), sizeof(int), cudaHostAllocMapped));
+    *kv->h_err = 0;
+    VG_CU(cudaHostGetDevicePointer(reinterpret_cast<void **>(&kv->d_err), kv->h_err, 0));
     kv->view.weights = kv->weights.as<float>();
     kv->view.heads = static_cast<uint32_t>(p.num_kv_heads);
     kv->view.dim = static_cast<uint32_t>(p.head_dim);
@@ -257,7 +312,7 @@ int vg_kv_get_info(const vg_kv_cache *kv, vg_kv_info *out) {
     out->block_tokens = kv->params.block_tokens;
     out->weight_stride = kv->view.stride;
     out->device_bytes = kv->codes[0].cap + kv->codes[1].cap + kv->scales[0].cap + kv->scales[1].cap + kv->weights.cap +
-                        kv->ws_lse.cap + kv->ws_kept.cap + kv->ws_part.cap + kv->ws_scores.cap;
+                        kv->ws_lse.cap + kv->ws_kept.cap + kv->ws_part.cap + kv->ws_scores.cap + kv->ws_tiles.cap;
     out->device = kv->device;
     return VG_OK;
   });
@@ -339,6 +394,8 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     if (q->num_heads % kv->params.num_kv_heads)
       return fail(VG_ERR_DIMENSION_MISMATCH, "the query heads must be a multiple of the cache's key/value heads");
     if (out->num_heads != q->num_heads) return fail(VG_ERR_DIMENSION_MISMATCH, "out must have the heads of q");
+    if (rows * (q->num_heads / kv->params.num_kv_heads) > 0x7fffffffull)
+      return fail(VG_ERR_INVALID_PARAMETER, "too many queries in one call");
     if (lse) VG_TRY(check_device_memory(lse, kv->device, "lse"));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Work work(kv, stream);
@@ -353,6 +410,7 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     a.scale = scale;
     a.causal = (flags & VG_KV_CAUSAL) != 0;
     a.lse = lse;
+    a.error = kv->d_err;
     if (flags & VG_KV_ACCUMULATE) {
       VG_CU(kv->ws_lse.reserve(rows * a.q_heads * sizeof(float)));
       a.lse2 = kv->ws_lse.as<float>();
@@ -361,7 +419,7 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     const auto no_units = [](size_t, PlanSeq &) { return 0u; };
     VG_TRY(for_plans_of(kv, counts, few, no_units, [&](Plan &plan) { return attend_decode(kv, a, plan, s); }));
     VG_TRY(for_plans_of(kv, counts, [&](uint32_t c) { return !few(c); }, no_units,
-                        [&](Plan &plan) { return attend_rows(kv, a, plan, s); }));
+                        [&](Plan &plan) { return attend_tiles(kv, a, plan, s); }));
     return VG_OK;
   });
 }

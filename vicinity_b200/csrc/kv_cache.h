@@ -36,8 +36,8 @@ struct PlanSeq {
   uint32_t count;  // tokens of this call
   uint32_t row0;   // first of them in the packed tensors
   uint32_t unit0;
-  uint32_t pad;
-  uint64_t aux;    // offset of its scores
+  uint32_t block0;  // the first of the launch's blocks of kTileRows rows that belongs to it
+  uint64_t aux;     // offset of its scores
 };
 struct Plan {
   uint32_t n, units;
@@ -107,17 +107,30 @@ struct AttendArgs {
   // Scores x of the call's rows, for the weights (nullable): entry e has
   // [heads][rows][len rounded up to 16] from scores + plan.s[e].aux
   float *scores;
+  // Query tiles of the tile kernels, [row block][head], and the factors of
+  // their rows, [row block][head][kTileRows]
+  uint8_t *q_tiles;
+  float *q_factor;
+  int *error;       // set nonzero when a bounded wait gives up (host-mapped)
 };
 // Sequences of at most kDecodeRows rows per key/value head.  Units: chunks (at least one per sequence).
 cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, cudaStream_t s);
 // Joins the partial sums of sequences that have more than one unit.
-cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, int part_rows, uint32_t max_rows,
+cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, uint32_t part_rows, uint32_t max_rows,
                                   cudaStream_t s);
 // Adds the probabilities of stored scores to the weights.  Units: kWeighTile tokens.
 constexpr uint32_t kWeighTile = 256;
 cudaError_t launch_kv_weigh_scores(const AttendArgs &a, const Plan &plan, cudaStream_t s);
 
-cudaError_t launch_kv_attend_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s);
-cudaError_t launch_kv_weigh_rows(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+// ---- kv_attend_tc.cu ----
+constexpr int kTileRows = 128;
+size_t query_tile_bytes(uint32_t dim);
+// blocks: row blocks of the plan (per head)
+cudaError_t launch_kv_query_tiles(const AttendArgs &a, const Plan &plan, uint32_t blocks, cudaStream_t s);
+// Any number of rows.  Units: row blocks times chunks (at least one) of each sequence.
+cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+// Weights from recomputed scores.  Units: kWeighRows tokens.
+constexpr uint32_t kWeighRows = 128;
+cudaError_t launch_kv_weigh_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s);
 
 }  // namespace vg
