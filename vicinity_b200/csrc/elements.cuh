@@ -56,6 +56,23 @@ __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
   }
 }
 
+// 16 elements as they lie in memory.
+template <class T>
+struct Raw16 {
+  uint4 w[sizeof(T)];
+  __device__ __forceinline__ void load(const T *p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else {
+      T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return to_f32(reinterpret_cast<const T *>(w)[i]); }
+};
+
 // Whether every row of a strided tensor starts on a 16-byte boundary.
 inline bool rows_aligned(const Strided &t, size_t elem) {
   return reinterpret_cast<uintptr_t>(t.p) % 16 == 0 && (t.token * static_cast<int64_t>(elem)) % 16 == 0 &&

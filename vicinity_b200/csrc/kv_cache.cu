@@ -71,6 +71,12 @@ int total_rows(const vg_kv_cache *kv, const uint32_t *counts, size_t *out) {
   return VG_OK;
 }
 
+// A launch over (unit, head, K or V) has a one-dimensional grid.
+int check_grid(const vg_kv_cache *kv, uint64_t units) {
+  if (units * 2 * kv->view.heads > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "too many tokens in one call");
+  return VG_OK;
+}
+
 // Calls launch(plan) for the sequences with a count, kPlanSeqs at a time.
 // entry(seq, PlanSeq&) fills in len and count and returns the entry's units.
 // Sequences that `take` refuses are passed over.
@@ -106,6 +112,7 @@ int for_plans_of(const vg_kv_cache *kv, const uint32_t *counts, Take &&take, Ent
 template <class Entry, class Launch>
 int for_plans(const vg_kv_cache *kv, const uint32_t *counts, Entry &&entry, Launch &&launch) {
   return for_plans_of(kv, counts, [](uint32_t) { return true; }, entry, [&](Plan &plan) -> int {
+    VG_TRY(check_grid(kv, plan.units));
     VG_CU(launch(plan));
     return VG_OK;
   });
@@ -462,7 +469,7 @@ int vg_kv_evict(vg_kv_cache *kv, size_t n, const uint32_t *src, const uint32_t *
         e.unit0 = static_cast<uint32_t>(units);
         units += ceil_div(std::min(e.len, e.count), kv->view.block);
       }
-      if (units > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "too many tokens in one call");
+      VG_TRY(check_grid(kv, units));
       plan.units = static_cast<uint32_t>(units);
       VG_CU(launch_kv_select(kv->view, plan, static_cast<uint32_t>(budget), static_cast<uint32_t>(recent),
                              kept + i0 * row, s));

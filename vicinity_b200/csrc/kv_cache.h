@@ -76,7 +76,7 @@ cudaError_t launch_rotary(const RotaryTable &t, int dtype, uint32_t dim, const i
 cudaError_t launch_kv_append(const KvView &kv, const Plan &plan, int dtype, const Strided &k, const Strided &v,
                              cudaStream_t s);
 // Units: tiles of kReadTile tokens of [len, len + count) -- len is the first token read.
-constexpr uint32_t kReadTile = 32;
+constexpr uint32_t kReadTile = 64;
 cudaError_t launch_kv_read(const KvView &kv, const Plan &plan, int dtype, const Strided &k, const Strided &v,
                            cudaStream_t s);
 // Selection: entry i keeps min(len, count = budget) tokens of sequence seq;
