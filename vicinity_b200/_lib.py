@@ -116,15 +116,6 @@ class VgProfile(C.Structure):
     ]
 
 
-class VgHeads(C.Structure):
-    _fields_ = [
-        ("data", C.c_void_p),
-        ("num_heads", C.c_uint64),
-        ("token_stride", C.c_int64),
-        ("head_stride", C.c_int64),
-    ]
-
-
 class VgRotaryParams(C.Structure):
     _fields_ = [
         ("dim", C.c_uint64),
@@ -163,7 +154,7 @@ class VgKvInfo(C.Structure):
 _vp = C.c_void_p
 _sz = C.c_size_t
 _i = C.c_int
-_hp = C.POINTER(VgHeads)
+_hp = C.c_void_p  # vg_heads: four 64-bit numbers
 
 # name -> (restype, argtypes); every declaration of include/vicinity_gpu.h.
 SIGNATURES = {

@@ -390,11 +390,12 @@ __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_c
   *w += sum;
 }
 
-template <class T, int D>
+template <class T, int D, bool kScores>
 cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  auto *kern = a.scores ? attend_decode_kernel<T, D, true> : attend_decode_kernel<T, D, false>;
+  static std::atomic<uint64_t> allowed{0};
+  auto *kern = attend_decode_kernel<T, D, kScores>;
   const int smem = kDecWarps * kStages * (2 * kStep * D + 16);
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   kern<<<dim3(plan.units, a.kv.heads), kDecWarps * 32, smem, s>>>(a, plan, rows_aligned(a.q, sizeof(T)),
                                                                   rows_aligned(a.out, sizeof(T)));
@@ -404,10 +405,10 @@ cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
 template <class T>
 cudaError_t decode_dim(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   switch (a.kv.dim) {
-    case 32: return decode<T, 32>(a, plan, s);
-    case 64: return decode<T, 64>(a, plan, s);
-    case 96: return decode<T, 96>(a, plan, s);
-    default: return decode<T, 128>(a, plan, s);
+    case 32: return a.scores ? decode<T, 32, true>(a, plan, s) : decode<T, 32, false>(a, plan, s);
+    case 64: return a.scores ? decode<T, 64, true>(a, plan, s) : decode<T, 64, false>(a, plan, s);
+    case 96: return a.scores ? decode<T, 96, true>(a, plan, s) : decode<T, 96, false>(a, plan, s);
+    default: return a.scores ? decode<T, 128, true>(a, plan, s) : decode<T, 128, false>(a, plan, s);
   }
 }
 

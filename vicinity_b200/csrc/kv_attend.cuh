@@ -5,6 +5,8 @@
 
 #include <stdint.h>
 
+#include <atomic>
+
 #include "elements.cuh"
 #include "kv_cache.h"
 #include "pipeline.cuh"
@@ -83,6 +85,17 @@ __device__ __forceinline__ float inverse_scale(float s) {
 __device__ __forceinline__ uint32_t tokens_seen(const PlanSeq &ps, uint32_t qi, bool causal) {
   const uint32_t behind = ps.count - 1 - qi;
   return !causal ? ps.len : ps.len > behind ? ps.len - behind : 0;
+}
+
+// Allows a kernel its shared memory, once per device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel *kern, size_t bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return e;
 }
 
 // The result of one row from its sums: 8 dimensions from c on, and the lse.

@@ -690,8 +690,8 @@ template <class T, int D>
 cudaError_t tile(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   auto *kern = attend_tile_kernel<T, D>;
   const size_t smem = std::max(tile_smem<D>(), kTwoPerSm);
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   kern<<<dim3(plan.units, a.kv.heads), kThreads, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
   return cudaGetLastError();
@@ -706,8 +706,8 @@ template <int D>
 cudaError_t weigh(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   auto *kern = weigh_tile_kernel<D>;
   const size_t smem = std::max(weigh_smem<D>(), kTwoPerSm);
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   kern<<<dim3(plan.units, a.kv.heads), kThreads, smem, s>>>(a, plan);
   return cudaGetLastError();

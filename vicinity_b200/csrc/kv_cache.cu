@@ -441,7 +441,9 @@ int vg_kv_evict(vg_kv_cache *kv, size_t n, const uint32_t *src, const uint32_t *
     std::vector<char> seen(kv->len.size(), 0);
     for (size_t i = 0; i < n; ++i)
       for (uint32_t s : {src[i], dst[i]}) {
-        if (s >= kv->len.size()) return fail(VG_ERR_INVALID_PARAMETER, "no sequence " + std::to_string(s));
+        if (s >= kv->len.size())
+          return fail(VG_ERR_INVALID_PARAMETER, "no sequence " + std::to_string(s) + ": the cache's are below " +
+                                                    std::to_string(kv->len.size()));
         if (seen[s]) return fail(VG_ERR_INVALID_PARAMETER, "sequence " + std::to_string(s) + " appears twice");
         seen[s] = 1;
       }

@@ -12,39 +12,45 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 
 import numpy as np
 
 from . import _lib
 
-_DTYPES = {"float32": _lib.F32, "float16": _lib.F16, "bfloat16": _lib.BF16}
+_NAMES = {"float32": _lib.F32, "float16": _lib.F16, "bfloat16": _lib.BF16}
+_CODES: dict = {}  # by the libraries' own dtype objects
 _SCALINGS = {"none": _lib.ROTARY_PLAIN, "linear": _lib.ROTARY_LINEAR, "by_parts": _lib.ROTARY_BY_PARTS}
 
 
 def _dtype(x) -> int:
-    name = str(x.dtype).rpartition(".")[2]
-    try:
-        return _DTYPES[name]
-    except KeyError:
-        raise ValueError(f"tensors are float32, float16 or bfloat16, got {name}") from None
+    code = _CODES.get(x.dtype)
+    if code is None:
+        name = str(x.dtype).rpartition(".")[2]
+        if name not in _NAMES:
+            raise ValueError(f"tensors are float32, float16 or bfloat16, got {name}")
+        code = _CODES[x.dtype] = _NAMES[name]
+    return code
 
 
-def _heads(x, name: str, tokens: int, dim: int, dtype: int) -> _lib.VgHeads:
-    """[tokens, heads, dim] with the last dimension contiguous."""
-    shape = tuple(x.shape)
+def _heads(x, name: str, tokens: int, dim: int, dtype: int) -> tuple:
+    """The vg_heads of a [tokens, heads, dim] array with its last dimension contiguous."""
+    shape, stride = x.shape, x.stride()
     if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
         raise ValueError(f"{name} must be [{tokens}, heads, {dim}], got {list(shape)}")
-    if _dtype(x) != dtype:
+    if _CODES.get(x.dtype, -1) != dtype and _dtype(x) != dtype:
         raise ValueError(f"{name} must have the element type of the other tensors")
-    st = x.stride()
-    if tokens and st[2] != 1:
+    if stride[2] != 1 and tokens:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    return _lib.VgHeads(x.data_ptr() or None, shape[1], st[0], st[1])
+    return x.data_ptr(), shape[1], stride[0], stride[1]
+
+
+_HEADS = 32  # bytes of a vg_heads
 
 
 def _flat(x, name: str, shape: tuple, dtype: str) -> int:
     """Address of a contiguous device array of the given shape and type."""
-    if tuple(x.shape) != shape or str(x.dtype).rpartition(".")[2] != dtype or not x.is_contiguous():
+    if x.shape != shape or not str(x.dtype).endswith(dtype) or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} array of shape {list(shape)}")
     return x.data_ptr()
 
@@ -107,15 +113,17 @@ class Rotary:
         n, d, dt = q.shape[0], q.shape[-1], _dtype(q)
         pos = _flat(positions, "positions", (n,), "int64")
         hq = _heads(q, "q", n, d, dt)
-        hqo = hq if out_q is None else _heads(out_q, "out_q", n, d, dt)
-        hk = hko = None
+        packed = hq + (hq if out_q is None else _heads(out_q, "out_q", n, d, dt))
         if k is not None:
             hk = _heads(k, "k", n, d, dt)
-            hko = hk if out_k is None else _heads(out_k, "out_k", n, d, dt)
+            packed += hk + (hk if out_k is None else _heads(out_k, "out_k", n, d, dt))
         elif out_k is not None:
             raise ValueError("out_k without k")
-        _lib.check(self._lib.vg_rotary_apply(self._h, dt, d, pos, n, hq, hqo, hk, hko, int(bool(transpose)),
-                                             q.device.index or 0, stream))
+        h = array("q", packed)
+        at = h.buffer_info()[0]
+        _lib.check(self._lib.vg_rotary_apply(
+            self._h, dt, d, pos, n, at, at + _HEADS, None if k is None else at + 2 * _HEADS,
+            None if k is None else at + 3 * _HEADS, 1 if transpose else 0, q.device.index or 0, stream))
 
 
 class _Weights:
@@ -191,27 +199,28 @@ class KVCache:
                         int(self.info().weight_stride))
 
     def _counts(self, counts, name: str = "counts"):
-        """A C array of one unsigned number per sequence, and their sum."""
-        if len(counts) != self.num_seqs:
+        """One unsigned number per sequence: an array, its address and the sum."""
+        try:
+            c = array("I", counts)
+        except (OverflowError, TypeError):
+            raise ValueError(f"{name} must not be negative, fractions or above 2^32 - 1") from None
+        if len(c) != self.num_seqs:
             raise ValueError(f"{name} must have one entry for each of the {self.num_seqs} sequences")
-        total = 0
-        for c in counts:
-            if not 0 <= c <= 0xFFFFFFFF:
-                raise ValueError(f"{name} must not be negative or above 2^32 - 1")
-            total += int(c)
-        return (C.c_uint32 * self.num_seqs)(*[int(c) for c in counts]), total
+        return c, c.buffer_info()[0], sum(c)
 
     def truncate(self, lengths) -> None:
         """Keep the first ``lengths[s]`` tokens of every sequence; 0 empties it."""
-        _lib.check(self._lib.vg_kv_truncate(self._h, self._counts(lengths, "lengths")[0]))
+        c, ptr, _ = self._counts(lengths, "lengths")
+        _lib.check(self._lib.vg_kv_truncate(self._h, ptr))
 
     def append(self, k, v, counts, stream=None) -> None:
         """Append ``counts[s]`` tokens to every sequence; ``k`` and ``v``
         [sum(counts), num_kv_heads, head_dim] hold them in sequence order."""
-        c, n = self._counts(counts)
+        c, ptr, n = self._counts(counts)
         dt = _dtype(k)
-        _lib.check(self._lib.vg_kv_append(self._h, c, dt, _heads(k, "k", n, self.head_dim, dt),
-                                          _heads(v, "v", n, self.head_dim, dt), stream))
+        h = array("q", _heads(k, "k", n, self.head_dim, dt) + _heads(v, "v", n, self.head_dim, dt))
+        at = h.buffer_info()[0]
+        _lib.check(self._lib.vg_kv_append(self._h, ptr, dt, at, at + _HEADS, stream))
 
     def attend(self, q, counts, out, lse=None, scale: float | None = None, causal: bool = True,
                accumulate: bool = False, stream=None) -> None:
@@ -220,12 +229,13 @@ class KVCache:
         of the denominators into ``lse``, f32 [sum(counts), heads]).  ``scale``
         defaults to head_dim ** -0.5.  ``accumulate`` adds the probabilities to
         ``weights``."""
-        c, n = self._counts(counts)
+        c, ptr, n = self._counts(counts)
         dt = _dtype(q)
         hq = _heads(q, "q", n, self.head_dim, dt)
+        h = array("q", hq + _heads(out, "out", n, self.head_dim, dt))
+        at = h.buffer_info()[0]
         _lib.check(self._lib.vg_kv_attend(
-            self._h, c, dt, hq, _heads(out, "out", n, self.head_dim, dt),
-            None if lse is None else _flat(lse, "lse", (n, hq.num_heads), "float32") or None,
+            self._h, ptr, dt, at, at + _HEADS, None if lse is None else _flat(lse, "lse", (n, hq[1]), "float32"),
             1.0 / math.sqrt(self.head_dim) if scale is None else scale,
             (_lib.KV_CAUSAL if causal else 0) | (_lib.KV_ACCUMULATE if accumulate else 0), stream))
 
@@ -233,26 +243,29 @@ class KVCache:
         """Cut sequences ``src`` down to ``budget`` tokens each into the
         sequences ``dst``: the ``recent`` newest and those of largest
         accumulated weight.  ``kept``: int32 [len(src), num_kv_heads, budget]."""
-        n = len(src)
-        if len(dst) != n:
+        try:
+            ids = array("I", src), array("I", dst)
+        except (OverflowError, TypeError):
+            raise ValueError(f"src and dst must be sequences below {self.num_seqs}") from None
+        n = len(ids[0])
+        if len(ids[1]) != n:
             raise ValueError("src and dst must have the same length")
         if budget < 1 or recent < 0:
             raise ValueError("budget must be greater than 0 and recent not negative")
-        if any(not 0 <= s < self.num_seqs for s in src) or any(not 0 <= s < self.num_seqs for s in dst):
-            raise ValueError(f"src and dst must be sequences below {self.num_seqs}")
-        ids = C.c_uint32 * n
         ptr = None if kept is None else _flat(kept, "kept", (n, self.num_kv_heads, budget), "int32") or None
-        _lib.check(self._lib.vg_kv_evict(self._h, n, ids(*src), ids(*dst), budget, recent, ptr, stream))
+        _lib.check(self._lib.vg_kv_evict(self._h, n, ids[0].buffer_info()[0], ids[1].buffer_info()[0], budget, recent,
+                                         ptr, stream))
 
     def read(self, starts, counts, k, v, stream=None) -> None:
         """The values of tokens [starts[s], starts[s] + counts[s]) of every
         sequence into ``k`` and ``v`` [sum(counts), num_kv_heads, head_dim]
         (exact in bf16 and f32)."""
-        first, _ = self._counts(starts, "starts")
-        c, n = self._counts(counts)
+        first, first_ptr, _ = self._counts(starts, "starts")
+        c, ptr, n = self._counts(counts)
         dt = _dtype(k)
-        _lib.check(self._lib.vg_kv_read(self._h, first, c, dt, _heads(k, "k", n, self.head_dim, dt),
-                                        _heads(v, "v", n, self.head_dim, dt), stream))
+        h = array("q", _heads(k, "k", n, self.head_dim, dt) + _heads(v, "v", n, self.head_dim, dt))
+        at = h.buffer_info()[0]
+        _lib.check(self._lib.vg_kv_read(self._h, first_ptr, ptr, dt, at, at + _HEADS, stream))
 
     def _shapes(self, n: int):
         h, d, nb = self.num_kv_heads, self.head_dim, -(-n // self.block_tokens)
