@@ -21,9 +21,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // vanish below 2^-38 of the largest.
 constexpr float kPShift = 13.0f, kLazy = 2.0f;
 
-__device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; 2^-inf = 0
+// 2 ulp; 0 below 2^-126 (the form that keeps subnormal results is four instructions)
+__device__ __forceinline__ float exp2_approx(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 

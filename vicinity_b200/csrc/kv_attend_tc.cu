@@ -343,6 +343,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
       const uint32_t at = t + (lane & 7) * 16;
       return lane < 16 && at < ps.len ? __ldg(scales + (at >> kv.block_shift)) : 1.0f;
     };
+    // the factor of a group's products; above 0 (also for keys that read as
+    // NaN, see below), so that -inf stays -inf
+    auto factor = [&](float ks) {
+      const float f = f_row * ks;
+      return f > 0.0f ? f : 1e-37f;
+    };
+    // products of 32 tokens from `from` on that the row does not see
+    auto hide = [&](uint32_t (&v)[32], uint32_t from) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        if (from + k >= lim) v[k] = 0xff800000u;
+    };
     float next = tiles ? scale_at(t0) : 1.0f;
     float mu = -VG_INF, l = 0.0f;
     bool ok = true;
@@ -361,19 +373,15 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
         uint32_t v[32];
         tmem_ld32_nowait(pS + c * 32, v);
         tmem_wait_ld();
-        if (t + (c + 1) * 32 > warp_lim) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (t + c * 32 + k >= lim) v[k] = 0xff800000u;
-        }
+        if (t + (c + 1) * 32 > warp_lim) hide(v, t + c * 32);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float f = f_row * __shfl_sync(VG_FULL_MASK, sc, 2 * c + g);
+          const float f = factor(__shfl_sync(VG_FULL_MASK, sc, 2 * c + g));
           const float lv = log2_scale(__shfl_sync(VG_FULL_MASK, sc, 8 + 2 * c + g));
           float x = -VG_INF;
 #pragma unroll
           for (int k = 0; k < 16; ++k) x = fmaxf(x, __uint_as_float(v[16 * g + k]));
-          m = fmaxf(m, x * f + lv);  // NaN (-inf times 0: nothing seen) is passed over
+          m = fmaxf(m, x * f + lv);
         }
       }
       if (__any_sync(VG_FULL_MASK, m > mu + kLazy)) {
@@ -400,10 +408,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
         uint32_t v[32], p[16];
         tmem_ld32_nowait(pS + c * 32, v);
         tmem_wait_ld();
-        const bool edge = t + (c + 1) * 32 > warp_lim;
+        if (t + (c + 1) * 32 > warp_lim) hide(v, t + c * 32);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float f = f_row * __shfl_sync(VG_FULL_MASK, sc, 2 * c + g);
+          const float kscale = __shfl_sync(VG_FULL_MASK, sc, 2 * c + g), f = factor(kscale);
           const float vscale = __shfl_sync(VG_FULL_MASK, sc, 8 + 2 * c + g);
           const float ref = base + log2_scale(vscale);
           const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
@@ -415,16 +423,13 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
                 f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2, ref2));
             x.x = exp2_approx(x.x);
             x.y = exp2_approx(x.y);
-            if (edge) {
-              if (t + c * 32 + e >= lim) x.x = 0.0f;
-              if (t + c * 32 + e + 1 >= lim) x.y = 0.0f;
-            }
             sum2 = f2_add(sum2, f2_pack(x.x, x.y));
             p[8 * g + k] = pack_half2(x.x, x.y);
           }
           const float2 sum = f2_unpack(sum2);
           l += (sum.x + sum.y) * inverse_scale(vscale);
-          if (vscale != vscale) {  // the values read as NaN: so does every row that sees one of them
+          if (kscale != kscale || vscale != vscale) {  // they read as NaN: so does every row that sees one of them
+            if (kscale != kscale && t + c * 32 + 16 * g < lim) l = kscale;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint32_t col = t + c * 32 + 16 * g + 2 * k;
