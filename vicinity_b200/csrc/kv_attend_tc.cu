@@ -8,13 +8,15 @@
 // every row block.  See kv_attend.cu for the scaling of scores and
 // probabilities.
 //
-// attend_tile_kernel, one CTA per (sequence, head, 128 rows, chunk of tokens),
-// two CTAs on an SM so that one's products fill the other's softmax:
-//   warps 0..3  softmax: one row per thread, S from TMEM, P back into its place
-//   warps 4..7  load codes, convert them to binary16 tiles in shared memory
-//               (keys as they are; values transposed: tokens are the
-//               contraction of the second product)
-//   warp 8      copies the query tile, issues S = Q K^T and O += P V
+// attend_tile_kernel, one CTA per (sequence, head, kTiles row tiles, chunk of
+// tokens).  Two row tiles share the converted codes and take turns: the
+// products of one run while the other is in its softmax.  A sequence of one row
+// tile gets a CTA of half the size, two of which share an SM instead.
+//   4 warps per row tile  softmax: one row per thread, S from TMEM, P back into its place
+//   4 warps               load codes, convert them to binary16 tiles in shared memory
+//                         (keys as they are; values transposed: tokens are the
+//                         contraction of the second product)
+//   1 warp                copies the query tiles, issues S = Q K^T and O += P V
 // Every wait is bounded: a protocol error sets the error flag and the kernel
 // drains its copies and products, frees its TMEM and returns.
 #include "common.cuh"
@@ -33,8 +35,8 @@ namespace {
 constexpr int kRows = kTileRows;              // 128
 constexpr uint32_t kTok = 128;                // tokens per tile
 constexpr uint32_t kKBlockBytes = kRows * 128;  // 64 binary16 columns of a 128-row tile
-constexpr int kThreads = 288;
-constexpr uint32_t kTmemColumns = 256;        // S (P in its first half) and O, or two S
+constexpr int kThreads = 288;                 // of the weights' kernel
+constexpr uint32_t kTmemColumns = 256;        // its two accumulators
 
 __device__ __forceinline__ uint32_t f16_idesc(uint32_t n) {  // D f32, A and B binary16 K-major, M = 128
   return (1u << 4) | ((n >> 3) << 17) | ((kRows >> 4) << 24);
@@ -63,6 +65,13 @@ __device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t *v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t *v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::
+                   "memory");
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
@@ -201,187 +210,220 @@ __global__ void __launch_bounds__(kImageThreads) query_tiles_kernel(const __grid
 
 // ---- attention ---------------------------------------------------------------------
 
-template <int D>
-constexpr size_t tile_smem() {
-  return 1024 + 2 * ((D + 63) / 64) * kKBlockBytes + 2 * D * 128 + 128;
-}
+template <int D, int kTiles>
+struct TileSmem {  // offsets from a 1024-byte boundary; kTiles stages of codes
+  static constexpr uint32_t kQ = ((D + 63) / 64) * kKBlockBytes, kK = kQ, kV = 2 * D * 128;
+  static constexpr uint32_t k = kTiles * kQ, v = k + kTiles * kK, table = v + kTiles * kV;
+  static constexpr uint32_t bars = table + 2 * 8 * sizeof(float4);
+  static constexpr size_t bytes = 1024 + bars + 32 * 8;
+};
 
-template <class T, int D>
-__global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_constant__ AttendArgs a,
-                                                                  const __grid_constant__ Plan plan,
-                                                                  const bool ovec) {
+template <class T, int D, int kTiles>
+__global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
+    attend_tile_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan, const bool ovec) {
+  using Smem = TileSmem<D, kTiles>;
+  constexpr int kSoftWarps = 4 * kTiles, kMmaWarp = kSoftWarps + 4;
+  constexpr uint32_t kColumns = 256 * kTiles;  // per row tile: S (P in its first half) and O
   extern __shared__ uint8_t tile_raw[];
   const uint32_t raw = smem_u32(tile_raw);
   uint8_t *sm = tile_raw + (((raw + 1023u) & ~1023u) - raw);  // swizzled tiles need 1024-byte alignment
-  constexpr uint32_t kQBytes = ((D + 63) / 64) * kKBlockBytes, kVBytes = 2 * D * 128;
-  uint8_t *sQ = sm, *sK = sm + kQBytes, *sV = sK + kQBytes;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(sV + kVBytes);
-  uint64_t *qfull = bars, *kfull = bars + 1, *kempty = bars + 2, *vfull = bars + 3, *vempty = bars + 4,
-           *sfull = bars + 5, *pfull = bars + 6, *drain = bars + 7;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 8);
+  uint8_t *sQ = sm, *sK = sm + Smem::k, *sV = sm + Smem::v;
+  // per 16 tokens: (key scale, log2 of the value scale, its reciprocal, whether one of them is NaN)
+  float4 *table = reinterpret_cast<float4 *>(sm + Smem::table);  // [2][8]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sm + Smem::bars);
+  uint64_t *qfull = bars, *drain = bars + 1, *tfull = bars + 2;           // tfull[2]
+  uint64_t *kfull = bars + 4, *kempty = bars + 6, *vfull = bars + 8, *vempty = bars + 10;  // [kTiles] stages
+  uint64_t *sfull = bars + 12, *pfull = bars + 14, *pvdone = bars + 16;   // [kTiles] row tiles
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = lane_id();
 
   const KvView &kv = a.kv;
   const uint32_t unit = blockIdx.x, head = blockIdx.y;
   const PlanSeq &ps = plan.s[plan_find(plan, unit)];
+  constexpr uint32_t kUnitRows = kRows * kTiles;
   const uint32_t rows = ps.count * a.group, ns = max(1u, (ps.len + a.chunk - 1) / a.chunk);
-  const uint32_t nrb = (rows + kRows - 1) / kRows;
+  const uint32_t nrb = (rows + kUnitRows - 1) / kUnitRows;
   const uint32_t rb = nrb - 1 - (unit - ps.unit0) / ns, sp = (unit - ps.unit0) % ns;  // last rows, which see most, first
-  const uint32_t last = min(rows, (rb + 1) * kRows) - 1;
+  const uint32_t last = min(rows, (rb + 1) * kUnitRows) - 1;
+  const uint32_t row_tiles = (last - rb * kUnitRows) / kRows + 1;  // of the unit's kTiles
   const uint32_t t0 = sp * a.chunk, t1 = min(tokens_seen(ps, last / a.group, a.causal), t0 + a.chunk);
   const uint32_t tiles = t1 > t0 ? (t1 - t0 + kTok - 1) / kTok : 0;
   const size_t r = static_cast<size_t>(ps.seq) * kv.heads + head, nb = kv.stride >> kv.block_shift;
+  const size_t q_at = static_cast<size_t>(ps.block0 + rb * kTiles) * kv.heads + head;  // + heads per row tile
 
   if (threadIdx.x == 0) {
     mbar_init(qfull, 1);
-    mbar_init(kfull, 4);
-    mbar_init(kempty, 1);
-    mbar_init(vfull, 4);
-    mbar_init(vempty, 1);
-    mbar_init(sfull, 1);
-    mbar_init(pfull, 4);
     mbar_init(drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tfull + i, 1);
+      mbar_init(kfull + i, 4);
+      mbar_init(kempty + i, 1);
+      mbar_init(vfull + i, 4);
+      mbar_init(vempty + i, 1);
+      mbar_init(sfull + i, 1);
+      mbar_init(pfull + i, 4);
+      mbar_init(pvdone + i, 1);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(kTmemColumns)
+                 "r"(kColumns)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tS = tmem, tO = tmem + kTok;
+  const uint32_t tmem = *tmem_slot;  // row tile x: S at 128 x, O at 128 (kTiles + x)
   auto give_up = [&](int code) {
     *abort_flag = 1;
     if (a.error) *reinterpret_cast<volatile int *>(a.error) = code;
   };
 
-  if (warp == 8) {
-    // ---- query tile and products ----
+  if (warp == kMmaWarp) {
+    // ---- query tiles and products ----
     if (lane == 0 && tiles) {
-      const size_t at = static_cast<size_t>(ps.block0 + rb) * kv.heads + head;
-      mbar_arrive_expect_tx(qfull, kQBytes);
-      bulk_copy_g2s(sQ, a.q_tiles + at * kQBytes, kQBytes, qfull);
+      mbar_arrive_expect_tx(qfull, row_tiles * Smem::kQ);
+      for (uint32_t x = 0; x < row_tiles; ++x)
+        bulk_copy_g2s(sQ + x * Smem::kQ, a.q_tiles + (q_at + static_cast<size_t>(x) * kv.heads) * Smem::kQ, Smem::kQ,
+                      qfull);
       bool ok = mbar_wait_sleep(qfull, 0);
       const uint32_t bQ = smem_u32(sQ), bK = smem_u32(sK), bV = smem_u32(sV);
-      for (uint32_t i = 0; ok && i < tiles; ++i) {
-        // S: the keys are there, and the previous tile's P (in S's place) has been used
-        if (*abort_flag || !mbar_wait_sleep(kfull, i & 1) || (i && !mbar_wait_sleep(vempty, (i - 1) & 1))) {
-          ok = false;
-          break;
+      auto scores = [&](uint32_t x, uint32_t i) {  // S of row tile x and token tile i
+        const uint32_t st = i % kTiles;
+        if (x == 0) {
+          ok = ok && mbar_wait_sleep(kfull + st, (i / kTiles) & 1);
+          if (!ok) return;
+          tc_fence_after();
         }
-        tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = (k >> 2) * kKBlockBytes + (k & 3) * 32;
-          umma_ss(tS, umma_desc(bQ + off), umma_desc(bK + off), f16_idesc(kTok), k != 0);
+          umma_ss(tmem + x * kTok, umma_desc(bQ + x * Smem::kQ + off), umma_desc(bK + st * Smem::kK + off),
+                  f16_idesc(kTok), k != 0);
         }
-        umma_commit(kempty);
-        umma_commit(sfull);
-        if (!mbar_wait_sleep(vfull, i & 1) || !mbar_wait_sleep(pfull, i & 1)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+        umma_commit(sfull + x);
+        if (x + 1 == row_tiles) umma_commit(kempty + st);
+      };
+      for (uint32_t x = 0; ok && x < row_tiles; ++x) scores(x, 0);
+      for (uint32_t i = 0; ok && i < tiles; ++i) {
+        const uint32_t st = i % kTiles;
+        for (uint32_t x = 0; ok && x < row_tiles; ++x) {
+          ok = !*abort_flag && (x || mbar_wait_sleep(vfull + st, (i / kTiles) & 1)) && mbar_wait_sleep(pfull + x, i & 1);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < static_cast<int>(kTok) / 16; ++k)
-          umma_ts(tO, tS + k * 8, umma_desc(bV + (k >> 2) * (D * 128) + (k & 3) * 32), f16_idesc(D), i != 0 || k != 0);
-        umma_commit(vempty);
+          for (int k = 0; k < static_cast<int>(kTok) / 16; ++k)
+            umma_ts(tmem + (kTiles + x) * kTok, tmem + x * kTok + k * 8,
+                    umma_desc(bV + st * Smem::kV + (k >> 2) * (D * 128) + (k & 3) * 32), f16_idesc(D), i != 0 || k != 0);
+          umma_commit(pvdone + x);
+          if (x + 1 == row_tiles) umma_commit(vempty + st);
+          // the next S takes the place of the P just used
+          if (i + 1 < tiles && (ok = mbar_wait(pvdone + x, i & 1))) scores(x, i + 1);
+        }
       }
       if (!ok) give_up(1);
       umma_commit(drain);  // every product issued is complete before TMEM is released
       mbar_wait(drain, 0);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= kSoftWarps) {
     // ---- codes to binary16 tiles ----
-    const uint32_t tid = threadIdx.x - 128;
+    const uint32_t tid = threadIdx.x - kSoftWarps * 32;
     const int8_t *kc = kv.codes[0] + (r * kv.stride + t0) * D, *vc = kv.codes[1] + (r * kv.stride + t0) * D;
+    const float *ks = kv.scales[0] + r * nb, *vs = kv.scales[1] + r * nb;
     KeyTile<D, 128> key;
     ValueTile<D> value;
-    if (tiles) key.load(kc, tid);
+    float2 scale = make_float2(1.0f, 1.0f);  // of group `lane` of the tile (first warp)
+    auto load_keys = [&](uint32_t i) {
+      key.load(kc + static_cast<size_t>(i) * kTok * D, tid);
+      const uint32_t t = t0 + i * kTok + tid * 16;
+      if (tid < 8 && t < ps.len) scale = make_float2(__ldg(ks + (t >> kv.block_shift)), __ldg(vs + (t >> kv.block_shift)));
+    };
+    if (tiles) load_keys(0);
     bool ok = true;
     for (uint32_t i = 0; i < tiles; ++i) {
+      const uint32_t st = i % kTiles, before = (i / kTiles - 1) & 1;  // phase of the stage's last use
       value.load(vc + static_cast<size_t>(i) * kTok * D, tid);
-      if (!__all_sync(VG_FULL_MASK, !i || mbar_wait_sleep(kempty, (i - 1) & 1))) {
+      // The stage's keys have been used and, two tiles ago, the table's entries
+      // (with one stage: waited for before the last tile's values).
+      ok = i < kTiles || (mbar_wait_sleep(kempty + st, before) && (kTiles == 1 || mbar_wait_sleep(vempty + st, before)));
+      if (!__all_sync(VG_FULL_MASK, ok)) {
         ok = false;
         break;
       }
-      key.store(sK, tid);
+      if (tid < 8)
+        table[(i & 1) * 8 + tid] =
+            make_float4(scale.x == scale.x ? scale.x : 1.0f, log2_scale(scale.y), inverse_scale(scale.y),
+                        scale.x != scale.x ? 2.0f : scale.y != scale.y ? 1.0f : 0.0f);
+      if (tid < 32) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tfull + (i & 1));
+      }
+      key.store(sK + st * Smem::kK, tid);
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(kfull);
-      if (i + 1 < tiles) key.load(kc + static_cast<size_t>(i + 1) * kTok * D, tid);
-      if (!__all_sync(VG_FULL_MASK, !i || mbar_wait_sleep(vempty, (i - 1) & 1))) {
+      if (lane == 0) mbar_arrive(kfull + st);
+      if (i + 1 < tiles) load_keys(i + 1);
+      if (!__all_sync(VG_FULL_MASK, i < kTiles || mbar_wait_sleep(vempty + st, before))) {
         ok = false;
         break;
       }
-      value.store(sV, tid);
+      value.store(sV + st * Smem::kV, tid);
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(vfull);
+      if (lane == 0) mbar_arrive(vfull + st);
     }
     if (!ok) give_up(2);
-  } else {
+  } else if (static_cast<uint32_t>(warp >> 2) < row_tiles) {
     // ---- softmax: thread = row = TMEM lane ----
-    const uint32_t row = rb * kRows + threadIdx.x;
+    const uint32_t x = warp >> 2, wr = threadIdx.x & 127;
+    const uint32_t row = rb * kUnitRows + threadIdx.x;
     const bool valid = row < rows;
     const uint32_t qi = row / a.group;
     const uint32_t lim = valid ? tokens_seen(ps, qi, a.causal) : 0xffffffffu;
     const uint32_t warp_lim = __reduce_min_sync(VG_FULL_MASK, lim);
-    const float f_row =
-        a.q_factor[(static_cast<size_t>(ps.block0 + rb) * kv.heads + head) * kRows + threadIdx.x];
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t pS = tS + lane_base, pO = tO + lane_base;
-    // lanes 0..7 and 8..15 hold the key and value scales of a tile's eight 16-token groups
-    const float *scales = kv.scales[lane >> 3 & 1] + r * nb;
-    auto scale_at = [&](uint32_t t) {
-      const uint32_t at = t + (lane & 7) * 16;
-      return lane < 16 && at < ps.len ? __ldg(scales + (at >> kv.block_shift)) : 1.0f;
-    };
-    // the factor of a group's products; above 0 (also for keys that read as
-    // NaN, see below), so that -inf stays -inf
-    auto factor = [&](float ks) {
-      const float f = f_row * ks;
-      return f > 0.0f ? f : 1e-37f;
-    };
+    const float f_row = a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t pS = tmem + x * kTok + lane_base, pO = tmem + (kTiles + x) * kTok + lane_base;
     // products of 32 tokens from `from` on that the row does not see
     auto hide = [&](uint32_t (&v)[32], uint32_t from) {
 #pragma unroll
       for (int k = 0; k < 32; ++k)
         if (from + k >= lim) v[k] = 0xff800000u;
     };
-    float next = tiles ? scale_at(t0) : 1.0f;
     float mu = -VG_INF, l = 0.0f;
     bool ok = true;
     for (uint32_t i = 0; i < tiles; ++i) {
       const uint32_t t = t0 + i * kTok;
-      const float sc = next;
-      if (i + 1 < tiles) next = scale_at(t + kTok);
-      if (!__all_sync(VG_FULL_MASK, mbar_wait_sleep(sfull, i & 1))) {
+      const float4 *tab = table + (i & 1) * 8;
+      if (!__all_sync(VG_FULL_MASK, mbar_wait_sleep(tfull + (i & 1), (i >> 1) & 1) && mbar_wait_sleep(sfull + x, i & 1))) {
         ok = false;
         break;
       }
       tc_fence_after();
+      // the factors of a group's products are above 0, so that -inf stays -inf
       float m = -VG_INF;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld32_nowait(pS + c * 32, v);
-        tmem_wait_ld();
-        if (t + (c + 1) * 32 > warp_lim) hide(v, t + c * 32);
+      {
+        uint32_t v[2][32];
+        tmem_ld32_nowait(pS, v[0]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float f = factor(__shfl_sync(VG_FULL_MASK, sc, 2 * c + g));
-          const float lv = log2_scale(__shfl_sync(VG_FULL_MASK, sc, 8 + 2 * c + g));
-          float x = -VG_INF;
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&w)[32] = v[c & 1];
+          tmem_wait_ld32(w);
+          if (c < 3) tmem_ld32_nowait(pS + (c + 1) * 32, v[(c + 1) & 1]);
+          if (t + (c + 1) * 32 > warp_lim) hide(w, t + c * 32);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x = fmaxf(x, __uint_as_float(v[16 * g + k]));
-          m = fmaxf(m, x * f + lv);
+          for (int g = 0; g < 2; ++g) {
+            const float4 e = tab[2 * c + g];
+            float top = -VG_INF;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(w[16 * g + k]));
+            m = fmaxf(m, fmaf(top, fmaxf(f_row * e.x, 1e-37f), e.y));
+          }
         }
       }
       if (__any_sync(VG_FULL_MASK, m > mu + kLazy)) {
@@ -395,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
             uint32_t v[16];
             tmem_ld8_nowait(pO + b, v);
             tmem_ld8_nowait(pO + b + 8, v + 8);
-            tmem_wait_ld();
+            tmem_wait_ld16(v);
 #pragma unroll
             for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * c);
             tmem_st16(pO + b, v);
@@ -403,69 +445,73 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
         }
       }
       const float base = kPShift - (mu == -VG_INF ? 0.0f : mu);
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32], p[16];
-        tmem_ld32_nowait(pS + c * 32, v);
-        tmem_wait_ld();
-        if (t + (c + 1) * 32 > warp_lim) hide(v, t + c * 32);
+      {
+        uint32_t v[2][32];
+        tmem_ld32_nowait(pS, v[0]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float kscale = __shfl_sync(VG_FULL_MASK, sc, 2 * c + g), f = factor(kscale);
-          const float vscale = __shfl_sync(VG_FULL_MASK, sc, 8 + 2 * c + g);
-          const float ref = base + log2_scale(vscale);
-          const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
-          f32x2 sum2 = 0;
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&w)[32] = v[c & 1];
+          tmem_wait_ld32(w);
+          if (c < 3) tmem_ld32_nowait(pS + (c + 1) * 32, v[(c + 1) & 1]);
+          if (t + (c + 1) * 32 > warp_lim) hide(w, t + c * 32);
+          uint32_t p[16];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int e = 16 * g + 2 * k;
-            float2 x = f2_unpack(
-                f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2, ref2));
-            x.x = exp2_approx(x.x);
-            x.y = exp2_approx(x.y);
-            sum2 = f2_add(sum2, f2_pack(x.x, x.y));
-            p[8 * g + k] = pack_half2(x.x, x.y);
-          }
-          const float2 sum = f2_unpack(sum2);
-          l += (sum.x + sum.y) * inverse_scale(vscale);
-          if (kscale != kscale || vscale != vscale) {  // they read as NaN: so does every row that sees one of them
-            if (kscale != kscale && t + c * 32 + 16 * g < lim) l = kscale;
+          for (int g = 0; g < 2; ++g) {
+            const float4 e = tab[2 * c + g];
+            const float f = fmaxf(f_row * e.x, 1e-37f), ref = base + e.y;
+            const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
+            f32x2 sum2 = 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const uint32_t col = t + c * 32 + 16 * g + 2 * k;
-              if (col < lim) p[8 * g + k] = (p[8 * g + k] & 0xffff0000u) | 0x7fffu;
-              if (col + 1 < lim) p[8 * g + k] |= 0x7fff0000u;
+              const int j = 16 * g + 2 * k;
+              float2 y = f2_unpack(f2_fma(f2_pack(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), f2, ref2));
+              y.x = exp2_approx(y.x);
+              y.y = exp2_approx(y.y);
+              sum2 = f2_add(sum2, f2_pack(y.x, y.y));
+              p[8 * g + k] = pack_half2(y.x, y.y);
+            }
+            const float2 sum = f2_unpack(sum2);
+            l = fmaf(sum.x + sum.y, e.z, l);
+            if (e.w != 0.0f) {  // keys or values read as NaN: so does every row that sees one of them
+              const uint32_t at = t + c * 32 + 16 * g;
+              if (e.w == 2.0f && at < lim) l = __int_as_float(0x7fffffff);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                if (at + 2 * k < lim) p[8 * g + k] = (p[8 * g + k] & 0xffff0000u) | 0x7fffu;
+                if (at + 2 * k + 1 < lim) p[8 * g + k] |= 0x7fff0000u;
+              }
             }
           }
+          // P of these 32 tokens lies over S of tokens that have been read (also by the load in flight)
+          tmem_st16(pS + c * 16, p);
         }
-        tmem_st16(pS + c * 16, p);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pfull);
+      if (lane == 0) mbar_arrive(pfull + x);
     }
     if (ok && tiles) {
-      ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(vempty, (tiles - 1) & 1));
+      ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(pvdone + x, (tiles - 1) & 1));
       tc_fence_after();
     }
     if (ok) {
       const bool whole = ps.len <= a.chunk;
-      const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kRows + threadIdx.x;
+      const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kUnitRows + threadIdx.x;
 #pragma unroll 1
       for (int b = 0; b < D / 4; b += 8) {  // dimensions 4 b .. 4 b + 31
-        uint32_t v[4][8] = {};
+        uint32_t v[32] = {};
         if (tiles) {
 #pragma unroll
-          for (int d = 0; d < 4; ++d) tmem_ld8_nowait(pO + d * (D / 4) + b, v[d]);
-          tmem_wait_ld();
+          for (int d = 0; d < 4; ++d) tmem_ld8_nowait(pO + d * (D / 4) + b, v + 8 * d);
+          tmem_wait_ld32(v);
         }
         if (!valid) continue;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float y[8];
 #pragma unroll
-          for (int d = 0; d < 8; ++d) y[d] = __uint_as_float(v[d & 3][2 * k + (d >> 2)]);
+          for (int d = 0; d < 8; ++d) y[d] = __uint_as_float(v[8 * (d & 3) + 2 * k + (d >> 2)]);
           const uint32_t c = 4 * b + 8 * k;
           if (whole) {
             finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, l, y);
@@ -483,9 +529,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_tile_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
   }
 }
 
@@ -650,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
       for (int c = 0; c < 4; ++c) {
         uint32_t v[32];
         tmem_ld32_nowait(pS + c * 32, v);
-        tmem_wait_ld();
+        tmem_wait_ld32(v);
         if (c == 3) {  // in registers: the accumulator is free
           tc_fence_before();
           __syncwarp();
@@ -688,23 +734,24 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
 
 // ---- launches ---------------------------------------------------------------------------
 
-// At most two CTAs may be on an SM: each holds half of its TMEM.
+// Shared memory that lets at most two CTAs be on an SM, where each holds half of its TMEM.
 constexpr size_t kTwoPerSm = 80 * 1024;
 
-template <class T, int D>
+template <class T, int D, int kTiles>
 cudaError_t tile(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  auto *kern = attend_tile_kernel<T, D>;
-  const size_t smem = std::max(tile_smem<D>(), kTwoPerSm);
+  auto *kern = attend_tile_kernel<T, D, kTiles>;
+  const size_t smem = std::max(TileSmem<D, kTiles>::bytes, kTiles == 1 ? kTwoPerSm : size_t(0));
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(plan.units, a.kv.heads), kThreads, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
+  kern<<<dim3(plan.units, a.kv.heads), 128 * kTiles + 160, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
   return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t tile_type(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  return a.dtype == VG_F16 ? tile<__half, D>(a, plan, s) : tile<__nv_bfloat16, D>(a, plan, s);
+cudaError_t tile_type(const AttendArgs &a, const Plan &plan, uint32_t tiles, cudaStream_t s) {
+  if (a.dtype == VG_F16) return tiles == 1 ? tile<__half, D, 1>(a, plan, s) : tile<__half, D, 2>(a, plan, s);
+  return tiles == 1 ? tile<__nv_bfloat16, D, 1>(a, plan, s) : tile<__nv_bfloat16, D, 2>(a, plan, s);
 }
 
 template <int D>
@@ -730,13 +777,13 @@ cudaError_t launch_kv_query_tiles(const AttendArgs &a, const Plan &plan, uint32_
   return cudaGetLastError();
 }
 
-cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, uint32_t tiles, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
   switch (a.kv.dim) {
-    case 32: return tile_type<32>(a, plan, s);
-    case 64: return tile_type<64>(a, plan, s);
-    case 96: return tile_type<96>(a, plan, s);
-    default: return tile_type<128>(a, plan, s);
+    case 32: return tile_type<32>(a, plan, tiles, s);
+    case 64: return tile_type<64>(a, plan, tiles, s);
+    case 96: return tile_type<96>(a, plan, tiles, s);
+    default: return tile_type<128>(a, plan, tiles, s);
   }
 }
 

@@ -166,7 +166,7 @@ uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, uint32_t
 constexpr size_t kScoreBytes = size_t(1) << 30;  // stored scores of one launch, at most
 constexpr uint64_t kDecodeSlots = 148 * 3;       // CTAs of the decoding kernel that run at once
 constexpr uint32_t kDecodeQuantum = 64;          // 4 warps of 16 tokens
-constexpr uint64_t kTileSlots = 148 * 2;         // CTAs of the tile kernel that run at once
+constexpr uint64_t kTileSlots = 148 * 2;         // CTAs of the tile kernel that run at once; half as many of two row tiles
 constexpr uint32_t kSplitOverhead = 128;         // of a unit, in tokens
 
 // Query tiles of a plan's rows, for the tile kernels.
@@ -231,19 +231,20 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
   return VG_OK;
 }
 
-// Sequences of more rows.
-int attend_tiles(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
-  const auto blocks = [&](const PlanSeq &e) { return ceil_div(e.count * a.group, kTileRows); };
+// Sequences of more rows, in units of `tiles` row tiles.
+int attend_tiles(vg_kv_cache *kv, AttendArgs a, Plan &plan, uint32_t tiles, cudaStream_t s) {
+  const uint32_t unit_rows = tiles * kTileRows;
+  const auto blocks = [&](const PlanSeq &e) { return ceil_div(e.count * a.group, unit_rows); };
   VG_TRY(query_tiles(kv, a, plan, s));
-  a.chunk = pick_chunk(plan, kTileSlots, kTileRows, kSplitOverhead,
+  a.chunk = pick_chunk(plan, tiles == 1 ? kTileSlots : kTileSlots / 2, kTileRows, kSplitOverhead,
                        [&](const PlanSeq &e) { return uint64_t(kv->view.heads) * blocks(e); });
   VG_TRY(set_units(plan, [&](const PlanSeq &e) { return uint64_t(blocks(e)) * std::max(1u, ceil_div(e.len, a.chunk)); }));
   uint32_t max_rows = 0;  // of the sequences that are cut
   for (uint32_t i = 0; i < plan.n; ++i)
     if (plan.s[i].len > a.chunk) max_rows = std::max(max_rows, plan.s[i].count * a.group);
-  if (max_rows) VG_TRY(reserve_parts(kv, a, plan, kTileRows));
-  VG_CU(launch_kv_attend_tiles(a, plan, s));
-  if (max_rows) VG_CU(launch_kv_attend_join(a, plan, kTileRows, max_rows, s));
+  if (max_rows) VG_TRY(reserve_parts(kv, a, plan, unit_rows));
+  VG_CU(launch_kv_attend_tiles(a, plan, tiles, s));
+  if (max_rows) VG_CU(launch_kv_attend_join(a, plan, unit_rows, max_rows, s));
   if (a.lse2) VG_TRY(weigh_tiles(a, plan, s));
   return VG_OK;
 }
@@ -422,11 +423,15 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
       VG_CU(kv->ws_lse.reserve(rows * a.q_heads * sizeof(float)));
       a.lse2 = kv->ws_lse.as<float>();
     }
-    const auto few = [&](uint32_t count) { return count <= kDecodeRows / a.group; };
+    // by the rows of a key/value head: 16 in the decoding kernel, one row tile, more
     const auto no_units = [](size_t, PlanSeq &) { return 0u; };
-    VG_TRY(for_plans_of(kv, counts, few, no_units, [&](Plan &plan) { return attend_decode(kv, a, plan, s); }));
-    VG_TRY(for_plans_of(kv, counts, [&](uint32_t c) { return !few(c); }, no_units,
-                        [&](Plan &plan) { return attend_tiles(kv, a, plan, s); }));
+    const auto rows_of = [&](uint32_t count) { return uint64_t(count) * a.group; };
+    VG_TRY(for_plans_of(kv, counts, [&](uint32_t c) { return rows_of(c) <= kDecodeRows; }, no_units,
+                        [&](Plan &plan) { return attend_decode(kv, a, plan, s); }));
+    VG_TRY(for_plans_of(kv, counts, [&](uint32_t c) { return rows_of(c) > kDecodeRows && rows_of(c) <= kTileRows; },
+                        no_units, [&](Plan &plan) { return attend_tiles(kv, a, plan, 1, s); }));
+    VG_TRY(for_plans_of(kv, counts, [&](uint32_t c) { return rows_of(c) > kTileRows; }, no_units,
+                        [&](Plan &plan) { return attend_tiles(kv, a, plan, 2, s); }));
     return VG_OK;
   });
 }

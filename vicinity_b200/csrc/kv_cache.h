@@ -127,8 +127,8 @@ constexpr int kTileRows = 128;
 size_t query_tile_bytes(uint32_t dim);
 // blocks: row blocks of the plan (per head)
 cudaError_t launch_kv_query_tiles(const AttendArgs &a, const Plan &plan, uint32_t blocks, cudaStream_t s);
-// Any number of rows.  Units: row blocks times chunks (at least one) of each sequence.
-cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+// tiles: 1 or 2 row tiles a unit.  Units: blocks of tiles * kTileRows rows times chunks (at least one) of each sequence.
+cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, uint32_t tiles, cudaStream_t s);
 // Weights from recomputed scores.  Units: kWeighRows tokens.
 constexpr uint32_t kWeighRows = 128;
 cudaError_t launch_kv_weigh_tiles(const AttendArgs &a, const Plan &plan, cudaStream_t s);
