@@ -17,6 +17,10 @@
 //                         (keys as they are; values transposed: tokens are the
 //                         contraction of the second product)
 //   1 warp                copies the query tiles, issues S = Q K^T and O += P V
+// With two row tiles the softmax warps hold their row's 128 scores in
+// registers: the block is launched with 128 a thread (16 warps, three of them
+// idle) and moves them to 176 for softmax, 96 for conversion and 64 for the
+// rest.  Half-size CTAs read S twice instead, 32 scores at a time.
 // Every wait is bounded: a protocol error sets the error flag and the kernel
 // drains its copies and products, frees its TMEM and returns.
 #include "common.cuh"
@@ -83,6 +87,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Registers of the calling warpgroup's threads, drawn from what the block was launched with.
+template <int kCount, bool kMore>
+__device__ __forceinline__ void set_registers() {
+  if (kMore) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCount));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCount));
+}
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -219,7 +230,7 @@ struct TileSmem {  // offsets from a 1024-byte boundary; kTiles stages of codes
 };
 
 template <class T, int D, int kTiles>
-__global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
+__global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     attend_tile_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan, const bool ovec) {
   using Smem = TileSmem<D, kTiles>;
   constexpr int kSoftWarps = 4 * kTiles, kMmaWarp = kSoftWarps + 4;
@@ -233,8 +244,9 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
   uint64_t *bars = reinterpret_cast<uint64_t *>(sm + Smem::bars);
   uint64_t *qfull = bars, *drain = bars + 1, *tfull = bars + 2;           // tfull[2]
   uint64_t *kfull = bars + 4, *kempty = bars + 6, *vfull = bars + 8, *vempty = bars + 10;  // [kTiles] stages
-  uint64_t *sfull = bars + 12, *pfull = bars + 14, *pvdone = bars + 16;   // [kTiles] row tiles
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
+  uint64_t *sfull = bars + 12, *pvdone = bars + 14;                       // [kTiles] row tiles
+  uint64_t *pfull = bars + 16;                                            // [kTiles][2] halves of a tile's tokens
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 20);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = lane_id();
 
@@ -262,7 +274,8 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
       mbar_init(vfull + i, 4);
       mbar_init(vempty + i, 1);
       mbar_init(sfull + i, 1);
-      mbar_init(pfull + i, 4);
+      mbar_init(pfull + 2 * i, 4);
+      mbar_init(pfull + 2 * i + 1, 4);
       mbar_init(pvdone + i, 1);
     }
     *abort_flag = 0;
@@ -284,9 +297,10 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
     if (a.error) *reinterpret_cast<volatile int *>(a.error) = code;
   };
 
-  if (warp == kMmaWarp) {
+  if (warp >= kMmaWarp) {
     // ---- query tiles and products ----
-    if (lane == 0 && tiles) {
+    if (kTiles == 2) set_registers<64, false>();
+    if (warp == kMmaWarp && lane == 0 && tiles) {
       mbar_arrive_expect_tx(qfull, row_tiles * Smem::kQ);
       for (uint32_t x = 0; x < row_tiles; ++x)
         bulk_copy_g2s(sQ + x * Smem::kQ, a.q_tiles + (q_at + static_cast<size_t>(x) * kv.heads) * Smem::kQ, Smem::kQ,
@@ -296,7 +310,7 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
       auto scores = [&](uint32_t x, uint32_t i) {  // S of row tile x and token tile i
         const uint32_t st = i % kTiles;
         if (x == 0) {
-          ok = ok && mbar_wait_sleep(kfull + st, (i / kTiles) & 1);
+          ok = ok && mbar_wait(kfull + st, (i / kTiles) & 1);
           if (!ok) return;
           tc_fence_after();
         }
@@ -313,13 +327,19 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
       for (uint32_t i = 0; ok && i < tiles; ++i) {
         const uint32_t st = i % kTiles;
         for (uint32_t x = 0; ok && x < row_tiles; ++x) {
-          ok = !*abort_flag && (x || mbar_wait_sleep(vfull + st, (i / kTiles) & 1)) && mbar_wait_sleep(pfull + x, i & 1);
-          if (!ok) break;
-          tc_fence_after();
+          ok = !*abort_flag && (x || mbar_wait(vfull + st, (i / kTiles) & 1));
 #pragma unroll
-          for (int k = 0; k < static_cast<int>(kTok) / 16; ++k)
-            umma_ts(tmem + (kTiles + x) * kTok, tmem + x * kTok + k * 8,
-                    umma_desc(bV + st * Smem::kV + (k >> 2) * (D * 128) + (k & 3) * 32), f16_idesc(D), i != 0 || k != 0);
+          for (int h = 0; h < 2; ++h) {  // the half of the tokens whose P is there
+            ok = ok && mbar_wait(pfull + 2 * x + h, i & 1);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)
+              umma_ts(tmem + (kTiles + x) * kTok, tmem + x * kTok + k * 8,
+                      umma_desc(bV + st * Smem::kV + (k >> 2) * (D * 128) + (k & 3) * 32), f16_idesc(D),
+                      i != 0 || k != 0);
+          }
+          if (!ok) break;
           umma_commit(pvdone + x);
           if (x + 1 == row_tiles) umma_commit(vempty + st);
           // the next S takes the place of the P just used
@@ -332,6 +352,7 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
     }
   } else if (warp >= kSoftWarps) {
     // ---- codes to binary16 tiles ----
+    if (kTiles == 2) set_registers<96, false>();
     const uint32_t tid = threadIdx.x - kSoftWarps * 32;
     const int8_t *kc = kv.codes[0] + (r * kv.stride + t0) * D, *vc = kv.codes[1] + (r * kv.stride + t0) * D;
     const float *ks = kv.scales[0] + r * nb, *vs = kv.scales[1] + r * nb;
@@ -378,26 +399,97 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
       if (lane == 0) mbar_arrive(vfull + st);
     }
     if (!ok) give_up(2);
-  } else if (static_cast<uint32_t>(warp >> 2) < row_tiles) {
+  } else {
     // ---- softmax: thread = row = TMEM lane ----
+    if (kTiles == 2) set_registers<176, true>();
     const uint32_t x = warp >> 2, wr = threadIdx.x & 127;
     const uint32_t row = rb * kUnitRows + threadIdx.x;
     const bool valid = row < rows;
     const uint32_t qi = row / a.group;
     const uint32_t lim = valid ? tokens_seen(ps, qi, a.causal) : 0xffffffffu;
     const uint32_t warp_lim = __reduce_min_sync(VG_FULL_MASK, lim);
-    const float f_row = a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
+    const uint32_t my_tiles = x < row_tiles ? tiles : 0;  // a row tile past the unit's rows has nothing to do
+    const float f_row = x >= row_tiles ? 0.0f : a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t pS = tmem + x * kTok + lane_base, pO = tmem + (kTiles + x) * kTok + lane_base;
+    float mu = -VG_INF, l = 0.0f;
     // products of 32 tokens from `from` on that the row does not see
-    auto hide = [&](uint32_t (&v)[32], uint32_t from) {
+    auto hide = [&](uint32_t *v, uint32_t from) {
 #pragma unroll
       for (int k = 0; k < 32; ++k)
         if (from + k >= lim) v[k] = 0xff800000u;
     };
-    float mu = -VG_INF, l = 0.0f;
+    // largest score plus log2 of the value scale of 32 products; the factors
+    // are above 0, so that -inf stays -inf
+    auto largest = [&](const uint32_t *v, const float4 *tab, float m) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 e = tab[g];
+        float top = -VG_INF;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(v[16 * g + k]));
+        m = fmaxf(m, fmaf(top, fmaxf(f_row * e.x, 1e-37f), e.y));
+      }
+      return m;
+    };
+    // takes the reference up to m where it lags too far: the sums so far shrink
+    auto raise = [&](float m, bool sums) {
+      if (!__any_sync(VG_FULL_MASK, m > mu + kLazy)) return;
+      m = fmaxf(m, mu);
+      const float c = m == -VG_INF ? 1.0f : exp2_approx(mu - m);
+      mu = m;
+      l *= c;
+      if (!sums) return;
+#pragma unroll 1
+      for (int b = 0; b < D; b += 16) {
+        uint32_t v[16];
+        tmem_ld8_nowait(pO + b, v);
+        tmem_ld8_nowait(pO + b + 8, v + 8);
+        tmem_wait_ld16(v);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * c);
+        tmem_st16(pO + b, v);
+      }
+    };
+    // P of 32 tokens from `from` on, into the denominator and binary16 pairs
+    auto powers = [&](const uint32_t *v, const float4 *tab, uint32_t from, uint32_t (&p)[16]) {
+      const float base = kPShift - (mu == -VG_INF ? 0.0f : mu);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 e = tab[g];
+        const float f = fmaxf(f_row * e.x, 1e-37f), ref = base + e.y;
+        const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
+        f32x2 sum2[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = 16 * g + 2 * k;
+          float2 y = f2_unpack(f2_fma(f2_pack(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f2, ref2));
+          y.x = exp2_approx(y.x);
+          y.y = exp2_approx(y.y);
+          sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(y.x, y.y));
+          p[8 * g + k] = pack_half2(y.x, y.y);
+        }
+        const float2 sum = f2_unpack(f2_add(sum2[0], sum2[1]));
+        l = fmaf(sum.x + sum.y, e.z, l);
+        if (e.w != 0.0f) {  // keys or values read as NaN: so does every row that sees one of them
+          const uint32_t at = from + 16 * g;
+          if (e.w == 2.0f && at < lim) l = __int_as_float(0x7fffffff);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (at + 2 * k < lim) p[8 * g + k] = (p[8 * g + k] & 0xffff0000u) | 0x7fffu;
+            if (at + 2 * k + 1 < lim) p[8 * g + k] |= 0x7fff0000u;
+          }
+        }
+      }
+    };
+    auto half_done = [&](int h) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull + 2 * x + h);
+    };
     bool ok = true;
-    for (uint32_t i = 0; i < tiles; ++i) {
+    for (uint32_t i = 0; i < my_tiles; ++i) {
       const uint32_t t = t0 + i * kTok;
       const float4 *tab = table + (i & 1) * 8;
       if (!__all_sync(VG_FULL_MASK, mbar_wait_sleep(tfull + (i & 1), (i >> 1) & 1) && mbar_wait_sleep(sfull + x, i & 1))) {
@@ -405,94 +497,55 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
         break;
       }
       tc_fence_after();
-      // the factors of a group's products are above 0, so that -inf stays -inf
+      const bool edge = t + kTok > warp_lim;
       float m = -VG_INF;
-      {
-        uint32_t v[2][32];
-        tmem_ld32_nowait(pS, v[0]);
+      if constexpr (kTiles == 2) {
+        uint32_t v[kTok];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(pS + c * 32, v + c * 32);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld32(v + c * 32);
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) hide(v + c * 32, t + c * 32);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m = largest(v + c * 32, tab + 2 * c, m);
+        raise(m, i != 0);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t(&w)[32] = v[c & 1];
-          tmem_wait_ld32(w);
-          if (c < 3) tmem_ld32_nowait(pS + (c + 1) * 32, v[(c + 1) & 1]);
-          if (t + (c + 1) * 32 > warp_lim) hide(w, t + c * 32);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 e = tab[2 * c + g];
-            float top = -VG_INF;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(w[16 * g + k]));
-            m = fmaxf(m, fmaf(top, fmaxf(f_row * e.x, 1e-37f), e.y));
-          }
-        }
-      }
-      if (__any_sync(VG_FULL_MASK, m > mu + kLazy)) {
-        m = fmaxf(m, mu);
-        const float c = m == -VG_INF ? 1.0f : exp2_approx(mu - m);
-        mu = m;
-        l *= c;
-        if (i) {
-#pragma unroll 1
-          for (int b = 0; b < D; b += 16) {
-            uint32_t v[16];
-            tmem_ld8_nowait(pO + b, v);
-            tmem_ld8_nowait(pO + b + 8, v + 8);
-            tmem_wait_ld16(v);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * c);
-            tmem_st16(pO + b, v);
-          }
-        }
-      }
-      const float base = kPShift - (mu == -VG_INF ? 0.0f : mu);
-      {
-        uint32_t v[2][32];
-        tmem_ld32_nowait(pS, v[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t(&w)[32] = v[c & 1];
-          tmem_wait_ld32(w);
-          if (c < 3) tmem_ld32_nowait(pS + (c + 1) * 32, v[(c + 1) & 1]);
-          if (t + (c + 1) * 32 > warp_lim) hide(w, t + c * 32);
           uint32_t p[16];
+          powers(v + c * 32, tab + 2 * c, t + c * 32, p);
+          tmem_st16(pS + c * 16, p);
+          if (c & 1) half_done(c >> 1);
+        }
+      } else {
+        uint32_t v[2][32];
+        tmem_ld32_nowait(pS, v[0]);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 e = tab[2 * c + g];
-            const float f = fmaxf(f_row * e.x, 1e-37f), ref = base + e.y;
-            const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
-            f32x2 sum2 = 0;
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld32(v[c & 1]);
+          if (c < 3) tmem_ld32_nowait(pS + (c + 1) * 32, v[(c + 1) & 1]);
+          if (edge) hide(v[c & 1], t + c * 32);
+          m = largest(v[c & 1], tab + 2 * c, m);
+        }
+        raise(m, i != 0);
+        tmem_ld32_nowait(pS, v[0]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int j = 16 * g + 2 * k;
-              float2 y = f2_unpack(f2_fma(f2_pack(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), f2, ref2));
-              y.x = exp2_approx(y.x);
-              y.y = exp2_approx(y.y);
-              sum2 = f2_add(sum2, f2_pack(y.x, y.y));
-              p[8 * g + k] = pack_half2(y.x, y.y);
-            }
-            const float2 sum = f2_unpack(sum2);
-            l = fmaf(sum.x + sum.y, e.z, l);
-            if (e.w != 0.0f) {  // keys or values read as NaN: so does every row that sees one of them
-              const uint32_t at = t + c * 32 + 16 * g;
-              if (e.w == 2.0f && at < lim) l = __int_as_float(0x7fffffff);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                if (at + 2 * k < lim) p[8 * g + k] = (p[8 * g + k] & 0xffff0000u) | 0x7fffu;
-                if (at + 2 * k + 1 < lim) p[8 * g + k] |= 0x7fff0000u;
-              }
-            }
-          }
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld32(v[c & 1]);
+          if (c < 3) tmem_ld32_nowait(pS + (c + 1) * 32, v[(c + 1) & 1]);
+          if (edge) hide(v[c & 1], t + c * 32);
+          uint32_t p[16];
+          powers(v[c & 1], tab + 2 * c, t + c * 32, p);
           // P of these 32 tokens lies over S of tokens that have been read (also by the load in flight)
           tmem_st16(pS + c * 16, p);
+          if (c & 1) half_done(c >> 1);
         }
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pfull + x);
     }
-    if (ok && tiles) {
-      ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(pvdone + x, (tiles - 1) & 1));
+    if (ok && my_tiles) {
+      ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(pvdone + x, (my_tiles - 1) & 1));
       tc_fence_after();
     }
     if (ok) {
@@ -501,7 +554,7 @@ __global__ void __launch_bounds__(128 * kTiles + 160, 3 - kTiles)
 #pragma unroll 1
       for (int b = 0; b < D / 4; b += 8) {  // dimensions 4 b .. 4 b + 31
         uint32_t v[32] = {};
-        if (tiles) {
+        if (my_tiles) {
 #pragma unroll
           for (int d = 0; d < 4; ++d) tmem_ld8_nowait(pO + d * (D / 4) + b, v + 8 * d);
           tmem_wait_ld32(v);
@@ -744,7 +797,7 @@ cudaError_t tile(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(plan.units, a.kv.heads), 128 * kTiles + 160, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
+  kern<<<dim3(plan.units, a.kv.heads), kTiles == 2 ? 512 : 288, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
   return cudaGetLastError();
 }
 
