@@ -46,23 +46,41 @@ __device__ __forceinline__ uint32_t f16_idesc(uint32_t n) {  // D f32, A and B b
   return (1u << 4) | ((n >> 3) << 17) | ((kRows >> 4) << 24);
 }
 
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Matrix descriptors differ in their low word only (umma_desc of an address in
+// the first 256 KB); kDescHigh is the rest.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4 | 1u << 16; }
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
 
 // A from TMEM: binary16 pairs, 8 columns per K-step of 16
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
+}
+
+// d = a b^T over `steps` K-steps of two K-major tiles of 128-row K-blocks (low descriptor words)
+__device__ __forceinline__ void umma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps) {
+#pragma unroll 1  // little code: the issuing thread shares the instruction caches with everyone else
+  for (int k = 0; k < steps; k += 2) {
+    const uint32_t off = (k >> 2) * (kKBlockBytes >> 4) + (k & 3) * 2;
+    umma_ss(d, a + off, b + off, idesc, k != 0);
+    umma_ss(d, a + off + 2, b + off + 2, idesc, 1);
+  }
 }
 
 __device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t *v) {
@@ -306,7 +324,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         bulk_copy_g2s(sQ + x * Smem::kQ, a.q_tiles + (q_at + static_cast<size_t>(x) * kv.heads) * Smem::kQ, Smem::kQ,
                       qfull);
       bool ok = mbar_wait_sleep(qfull, 0);
-      const uint32_t bQ = smem_u32(sQ), bK = smem_u32(sK), bV = smem_u32(sV);
+      const uint32_t dQ = desc_low(smem_u32(sQ)), dK = desc_low(smem_u32(sK)), dV = desc_low(smem_u32(sV));
       auto scores = [&](uint32_t x, uint32_t i) {  // S of row tile x and token tile i
         const uint32_t st = i % kTiles;
         if (x == 0) {
@@ -314,12 +332,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           if (!ok) return;
           tc_fence_after();
         }
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * kKBlockBytes + (k & 3) * 32;
-          umma_ss(tmem + x * kTok, umma_desc(bQ + x * Smem::kQ + off), umma_desc(bK + st * Smem::kK + off),
-                  f16_idesc(kTok), k != 0);
-        }
+        umma_rows(tmem + x * kTok, dQ + x * (Smem::kQ >> 4), dK + st * (Smem::kK >> 4), f16_idesc(kTok), D / 16);
         umma_commit(sfull + x);
         if (x + 1 == row_tiles) umma_commit(kempty + st);
       };
@@ -328,16 +341,15 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         const uint32_t st = i % kTiles;
         for (uint32_t x = 0; ok && x < row_tiles; ++x) {
           ok = !*abort_flag && (x || mbar_wait(vfull + st, (i / kTiles) & 1));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {  // the half of the tokens whose P is there
-            ok = ok && mbar_wait(pfull + 2 * x + h, i & 1);
-            if (!ok) break;
+#pragma unroll 1
+          for (int h = 0; ok && h < 2; ++h) {  // the half of the tokens whose P is there
+            ok = mbar_wait(pfull + 2 * x + h, i & 1);
             tc_fence_after();
+            const uint32_t b = dV + st * (Smem::kV >> 4) + h * (D * 128 >> 4);
+            const uint32_t d = tmem + (kTiles + x) * kTok, p = tmem + x * kTok + h * 32;
+            umma_ts(d, p, b, f16_idesc(D), (i | h) != 0);
 #pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; ++k)
-              umma_ts(tmem + (kTiles + x) * kTok, tmem + x * kTok + k * 8,
-                      umma_desc(bV + st * Smem::kV + (k >> 2) * (D * 128) + (k & 3) * 32), f16_idesc(D),
-                      i != 0 || k != 0);
+            for (int k = 1; k < 4; ++k) umma_ts(d, p + k * 8, b + k * 2, f16_idesc(D), 1);
           }
           if (!ok) break;
           umma_commit(pvdone + x);
@@ -413,6 +425,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t pS = tmem + x * kTok + lane_base, pO = tmem + (kTiles + x) * kTok + lane_base;
     float mu = -VG_INF, l = 0.0f;
+    float poison = 0.0f;  // whether the row has seen values (1) or keys (2) that read as NaN
     // products of 32 tokens from `from` on that the row does not see
     auto hide = [&](uint32_t *v, uint32_t from) {
 #pragma unroll
@@ -471,15 +484,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         }
         const float2 sum = f2_unpack(f2_add(sum2[0], sum2[1]));
         l = fmaf(sum.x + sum.y, e.z, l);
-        if (e.w != 0.0f) {  // keys or values read as NaN: so does every row that sees one of them
-          const uint32_t at = from + 16 * g;
-          if (e.w == 2.0f && at < lim) l = __int_as_float(0x7fffffff);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (at + 2 * k < lim) p[8 * g + k] = (p[8 * g + k] & 0xffff0000u) | 0x7fffu;
-            if (at + 2 * k + 1 < lim) p[8 * g + k] |= 0x7fff0000u;
-          }
-        }
+        if (e.w != 0.0f && from + 16 * g < lim) poison = fmaxf(poison, e.w);
       }
     };
     auto half_done = [&](int h) {
@@ -550,6 +555,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     }
     if (ok) {
       const bool whole = ps.len <= a.chunk;
+      const float nan = __int_as_float(0x7fffffff);
+      if (poison == 2.0f) l = nan;
       const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kUnitRows + threadIdx.x;
 #pragma unroll 1
       for (int b = 0; b < D / 4; b += 8) {  // dimensions 4 b .. 4 b + 31
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         for (int k = 0; k < 4; ++k) {
           float y[8];
 #pragma unroll
-          for (int d = 0; d < 8; ++d) y[d] = __uint_as_float(v[8 * (d & 3) + 2 * k + (d >> 2)]);
+          for (int d = 0; d < 8; ++d) y[d] = poison != 0.0f ? nan : __uint_as_float(v[8 * (d & 3) + 2 * k + (d >> 2)]);
           const uint32_t c = 4 * b + 8 * k;
           if (whole) {
             finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, l, y);
@@ -661,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
 
   if (warp == 8) {
     if (lane == 0) {
-      const uint32_t bK = smem_u32(sK);
+      const uint32_t dK = desc_low(smem_u32(sK)), dQ = desc_low(smem_u32(sQ));
       const uint32_t n = nrb - rb0;
       auto copy = [&](uint32_t i) {  // row block rb0 + i into stage i & 1
         const size_t at = static_cast<size_t>(ps.block0 + rb0 + i) * kv.heads + head;
@@ -679,12 +686,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
           break;
         }
         tc_fence_after();
-        const uint32_t bQ = smem_u32(sQ + st * kQBytes);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * kKBlockBytes + (k & 3) * 32;
-          umma_ss(tmem + st * kRows, umma_desc(bK + off), umma_desc(bQ + off), f16_idesc(kRows), k != 0);
-        }
+        umma_rows(tmem + st * kRows, dK, dQ + st * (kQBytes >> 4), f16_idesc(kRows), D / 16);
         umma_commit(qempty + st);
         umma_commit(sfull + st);
         if (i + 2 < n) {
