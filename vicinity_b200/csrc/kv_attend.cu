@@ -11,6 +11,8 @@
 #include "kv_attend.cuh"
 #include "kv_cache.h"
 
+#include <algorithm>
+
 namespace vg {
 
 namespace {
@@ -21,10 +23,14 @@ namespace {
 // four warps takes (sequence, head, chunk of tokens); each warp walks its own
 // 16-token steps, which it copies into its own shared-memory ring (cp.async,
 // kStages steps ahead, no barrier between warps), converts to binary16 in
-// registers and multiplies with mma.sync m16n8k16, the rows' 16 being all that
-// there is.  The order of the dimensions inside a product is free, so a lane
-// takes whole words of a row: dim / 4 consecutive key dimensions, dim / 8
-// consecutive value dimensions.
+// registers and multiplies with mma.sync m16n8k16.  Tokens, then dimensions,
+// are the 16 rows of a product and the queries its 8 columns (kCols: one or two
+// groups of them): with the queries as rows, most of the 16 would be empty and
+// there would be twice as many products.  Scores come out with a token per
+// row; movmatrix turns the probabilities into the second product's operand.
+// The order of the dimensions inside a product is free, so a lane takes whole
+// words of a token: dim / 4 consecutive key dimensions, dim / 8 consecutive
+// value dimensions.
 constexpr int kDecWarps = 4;
 constexpr int kStages = 4;
 constexpr int kStep = 16;  // tokens per step: one scale each for keys and values (blocks are multiples of 16)
@@ -63,17 +69,26 @@ __device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint3
   }
 }
 
-template <class T, int D, bool kScores>
-__global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const __grid_constant__ AttendArgs a,
-                                                                          const __grid_constant__ Plan plan,
-                                                                          const bool qvec, const bool ovec) {
+// transposes an 8 x 8 matrix of binary16 (lane 4 r + c holds columns 2 c, 2 c + 1 of row r)
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <class T, int D, int kCols, bool kScores>
+__global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
+    attend_decode_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan, const bool qvec,
+                         const bool ovec) {
   constexpr int kPlane = kStep * D;                    // bytes of one step's keys (or values)
   constexpr int kStage = 2 * kPlane + 16;              // and the two scales
+  constexpr int kRing = kCols == 1 ? kStages - 1 : kStages;  // fewer stages where more CTAs share an SM
   constexpr int kK = D / 16;                           // key words per lane and token = k-steps
   constexpr int kV = D / 32;                           // value words per lane and token
+  constexpr uint32_t kRowsMax = 8 * kCols;
   extern __shared__ __align__(16) uint8_t dec_smem[];
   const int warp = threadIdx.x >> 5, lane = lane_id(), n = lane >> 2, j = lane & 3;
-  uint8_t *ring = dec_smem + warp * (kStages * kStage);
+  uint8_t *ring = dec_smem + warp * (kRing * kStage);
   const KvView &kv = a.kv;
   const uint32_t unit = blockIdx.x, entry = plan_find(plan, unit), head = blockIdx.y;
   const PlanSeq &ps = plan.s[entry];
@@ -100,23 +115,20 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(warp + i * kDecWarps, i);
+  for (int i = 0; i < kRing - 1; ++i) fetch(warp + i * kDecWarps, i);
 
-  // the lane's two rows: their limits, and the query as A fragments
+  // the queries as B fragments: lane (n, j) holds its dimensions of row n of each group
   const uint32_t rows = ps.count * a.group;
-  const uint32_t score_stride = (ps.len + kStep - 1) / kStep * kStep;
-  float *scores = a.scores + ps.aux + static_cast<size_t>(head) * rows * score_stride;
-  uint32_t lim[2];
-  float qs[2];
-  uint32_t qa[kK][4];
+  const uint32_t row_stride = (rows + 1) & ~1u;  // of the scores: [token][row_stride]
+  float *scores = a.scores + ps.aux + static_cast<size_t>(head) * row_stride * ((ps.len + kStep - 1) / kStep * kStep);
+  float q_scale[kCols];
+  uint32_t qb[kCols][kK][2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t row = n + 8 * h;
+  for (int g = 0; g < kCols; ++g) {
+    const uint32_t row = n + 8 * g;
     float x[D / 4];
-    lim[h] = 0;
     if (row < rows) {
       const uint32_t qi = row / a.group;
-      lim[h] = tokens_seen(ps, qi, a.causal);
       const T *q = static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + qi) * a.q.token +
                    static_cast<int64_t>(head * a.group + row - qi * a.group) * a.q.head + j * (D / 4);
 #pragma unroll
@@ -131,28 +143,47 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
     top = fmaxf(top, __shfl_xor_sync(VG_FULL_MASK, top, 1));
     top = fmaxf(top, __shfl_xor_sync(VG_FULL_MASK, top, 2));
     float inv;
-    row_scale(top, qs[h], inv);
-    qs[h] *= a.scale * kLog2e;
+    row_scale(top, q_scale[g], inv);
+    q_scale[g] *= a.scale * kLog2e;
 #pragma unroll
     for (int s = 0; s < kK; ++s) {
-      qa[s][h] = pack_half2(x[4 * s] * inv, x[4 * s + 1] * inv);
-      qa[s][2 + h] = pack_half2(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
+      qb[g][s][0] = pack_half2(x[4 * s] * inv, x[4 * s + 1] * inv);
+      qb[g][s][1] = pack_half2(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
     }
   }
-
-  float o[D / 8][4];
+  // results: a lane has rows 2 j and 2 j + 1 of each group, tokens n and n + 8
+  uint32_t lim[2 * kCols], all_see = t1;
+  float qs[2 * kCols];
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float mu[2] = {-VG_INF, -VG_INF}, l[2] = {0.0f, 0.0f};
-  const uint32_t all_see = __reduce_min_sync(VG_FULL_MASK, min(n < rows ? lim[0] : t1, n + 8 < rows ? lim[1] : t1));
+  for (int h = 0; h < 2 * kCols; ++h) {
+    const uint32_t row = 8 * (h >> 1) + 2 * j + (h & 1);
+    qs[h] = __shfl_sync(VG_FULL_MASK, q_scale[h >> 1], 4 * (2 * j + (h & 1)));
+    lim[h] = row < rows ? tokens_seen(ps, row / a.group, a.causal) : t1;
+    all_see = min(all_see, lim[h]);
+  }
+  all_see = __reduce_min_sync(VG_FULL_MASK, all_see);
 
-  for (uint32_t step = warp, i = 0; step < steps; step += kDecWarps, ++i) {
-    fetch(step + (kStages - 1) * kDecWarps, (i + kStages - 1) % kStages);
-    cp_async_wait<kStages - 1>();
+  float o[kCols][D / 16][4];
+#pragma unroll
+  for (int g = 0; g < kCols; ++g)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
+  float mu[2 * kCols], l[2 * kCols];
+#pragma unroll
+  for (int h = 0; h < 2 * kCols; ++h) {
+    mu[h] = -VG_INF;
+    l[h] = 0.0f;
+  }
+
+  uint32_t slot = 0;
+  for (uint32_t step = warp; step < steps; step += kDecWarps) {
+    fetch(step + (kRing - 1) * kDecWarps, slot == 0 ? kRing - 1 : slot - 1);
+    cp_async_wait<kRing - 1>();
     __syncwarp();
-    const uint8_t *st = ring + (i % kStages) * kStage;
+    const uint8_t *st = ring + slot * kStage;
+    slot = slot + 1 == kRing ? 0 : slot + 1;
     const uint32_t t = t0 + step * kStep;
-    float s[2][4] = {};
+    float s[kCols][4] = {};  // (token n, rows 2 j, 2 j + 1), (token n + 8, ...)
     {
       uint32_t w0[kK], w1[kK];
       row_words<D>(st, n, j * (D / 4), w0);
@@ -160,80 +191,76 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
 #pragma unroll
       for (int c = 0; c < kK; ++c) {
         const uint32_t x0 = w0[c] ^ 0x80808080u, x1 = w1[c] ^ 0x80808080u;
-        mma_f16(s[0], qa[c], half2_of<0x4140>(x0), half2_of<0x4342>(x0));
-        mma_f16(s[1], qa[c], half2_of<0x4140>(x1), half2_of<0x4342>(x1));
+        const uint32_t ka[4] = {half2_of<0x4140>(x0), half2_of<0x4140>(x1), half2_of<0x4342>(x0), half2_of<0x4342>(x1)};
+#pragma unroll
+        for (int g = 0; g < kCols; ++g) mma_f16(s[g], ka, qb[g][c][0], qb[g][c][1]);
       }
     }
     const float kscale = *reinterpret_cast<const float *>(st + 2 * kPlane);
     const float vscale = *reinterpret_cast<const float *>(st + 2 * kPlane + 4);
-    const float lv = log2_scale(vscale);
-    float gm[2];
+    const float lv = log2_scale(vscale), per_v = inverse_scale(vscale);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float f = kscale * qs[h];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[c >> 1][2 * h + (c & 1)] *= f;
+    for (int h = 0; h < 2 * kCols; ++h) {
+      s[h >> 1][h & 1] *= kscale * qs[h];
+      s[h >> 1][2 + (h & 1)] *= kscale * qs[h];
     }
     if (t + kStep > all_see) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (t + 2 * j + (c & 1) + 8 * (c >> 1) >= lim[h]) s[c >> 1][2 * h + (c & 1)] = -VG_INF;
+      for (int h = 0; h < 2 * kCols; ++h) {
+        if (t + n >= lim[h]) s[h >> 1][h & 1] = -VG_INF;
+        if (t + n + 8 >= lim[h]) s[h >> 1][2 + (h & 1)] = -VG_INF;
+      }
     }
     if (kScores) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (n + 8 * h < rows) {
-          float *sc = scores + static_cast<size_t>(n + 8 * h) * score_stride + t + 2 * j;
-          *reinterpret_cast<float2 *>(sc) = make_float2(s[0][2 * h], s[0][2 * h + 1]);
-          *reinterpret_cast<float2 *>(sc + 8) = make_float2(s[1][2 * h], s[1][2 * h + 1]);
+      for (int g = 0; g < kCols; ++g)
+        if (8u * g + 2 * j < rows) {
+          float *sc = scores + static_cast<size_t>(t + n) * row_stride + 8 * g + 2 * j;
+          *reinterpret_cast<float2 *>(sc) = make_float2(s[g][0], s[g][1]);
+          *reinterpret_cast<float2 *>(sc + 8 * row_stride) = make_float2(s[g][2], s[g][3]);
         }
     }
     bool raise = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      gm[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])) + lv;
-      raise |= gm[h] > mu[h] + kLazy;
-    }
+    for (int h = 0; h < 2 * kCols; ++h)
+      raise |= fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) + lv > mu[h] + kLazy;
     if (__any_sync(VG_FULL_MASK, raise)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        gm[h] = fmaxf(gm[h], __shfl_xor_sync(VG_FULL_MASK, gm[h], 1));
-        gm[h] = fmaxf(gm[h], __shfl_xor_sync(VG_FULL_MASK, gm[h], 2));
-        const float m = fmaxf(mu[h], gm[h]);
+      for (int h = 0; h < 2 * kCols; ++h) {
+        float m = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) + lv;
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
+        m = fmaxf(m, mu[h]);
         const float c = m == -VG_INF ? 1.0f : exp2_approx(mu[h] - m);
         mu[h] = m;
         l[h] *= c;
 #pragma unroll
-        for (int i2 = 0; i2 < D / 8; ++i2) {
-          o[i2][2 * h] *= c;
-          o[i2][2 * h + 1] *= c;
+        for (int i = 0; i < D / 16; ++i) {
+          o[h >> 1][i][h & 1] *= c;
+          o[h >> 1][i][2 + (h & 1)] *= c;
         }
       }
     }
-    uint32_t pa[4];
-    const float per_v = inverse_scale(vscale);
+    uint32_t pb[kCols][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float ref = lv + kPShift - (mu[h] == -VG_INF ? 0.0f : mu[h]);
-      float p[4], sum = 0.0f;
+    for (int g = 0; g < kCols; ++g) {
+      float p[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        p[c] = exp2_approx(s[c >> 1][2 * h + (c & 1)] + ref);
-        sum += p[c];
+      for (int h = 0; h < 2; ++h) {
+        const float ref = lv + kPShift - (mu[2 * g + h] == -VG_INF ? 0.0f : mu[2 * g + h]);
+        p[h] = exp2_approx(s[g][h] + ref);
+        p[2 + h] = exp2_approx(s[g][2 + h] + ref);
+        l[2 * g + h] += (p[h] + p[2 + h]) * per_v;
+        if (vscale != vscale) {  // the values read as NaN: so does every row that sees one of them
+          if (t + n < lim[2 * g + h]) p[h] = vscale;
+          if (t + n + 8 < lim[2 * g + h]) p[2 + h] = vscale;
+        }
       }
-      l[h] += sum * per_v;
-      if (vscale != vscale) {  // the values read as NaN: so does every row that sees one of them
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (t + 2 * j + (c & 1) + 8 * (c >> 1) < lim[h]) p[c] = vscale;
-      }
-      pa[h] = pack_half2(p[0], p[1]);
-      pa[2 + h] = pack_half2(p[2], p[3]);
+      pb[g][0] = transposed(pack_half2(p[0], p[1]));
+      pb[g][1] = transposed(pack_half2(p[2], p[3]));
     }
     {
-      uint32_t w[4][kV];
+      uint32_t w[4][kV];  // tokens 2 j, 2 j + 1, 2 j + 8, 2 j + 9
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         row_words<D>(st + kPlane, 2 * j + (c & 1) + 8 * (c >> 1), n * (D / 8), w[c]);
@@ -244,8 +271,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
           const uint32_t sel = hi ? 0x7362u : 0x5140u;
           const uint32_t x0 = __byte_perm(w[0][c], w[1][c], sel) ^ 0x80808080u;
           const uint32_t x1 = __byte_perm(w[2][c], w[3][c], sel) ^ 0x80808080u;
-          mma_f16(o[4 * c + 2 * hi], pa, half2_of<0x4140>(x0), half2_of<0x4140>(x1));
-          mma_f16(o[4 * c + 2 * hi + 1], pa, half2_of<0x4342>(x0), half2_of<0x4342>(x1));
+          const uint32_t va[4] = {half2_of<0x4140>(x0), half2_of<0x4342>(x0), half2_of<0x4140>(x1), half2_of<0x4342>(x1)};
+#pragma unroll
+          for (int g = 0; g < kCols; ++g) mma_f16(o[g][2 * c + hi], va, pb[g][0], pb[g][1]);
         }
       }
     }
@@ -254,25 +282,23 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
 
   // join the four warps, then write the rows out or, one chunk of several, as partial sums
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(VG_FULL_MASK, l[h], 1);
-    l[h] += __shfl_xor_sync(VG_FULL_MASK, l[h], 2);
-  }
+  for (int h = 0; h < 2 * kCols; ++h)
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) l[h] += __shfl_xor_sync(VG_FULL_MASK, l[h], w);
   cp_async_wait<0>();
   __syncthreads();
-  float *so = reinterpret_cast<float *>(dec_smem);                       // [warp][16][D]
-  float2 *sml = reinterpret_cast<float2 *>(so + kDecWarps * kDecodeRows * D);  // [warp][16]
+  // [warp][row][D], rows padded so that a lane's pairs of dimensions spread over the banks
+  constexpr int kPad = D + 2;
+  float *so = reinterpret_cast<float *>(dec_smem);
+  float2 *sml = reinterpret_cast<float2 *>(so + kDecWarps * kRowsMax * kPad);  // [warp][row]
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float *row = so + (warp * kDecodeRows + n + 8 * h) * D + 2 * j * (D / 8);
+  for (int h = 0; h < 2 * kCols; ++h) {
+    const uint32_t row = 8 * (h >> 1) + 2 * j + (h & 1);
+    float *dst = so + (warp * kRowsMax + row) * kPad + n * (D / 8);
 #pragma unroll
-    for (int i = 0; i < D / 8; i += 4) {
-      *reinterpret_cast<float4 *>(row + i) =
-          make_float4(o[i][2 * h], o[i + 1][2 * h], o[i + 2][2 * h], o[i + 3][2 * h]);
-      *reinterpret_cast<float4 *>(row + D / 8 + i) =
-          make_float4(o[i][2 * h + 1], o[i + 1][2 * h + 1], o[i + 2][2 * h + 1], o[i + 3][2 * h + 1]);
-    }
-    if (j == 0) sml[warp * kDecodeRows + n + 8 * h] = make_float2(mu[h], l[h]);
+    for (int i = 0; i < D / 16; ++i)
+      *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[h >> 1][i][h & 1], o[h >> 1][i][2 + (h & 1)]);
+    if (n == 0) sml[warp * kRowsMax + row] = make_float2(mu[h], l[h]);
   }
   __syncthreads();
   const bool whole = ps.len <= a.chunk;
@@ -280,14 +306,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, 3) attend_decode_kernel(const 
     const uint32_t row = e / (D / 8), c = e % (D / 8) * 8;
     float m = -VG_INF, sum = 0.0f, y[8] = {};
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, sml[w * kDecodeRows + row].x);
+    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, sml[w * kRowsMax + row].x);
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
-      const float2 ml = sml[w * kDecodeRows + row];
+      const float2 ml = sml[w * kRowsMax + row];
       const float f = ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
       sum += f * ml.y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kDecodeRows + row) * D + c + i];
+      for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kRowsMax + row) * kPad + c + i];
     }
     if (whole) {
       const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
@@ -376,25 +402,33 @@ __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_c
   const PlanSeq &ps = plan.s[plan_find(plan, blockIdx.x)];
   const uint32_t t = (blockIdx.x - ps.unit0) * kWeighTile + threadIdx.x, head = blockIdx.y;
   if (t >= ps.len) return;
-  const uint32_t rows = ps.count * a.group, stride = (ps.len + kStep - 1) / kStep * kStep;
-  const float *sc = a.scores + ps.aux + static_cast<size_t>(head) * rows * stride + t;
+  const uint32_t rows = ps.count * a.group, stride = (rows + 1) & ~1u;
+  const float *sc =
+      a.scores + ps.aux + (static_cast<size_t>(head) * ((ps.len + kStep - 1) / kStep * kStep) + t) * stride;
   const float *lse = a.lse2 + static_cast<size_t>(ps.row0) * a.q_heads + head * a.group;
   float sum = 0.0f;
-  for (uint32_t row = 0; row < rows; ++row) {
-    const uint32_t qi = row / a.group;
-    const float x = sc[static_cast<size_t>(row) * stride];
-    const float p = exp2_approx(x - lse[static_cast<size_t>(qi) * a.q_heads + row - qi * a.group]);
-    sum += x == -VG_INF ? 0.0f : p;  // not seen
+  for (uint32_t row = 0; row < rows; row += 2) {
+    const float2 x = *reinterpret_cast<const float2 *>(sc + row);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      if (row + h >= rows) break;
+      const uint32_t qi = (row + h) / a.group;
+      const float y = h ? x.y : x.x;
+      const float p = exp2_approx(y - lse[static_cast<size_t>(qi) * a.q_heads + row + h - qi * a.group]);
+      sum += y == -VG_INF ? 0.0f : p;  // not seen
+    }
   }
   float *w = a.kv.weights + (static_cast<size_t>(ps.seq) * a.kv.heads + head) * a.kv.stride + t;
   *w += sum;
 }
 
-template <class T, int D, bool kScores>
+template <class T, int D, int kCols, bool kScores>
 cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
-  auto *kern = attend_decode_kernel<T, D, kScores>;
-  const int smem = kDecWarps * kStages * (2 * kStep * D + 16);
+  auto *kern = attend_decode_kernel<T, D, kCols, kScores>;
+  constexpr size_t ring = kDecWarps * (kCols == 1 ? kStages - 1 : kStages) * (2 * kStep * D + 16);
+  constexpr size_t join = kDecWarps * 8 * kCols * ((D + 2) * sizeof(float) + sizeof(float2));
+  constexpr size_t smem = std::max(ring, join);
   const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   kern<<<dim3(plan.units, a.kv.heads), kDecWarps * 32, smem, s>>>(a, plan, rows_aligned(a.q, sizeof(T)),
@@ -402,21 +436,27 @@ cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+template <class T, int D>
+cudaError_t decode_rows(const AttendArgs &a, const Plan &plan, uint32_t rows, cudaStream_t s) {
+  if (rows <= 8) return a.scores ? decode<T, D, 1, true>(a, plan, s) : decode<T, D, 1, false>(a, plan, s);
+  return a.scores ? decode<T, D, 2, true>(a, plan, s) : decode<T, D, 2, false>(a, plan, s);
+}
+
 template <class T>
-cudaError_t decode_dim(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+cudaError_t decode_dim(const AttendArgs &a, const Plan &plan, uint32_t rows, cudaStream_t s) {
   switch (a.kv.dim) {
-    case 32: return a.scores ? decode<T, 32, true>(a, plan, s) : decode<T, 32, false>(a, plan, s);
-    case 64: return a.scores ? decode<T, 64, true>(a, plan, s) : decode<T, 64, false>(a, plan, s);
-    case 96: return a.scores ? decode<T, 96, true>(a, plan, s) : decode<T, 96, false>(a, plan, s);
-    default: return a.scores ? decode<T, 128, true>(a, plan, s) : decode<T, 128, false>(a, plan, s);
+    case 32: return decode_rows<T, 32>(a, plan, rows, s);
+    case 64: return decode_rows<T, 64>(a, plan, rows, s);
+    case 96: return decode_rows<T, 96>(a, plan, rows, s);
+    default: return decode_rows<T, 128>(a, plan, rows, s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
+cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, uint32_t max_rows, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
-  return a.dtype == VG_F16 ? decode_dim<__half>(a, plan, s) : decode_dim<__nv_bfloat16>(a, plan, s);
+  return a.dtype == VG_F16 ? decode_dim<__half>(a, plan, max_rows, s) : decode_dim<__nv_bfloat16>(a, plan, max_rows, s);
 }
 
 cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, uint32_t part_rows, uint32_t max_rows,

@@ -164,7 +164,8 @@ uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, uint32_t
 }
 
 constexpr size_t kScoreBytes = size_t(1) << 30;  // stored scores of one launch, at most
-constexpr uint64_t kDecodeSlots = 148 * 3;       // CTAs of the decoding kernel that run at once
+constexpr uint64_t kDecodeSlots8 = 148 * 4;      // CTAs of the decoding kernel that run at once, by rows
+constexpr uint64_t kDecodeSlots16 = 148 * 3;
 constexpr uint32_t kDecodeQuantum = 64;          // 4 warps of 16 tokens
 constexpr uint64_t kTileSlots = 148 * 2;         // CTAs of the tile kernel that run at once; half as many of two row tiles
 constexpr uint32_t kSplitOverhead = 128;         // of a unit, in tokens
@@ -200,17 +201,18 @@ int reserve_parts(vg_kv_cache *kv, AttendArgs &a, const Plan &plan, uint32_t par
 
 // Sequences of at most kDecodeRows rows per key/value head.
 int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
-  a.chunk = pick_chunk(plan, kDecodeSlots, kDecodeQuantum, kSplitOverhead,
-                       [&](const PlanSeq &) { return uint64_t(kv->view.heads); });
   uint32_t max_rows = 0;
+  for (uint32_t i = 0; i < plan.n; ++i) max_rows = std::max(max_rows, plan.s[i].count * a.group);
+  a.chunk = pick_chunk(plan, max_rows <= 8 ? kDecodeSlots8 : kDecodeSlots16, kDecodeQuantum, kSplitOverhead,
+                       [&](const PlanSeq &) { return uint64_t(kv->view.heads); });
   bool split = false;
   size_t scores = 0;
   for (uint32_t i = 0; i < plan.n; ++i) {
     PlanSeq &e = plan.s[i];
-    max_rows = std::max(max_rows, e.count * a.group);
     split |= e.len > a.chunk;
     e.aux = scores;
-    scores += static_cast<size_t>(kv->view.heads) * e.count * a.group * (static_cast<size_t>(ceil_div(e.len, 16)) * 16);
+    scores += static_cast<size_t>(kv->view.heads) * ((e.count * a.group + 1) & ~1u) *
+              (static_cast<size_t>(ceil_div(e.len, 16)) * 16);
   }
   VG_TRY(set_units(plan, [&](const PlanSeq &e) { return std::max(1u, ceil_div(e.len, a.chunk)); }));
   if (split) VG_TRY(reserve_parts(kv, a, plan, kDecodeRows));
@@ -219,7 +221,7 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
     VG_CU(kv->ws_scores.reserve(std::max<size_t>(scores, 1) * sizeof(float)));
     a.scores = kv->ws_scores.as<float>();
   }
-  VG_CU(launch_kv_attend_decode(a, plan, s));
+  VG_CU(launch_kv_attend_decode(a, plan, max_rows, s));
   if (split) VG_CU(launch_kv_attend_join(a, plan, kDecodeRows, max_rows, s));
   if (keep) {
     VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, kWeighTile); }));

@@ -105,7 +105,7 @@ struct AttendArgs {
   float *part_o;    // [..][dim]
   float2 *part_ml;  // [..] (reference mu, denominator)
   // Scores x of the call's rows, for the weights (nullable): entry e has
-  // [heads][rows][len rounded up to 16] from scores + plan.s[e].aux
+  // [heads][len rounded up to 16][rows rounded up to 2] from scores + plan.s[e].aux
   float *scores;
   // Query tiles of the tile kernels, [row block][head], and the factors of
   // their rows, [row block][head][kTileRows]
@@ -114,7 +114,7 @@ struct AttendArgs {
   int *error;       // set nonzero when a bounded wait gives up (host-mapped)
 };
 // Sequences of at most kDecodeRows rows per key/value head.  Units: chunks (at least one per sequence).
-cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, cudaStream_t s);
+cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, uint32_t max_rows, cudaStream_t s);
 // Joins the partial sums of sequences that have more than one unit.
 cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, uint32_t part_rows, uint32_t max_rows,
                                   cudaStream_t s);
