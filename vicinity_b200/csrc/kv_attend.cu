@@ -19,10 +19,10 @@ namespace {
 
 // ---- up to 16 query rows per key/value head ----------------------------------
 //
-// One token of decoding, or a few: bound by reading the codes once.  A CTA of
-// four warps takes (sequence, head, chunk of tokens); each warp walks its own
+// One token of decoding, or a few: bound by reading the codes once.  A CTA
+// (two on an SM) takes (sequence, head, chunk of tokens); each of its warps walks its own
 // 16-token steps, which it copies into its own shared-memory ring (cp.async,
-// kStages steps ahead, no barrier between warps), converts to binary16 in
+// kRing - 1 steps ahead, no barrier between warps), converts to binary16 in
 // registers and multiplies with mma.sync m16n8k16.  Tokens, then dimensions,
 // are the 16 rows of a product and the queries its 8 columns (kCols: one or two
 // groups of them): with the queries as rows, most of the 16 would be empty and
@@ -31,8 +31,6 @@ namespace {
 // The order of the dimensions inside a product is free, so a lane takes whole
 // words of a token: dim / 4 consecutive key dimensions, dim / 8 consecutive
 // value dimensions.
-constexpr int kDecWarps = 4;
-constexpr int kStages = 4;
 constexpr int kStep = 16;  // tokens per step: one scale each for keys and values (blocks are multiples of 16)
 
 // byte offset of (token, byte of its row) in a stage: 16-byte chunks XORed so
@@ -69,6 +67,12 @@ __device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint3
   }
 }
 
+// Factor of a partial sum with reference ml.x in one with reference m >= ml.x;
+// 0 for one that has seen nothing, 1 where its sums are NaN without a reference.
+__device__ __forceinline__ float part_weight(float2 ml, float m) {
+  return ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
+}
+
 // transposes an 8 x 8 matrix of binary16 (lane 4 r + c holds columns 2 c, 2 c + 1 of row r)
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -76,13 +80,20 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
+// Warps of a CTA and their rings' stages, by kCols: what the registers of two
+// CTAs on an SM allow, and some 64 KB on their way to an SM at any time.
+template <int kCols>
+struct Dec {
+  static constexpr int warps = kCols == 1 ? 8 : 6, ring = kCols == 1 ? 3 : 4;
+};
+
 template <class T, int D, int kCols, bool kScores>
-__global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
+__global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
     attend_decode_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan, const bool qvec,
                          const bool ovec) {
   constexpr int kPlane = kStep * D;                    // bytes of one step's keys (or values)
   constexpr int kStage = 2 * kPlane + 16;              // and the two scales
-  constexpr int kRing = kCols == 1 ? kStages - 1 : kStages;  // fewer stages where more CTAs share an SM
+  constexpr int kDecWarps = Dec<kCols>::warps, kRing = Dec<kCols>::ring;
   constexpr int kK = D / 16;                           // key words per lane and token = k-steps
   constexpr int kV = D / 32;                           // value words per lane and token
   constexpr uint32_t kRowsMax = 8 * kCols;
@@ -103,12 +114,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
     if (step < steps) {
       uint8_t *st = ring + slot * kStage;
       const uint32_t t = t0 + step * kStep;
-      const int8_t *sk = kc + static_cast<size_t>(t) * D, *sv = vc + static_cast<size_t>(t) * D;
+      const size_t at = static_cast<size_t>(t) * D + lane * 16;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         const uint32_t c = lane + 32 * i, tok = c / (D / 16), byte = (c % (D / 16)) * 16;
-        cp_async16(st + swz<D>(tok, byte), sk + c * 16);
-        cp_async16(st + kPlane + swz<D>(tok, byte), sv + c * 16);
+        cp_async16(st + swz<D>(tok, byte), kc + at + 512 * i);
+        cp_async16(st + kPlane + swz<D>(tok, byte), vc + at + 512 * i);
       }
       if (lane < 2) cp_async4(st + 2 * kPlane + lane * 4, (lane ? vs : ks) + (t >> kv.block_shift));
     }
@@ -144,7 +155,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
     top = fmaxf(top, __shfl_xor_sync(VG_FULL_MASK, top, 2));
     float inv;
     row_scale(top, q_scale[g], inv);
-    q_scale[g] *= a.scale * kLog2e;
+    q_scale[g] *= fabsf(a.scale) * kLog2e;
+    if (a.scale < 0.0f) inv = -inv;  // factors of the products are not negative
 #pragma unroll
     for (int s = 0; s < kK; ++s) {
       qb[g][s][0] = pack_half2(x[4 * s] * inv, x[4 * s + 1] * inv);
@@ -196,19 +208,18 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
         for (int g = 0; g < kCols; ++g) mma_f16(s[g], ka, qb[g][c][0], qb[g][c][1]);
       }
     }
-    const float kscale = *reinterpret_cast<const float *>(st + 2 * kPlane);
-    const float vscale = *reinterpret_cast<const float *>(st + 2 * kPlane + 4);
-    const float lv = log2_scale(vscale), per_v = inverse_scale(vscale);
+    const float2 scale = *reinterpret_cast<const float2 *>(st + 2 * kPlane);  // of keys, of values
+    const float lv = log2_scale(scale.y), per_v = inverse_scale(scale.y);
+    float f[2 * kCols];
 #pragma unroll
-    for (int h = 0; h < 2 * kCols; ++h) {
-      s[h >> 1][h & 1] *= kscale * qs[h];
-      s[h >> 1][2 + (h & 1)] *= kscale * qs[h];
-    }
-    if (t + kStep > all_see) {
+    for (int h = 0; h < 2 * kCols; ++h) f[h] = scale.x * qs[h];
+    if (t + kStep > all_see) {  // where a factor is 0 or NaN, -inf would not stay: scores from here on
 #pragma unroll
       for (int h = 0; h < 2 * kCols; ++h) {
-        if (t + n >= lim[h]) s[h >> 1][h & 1] = -VG_INF;
-        if (t + n + 8 >= lim[h]) s[h >> 1][2 + (h & 1)] = -VG_INF;
+        float &x = s[h >> 1][h & 1], &y = s[h >> 1][2 + (h & 1)];
+        x = t + n < lim[h] ? x * f[h] : -VG_INF;
+        y = t + n + 8 < lim[h] ? y * f[h] : -VG_INF;
+        f[h] = 1.0f;
       }
     }
     if (kScores) {
@@ -216,18 +227,18 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
       for (int g = 0; g < kCols; ++g)
         if (8u * g + 2 * j < rows) {
           float *sc = scores + static_cast<size_t>(t + n) * row_stride + 8 * g + 2 * j;
-          *reinterpret_cast<float2 *>(sc) = make_float2(s[g][0], s[g][1]);
-          *reinterpret_cast<float2 *>(sc + 8 * row_stride) = make_float2(s[g][2], s[g][3]);
+          *reinterpret_cast<float2 *>(sc) = make_float2(s[g][0] * f[2 * g], s[g][1] * f[2 * g + 1]);
+          *reinterpret_cast<float2 *>(sc + 8 * row_stride) = make_float2(s[g][2] * f[2 * g], s[g][3] * f[2 * g + 1]);
         }
     }
     bool raise = false;
 #pragma unroll
     for (int h = 0; h < 2 * kCols; ++h)
-      raise |= fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) + lv > mu[h] + kLazy;
+      raise |= fmaf(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h], lv) > mu[h] + kLazy;
     if (__any_sync(VG_FULL_MASK, raise)) {
 #pragma unroll
       for (int h = 0; h < 2 * kCols; ++h) {
-        float m = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) + lv;
+        float m = fmaf(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h], lv);
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
         m = fmaxf(m, mu[h]);
@@ -248,12 +259,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float ref = lv + kPShift - (mu[2 * g + h] == -VG_INF ? 0.0f : mu[2 * g + h]);
-        p[h] = exp2_approx(s[g][h] + ref);
-        p[2 + h] = exp2_approx(s[g][2 + h] + ref);
-        l[2 * g + h] += (p[h] + p[2 + h]) * per_v;
-        if (vscale != vscale) {  // the values read as NaN: so does every row that sees one of them
-          if (t + n < lim[2 * g + h]) p[h] = vscale;
-          if (t + n + 8 < lim[2 * g + h]) p[2 + h] = vscale;
+        p[h] = exp2_approx(fmaf(s[g][h], f[2 * g + h], ref));
+        p[2 + h] = exp2_approx(fmaf(s[g][2 + h], f[2 * g + h], ref));
+        l[2 * g + h] = fmaf(p[h] + p[2 + h], per_v, l[2 * g + h]);
+        if (scale.y != scale.y) {  // the values read as NaN: so does every row that sees one of them
+          if (t + n < lim[2 * g + h]) p[h] = scale.y;
+          if (t + n + 8 < lim[2 * g + h]) p[2 + h] = scale.y;
         }
       }
       pb[g][0] = transposed(pack_half2(p[0], p[1]));
@@ -280,7 +291,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
     __syncwarp();  // the slot is free for the next fetch
   }
 
-  // join the four warps, then write the rows out or, one chunk of several, as partial sums
+  // join the warps, then write the rows out or, one chunk of several, as partial sums
 #pragma unroll
   for (int h = 0; h < 2 * kCols; ++h)
 #pragma unroll
@@ -310,7 +321,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kCols == 1 ? 4 : 3)
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
       const float2 ml = sml[w * kRowsMax + row];
-      const float f = ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
+      const float f = part_weight(ml, m);
       sum += f * ml.y;
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kRowsMax + row) * kPad + c + i];
@@ -362,7 +373,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   float sum = 0.0f;
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
     const float2 ml = a.part_ml[first + i * step];
-    const float f = ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
+    const float f = part_weight(ml, m);
     weight[i] = f;
     sum += f * ml.y;
   }
@@ -426,12 +437,13 @@ template <class T, int D, int kCols, bool kScores>
 cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   auto *kern = attend_decode_kernel<T, D, kCols, kScores>;
-  constexpr size_t ring = kDecWarps * (kCols == 1 ? kStages - 1 : kStages) * (2 * kStep * D + 16);
-  constexpr size_t join = kDecWarps * 8 * kCols * ((D + 2) * sizeof(float) + sizeof(float2));
+  constexpr int warps = Dec<kCols>::warps;
+  constexpr size_t ring = warps * Dec<kCols>::ring * (2 * kStep * D + 16);
+  constexpr size_t join = warps * 8 * kCols * ((D + 2) * sizeof(float) + sizeof(float2));
   constexpr size_t smem = std::max(ring, join);
   const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(plan.units, a.kv.heads), kDecWarps * 32, smem, s>>>(a, plan, rows_aligned(a.q, sizeof(T)),
+  kern<<<dim3(plan.units, a.kv.heads), warps * 32, smem, s>>>(a, plan, rows_aligned(a.q, sizeof(T)),
                                                                   rows_aligned(a.out, sizeof(T)));
   return cudaGetLastError();
 }

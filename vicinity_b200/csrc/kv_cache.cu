@@ -133,10 +133,15 @@ int set_units(Plan &plan, Units &&units_of) {
 
 // Tokens per work unit when the tokens of every sequence are cut into chunks.
 // Units run `slots` at a time, so w waves of chunks of c tokens take about
-// w (c + overhead): of one to four full waves, and of leaving the sequences
-// whole, the cheapest.  per_chunk(entry): units of one chunk of it.
+// w (c + kUnitCost), and joining the chunks kJoinCost more: of one to four full
+// waves, and of leaving the sequences whole, the cheapest.  per_chunk(entry):
+// units of one chunk of it.  Costs are in tokens of a unit: a unit's start and
+// end take about 1 us, a join 4 us, where the decoding kernel's take 3 to 4 us per
+// 512 tokens.
+constexpr uint32_t kUnitCost = 128, kJoinCost = 512;
+
 template <class PerChunk>
-uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, uint32_t overhead, PerChunk &&per_chunk) {
+uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, PerChunk &&per_chunk) {
   uint32_t longest = 1;
   for (uint32_t i = 0; i < plan.n; ++i) longest = std::max(longest, plan.s[i].len);
   const auto units = [&](uint32_t chunk) {
@@ -145,16 +150,20 @@ uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, uint32_t
     return n;
   };
   const uint32_t least = std::max(1u, ceil_div(ceil_div(longest, kMaxSplits), quantum));
-  uint32_t best = std::max(least, ceil_div(longest, quantum));
-  uint64_t cost = (units(best * quantum) + slots - 1) / slots * (uint64_t(best) * quantum + overhead);
+  const uint32_t whole = std::max(least, ceil_div(longest, quantum));
+  const auto cost_of = [&](uint32_t c) {
+    return (units(c * quantum) + slots - 1) / slots * (uint64_t(c) * quantum + kUnitCost) + (c < whole ? kJoinCost : 0);
+  };
+  uint32_t best = whole;
+  uint64_t cost = cost_of(whole);
   for (uint32_t w = 1; w <= 4; ++w) {
-    uint32_t lo = least, hi = best;  // the smallest chunk that makes at most w waves
+    uint32_t lo = least, hi = whole;  // the smallest chunk that makes at most w waves
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo) / 2;
       if (units(mid * quantum) <= w * slots) hi = mid;
       else lo = mid + 1;
     }
-    const uint64_t c = (units(lo * quantum) + slots - 1) / slots * (uint64_t(lo) * quantum + overhead);
+    const uint64_t c = cost_of(lo);
     if (c < cost) {
       cost = c;
       best = lo;
@@ -164,11 +173,8 @@ uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, uint32_t
 }
 
 constexpr size_t kScoreBytes = size_t(1) << 30;  // stored scores of one launch, at most
-constexpr uint64_t kDecodeSlots8 = 148 * 4;      // CTAs of the decoding kernel that run at once, by rows
-constexpr uint64_t kDecodeSlots16 = 148 * 3;
-constexpr uint32_t kDecodeQuantum = 64;          // 4 warps of 16 tokens
-constexpr uint64_t kTileSlots = 148 * 2;         // CTAs of the tile kernel that run at once; half as many of two row tiles
-constexpr uint32_t kSplitOverhead = 128;         // of a unit, in tokens
+constexpr uint64_t kSlots = 148 * 2;             // CTAs that run at once, of the decoding and the tile kernel
+constexpr uint32_t kDecodeQuantum = 32;
 
 // Query tiles of a plan's rows, for the tile kernels.
 int query_tiles(vg_kv_cache *kv, AttendArgs &a, Plan &plan, cudaStream_t s) {
@@ -203,8 +209,7 @@ int reserve_parts(vg_kv_cache *kv, AttendArgs &a, const Plan &plan, uint32_t par
 int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
   uint32_t max_rows = 0;
   for (uint32_t i = 0; i < plan.n; ++i) max_rows = std::max(max_rows, plan.s[i].count * a.group);
-  a.chunk = pick_chunk(plan, max_rows <= 8 ? kDecodeSlots8 : kDecodeSlots16, kDecodeQuantum, kSplitOverhead,
-                       [&](const PlanSeq &) { return uint64_t(kv->view.heads); });
+  a.chunk = pick_chunk(plan, kSlots, kDecodeQuantum, [&](const PlanSeq &) { return uint64_t(kv->view.heads); });
   bool split = false;
   size_t scores = 0;
   for (uint32_t i = 0; i < plan.n; ++i) {
@@ -238,7 +243,7 @@ int attend_tiles(vg_kv_cache *kv, AttendArgs a, Plan &plan, uint32_t tiles, cuda
   const uint32_t unit_rows = tiles * kTileRows;
   const auto blocks = [&](const PlanSeq &e) { return ceil_div(e.count * a.group, unit_rows); };
   VG_TRY(query_tiles(kv, a, plan, s));
-  a.chunk = pick_chunk(plan, tiles == 1 ? kTileSlots : kTileSlots / 2, kTileRows, kSplitOverhead,
+  a.chunk = pick_chunk(plan, kSlots / tiles, kTileRows,
                        [&](const PlanSeq &e) { return uint64_t(kv->view.heads) * blocks(e); });
   VG_TRY(set_units(plan, [&](const PlanSeq &e) { return uint64_t(blocks(e)) * std::max(1u, ceil_div(e.len, a.chunk)); }));
   uint32_t max_rows = 0;  // of the sequences that are cut
