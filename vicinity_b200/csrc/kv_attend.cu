@@ -6,6 +6,7 @@
 // the sum of P / vs (powers of two: exact).  Codes are exact in binary16, and a
 // query row is scaled by a power of two into its range, so both products run on
 // the tensor cores in binary16 with f32 sums; only P is rounded, to 11 bits.
+#include "chain.cuh"
 #include "common.cuh"
 #include "elements.cuh"
 #include "kv_attend.cuh"
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
   constexpr int kV = D / 32;                           // value words per lane and token
   constexpr uint32_t kRowsMax = 8 * kCols;
   extern __shared__ __align__(16) uint8_t dec_smem[];
+  chain_release();
   const int warp = threadIdx.x >> 5, lane = lane_id(), n = lane >> 2, j = lane & 3;
   uint8_t *ring = dec_smem + warp * (kRing * kStage);
   const KvView &kv = a.kv;
@@ -352,6 +354,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   __shared__ float weight[kMaxSplits];
   __shared__ float red[kJoinThreads / 32];
   __shared__ float acc[kJoinThreads * 8];
+  chain_release();
+  chain_wait();
   const PlanSeq &ps = plan.s[blockIdx.z];
   const uint32_t head = blockIdx.y, row = blockIdx.x, D = a.kv.dim, rows = ps.count * a.group;
   if (ps.len <= a.chunk || row >= rows) return;
@@ -410,6 +414,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 // Weights from stored scores: a thread takes one token of one head.
 __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_constant__ AttendArgs a,
                                                                   const __grid_constant__ Plan plan) {
+  chain_wait();
   const PlanSeq &ps = plan.s[plan_find(plan, blockIdx.x)];
   const uint32_t t = (blockIdx.x - ps.unit0) * kWeighTile + threadIdx.x, head = blockIdx.y;
   if (t >= ps.len) return;
@@ -475,15 +480,13 @@ cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, uint32_
                                   cudaStream_t s) {
   const dim3 grid(max_rows, a.kv.heads, plan.n);
   const bool vec = rows_aligned(a.out, 2);
-  if (a.dtype == VG_F16) attend_join_kernel<__half><<<grid, kJoinThreads, 0, s>>>(a, plan, part_rows, vec);
-  else attend_join_kernel<__nv_bfloat16><<<grid, kJoinThreads, 0, s>>>(a, plan, part_rows, vec);
-  return cudaGetLastError();
+  return launch_chained(a.dtype == VG_F16 ? attend_join_kernel<__half> : attend_join_kernel<__nv_bfloat16>, grid,
+                        kJoinThreads, 0, s, a, plan, part_rows, vec);
 }
 
 cudaError_t launch_kv_weigh_scores(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
-  weigh_scores_kernel<<<dim3(plan.units, a.kv.heads), kWeighTile, 0, s>>>(a, plan);
-  return cudaGetLastError();
+  return launch_chained(weigh_scores_kernel, dim3(plan.units, a.kv.heads), kWeighTile, 0, s, a, plan);
 }
 
 }  // namespace vg

@@ -23,6 +23,7 @@
 // rest.  Half-size CTAs read S twice instead, 32 scores at a time.
 // Every wait is bounded: a protocol error sets the error flag and the kernel
 // drains its copies and products, frees its TMEM and returns.
+#include "chain.cuh"
 #include "common.cuh"
 #include "elements.cuh"
 #include "f32x2.cuh"
@@ -199,6 +200,7 @@ template <class T>
 __global__ void __launch_bounds__(kImageThreads) query_tiles_kernel(const __grid_constant__ AttendArgs a,
                                                                     const __grid_constant__ Plan plan,
                                                                     const uint32_t blocks, const bool qvec) {
+  chain_release();
   const uint32_t D = a.kv.dim, head = blockIdx.y;
   uint32_t lo = 0, hi = plan.n;  // the entry that row block blockIdx.x belongs to
   while (hi - lo > 1) {
@@ -309,6 +311,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  chain_release();  // not before this CTA has its TMEM: a successor that waits may hold some
+  chain_wait();     // the query tiles
   const uint32_t tmem = *tmem_slot;  // row tile x: S at 128 x, O at 128 (kTiles + x)
   auto give_up = [&](int code) {
     *abort_flag = 1;
@@ -665,6 +669,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
     *abort_flag = 1;
     if (a.error) *reinterpret_cast<volatile int *>(a.error) = code;
   };
+  chain_wait();  // the query tiles and what the attention left of its rows
 
   if (warp == 8) {
     if (lane == 0) {
@@ -799,8 +804,8 @@ cudaError_t tile(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(plan.units, a.kv.heads), kTiles == 2 ? 512 : 288, smem, s>>>(a, plan, rows_aligned(a.out, sizeof(T)));
-  return cudaGetLastError();
+  return launch_chained(kern, dim3(plan.units, a.kv.heads), kTiles == 2 ? 512 : 288, smem, s, a, plan,
+                        rows_aligned(a.out, sizeof(T)));
 }
 
 template <int D>
@@ -816,8 +821,7 @@ cudaError_t weigh(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(plan.units, a.kv.heads), kThreads, smem, s>>>(a, plan);
-  return cudaGetLastError();
+  return launch_chained(kern, dim3(plan.units, a.kv.heads), kThreads, smem, s, a, plan);
 }
 
 }  // namespace

@@ -6,6 +6,7 @@
 // bfloat16): the stored codes are a function of the inputs alone, the same
 // in any precision, at the price of up to one of the eight bits (a scale of
 // max |x| / 127 would use the whole range, but rounds in every product).
+#include "chain.cuh"
 #include "common.cuh"
 #include "elements.cuh"
 #include "kv_cache.h"
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const __grid_
                                                                    int32_t *kept) {
   __shared__ __align__(16) uint32_t hist[4096];
   __shared__ uint32_t warp_sum[2][32], sh_digit, sh_need, sh_count;
+  chain_release();
   const uint32_t head = blockIdx.x, entry = blockIdx.y;
   const PlanSeq &ps = plan.s[entry];
   const uint32_t len = ps.len;
@@ -402,6 +404,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv_gather_kernel(const __grid_c
   uint4 *dst = reinterpret_cast<uint4 *>((u.which ? kv.codes[1] : kv.codes[0]) + (rd * kv.stride + blk0) * kv.dim);
   if (threadIdx.x == 0) top = 0;
   __syncthreads();
+  chain_wait();  // the selection
   if (threadIdx.x < n) {
     const int32_t t = kept[(static_cast<size_t>(entry) * kv.heads + u.head) * budget + blk0 + threadIdx.x];
     at[threadIdx.x] = t;
@@ -479,8 +482,8 @@ cudaError_t launch_kv_gather(const KvView &kv, const Plan &plan, uint32_t budget
                              cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
   return with_items(kv, [&](auto items) {
-    kv_gather_kernel<items.value><<<store_grid(kv, plan), kStoreThreads, 0, s>>>(kv, plan, budget, kept);
-    return cudaGetLastError();
+    return launch_chained(kv_gather_kernel<items.value>, store_grid(kv, plan), kStoreThreads, 0, s, kv, plan, budget,
+                          kept);
   });
 }
 
