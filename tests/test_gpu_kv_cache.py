@@ -606,3 +606,32 @@ def test_empty_calls():
     c.evict([0], [1], 4, 1)
     Rotary(64).apply(torch.zeros(0, dtype=torch.int64, device="cuda"), none)
     assert c.lengths.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("seqs", [16, 17, 40, 300])
+def test_many_sequences(seqs):
+    # plans of up to 16 and of up to 256 sequences, and more than one plan;
+    # some sequences take no part, and the rows of the others still line up
+    g = np.random.default_rng(seqs)
+    m = Mirror(2 * seqs, 48, 1, 32, 16)
+    m.fill(g, [int(c) for c in g.integers(0, 40, seqs)] + [0] * seqs)
+    counts = [int(c) for c in g.integers(0, 4, 2 * seqs)]
+    m.fill(g, counts)
+    m.check()
+    q = _rand(g, sum(counts), 2, 32, dtype="bf16")
+    m.attend(counts, q, "bf16", accumulate=True)
+    more = [int(c) for c in g.choice([0, 1, 20], 2 * seqs)]      # both attention kernels in one call
+    m.attend(more, _rand(g, sum(more), 2, 32, dtype="f16"), "f16", accumulate=True)
+    kept = torch.empty(seqs, 1, 9, dtype=torch.int32, device="cuda")
+    lens = m.cache.lengths.tolist()
+    m.cache.evict(list(range(seqs)), list(range(seqs, 2 * seqs)), 9, 2, kept=kept)
+    for s in range(seqs):
+        at = ref.keep(m.w[s][0], lens[s], 9, 2)
+        assert np.array_equal(kept[s, 0].cpu().numpy(), np.pad(at, (0, 9 - len(at)), constant_values=-1))
+        m.k[seqs + s][0], m.v[seqs + s][0] = m.k[s][0].kept(at), m.v[s][0].kept(at)
+    m.check()
+    lens = m.cache.lengths.tolist()
+    k, v = (torch.empty(sum(lens), 1, 32, dtype=torch.float32, device="cuda") for _ in range(2))
+    m.cache.read([0] * (2 * seqs), lens, k, v)
+    assert np.array_equal(_np(k)[:, 0], np.concatenate([h[0].values() for h in m.k]))
+    assert np.array_equal(_np(v)[:, 0], np.concatenate([h[0].values() for h in m.v]))

@@ -56,6 +56,17 @@ __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
   }
 }
 
+// 8 consecutive 16-bit elements, binary16 or bfloat16 by a flag: for kernels
+// that read or write them at their edges only.
+__device__ __forceinline__ void load8_16(const void *base, int64_t at, bool f16, bool vec, float (&x)[8]) {
+  if (f16) load8(static_cast<const __half *>(base) + at, vec, x);
+  else load8(static_cast<const __nv_bfloat16 *>(base) + at, vec, x);
+}
+__device__ __forceinline__ void store8_16(void *base, int64_t at, bool f16, bool vec, const float (&x)[8]) {
+  if (f16) store8(static_cast<__half *>(base) + at, vec, x);
+  else store8(static_cast<__nv_bfloat16 *>(base) + at, vec, x);
+}
+
 // 16 elements as they lie in memory.
 template <class T>
 struct Raw16 {

@@ -13,6 +13,7 @@
 #include "kv_cache.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vg {
 
@@ -88,9 +89,9 @@ struct Dec {
   static constexpr int warps = kCols == 1 ? 8 : 6, ring = kCols == 1 ? 3 : 4;
 };
 
-template <class T, int D, int kCols, bool kScores>
+template <int D, int kCols, bool kScores, class P>
 __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
-    attend_decode_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan, const bool qvec,
+    attend_decode_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ P plan, const bool qvec,
                          const bool ovec) {
   constexpr int kPlane = kStep * D;                    // bytes of one step's keys (or values)
   constexpr int kStage = 2 * kPlane + 16;              // and the two scales
@@ -142,10 +143,11 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
     float x[D / 4];
     if (row < rows) {
       const uint32_t qi = row / a.group;
-      const T *q = static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + qi) * a.q.token +
+      const int64_t at = static_cast<int64_t>(ps.row0 + qi) * a.q.token +
                    static_cast<int64_t>(head * a.group + row - qi * a.group) * a.q.head + j * (D / 4);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) load8(q + 8 * i, qvec, *reinterpret_cast<float(*)[8]>(x + 8 * i));
+      for (int i = 0; i < D / 32; ++i)
+        load8_16(a.q.p, at + 8 * i, a.dtype == VG_F16, qvec, *reinterpret_cast<float(*)[8]>(x + 8 * i));
     } else {
 #pragma unroll
       for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
     }
     if (whole) {
       const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-      finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
+      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
     } else {
       const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kDecodeRows + row;
       float *dst = a.part_o + at * D + c;
@@ -347,9 +349,9 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
 // groups of threads taking every kGroups-th chunk.
 constexpr int kJoinThreads = 256;
 
-template <class T>
+template <class P>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendArgs a,
-                                                                   const __grid_constant__ Plan plan,
+                                                                   const __grid_constant__ P plan,
                                                                    const uint32_t part_rows, const bool ovec) {
   __shared__ float weight[kMaxSplits];
   __shared__ float red[kJoinThreads / 32];
@@ -407,13 +409,14 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += acc[(w * per + threadIdx.x) * 8 + i];
     const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-    finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
+    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
   }
 }
 
 // Weights from stored scores: a thread takes one token of one head.
+template <class P>
 __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_constant__ AttendArgs a,
-                                                                  const __grid_constant__ Plan plan) {
+                                                                  const __grid_constant__ P plan) {
   chain_wait();
   const PlanSeq &ps = plan.s[plan_find(plan, blockIdx.x)];
   const uint32_t t = (blockIdx.x - ps.unit0) * kWeighTile + threadIdx.x, head = blockIdx.y;
@@ -438,55 +441,54 @@ __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_c
   *w += sum;
 }
 
-template <class T, int D, int kCols, bool kScores>
+template <int D, int kCols, bool kScores>
 cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  static std::atomic<uint64_t> allowed{0};
-  auto *kern = attend_decode_kernel<T, D, kCols, kScores>;
   constexpr int warps = Dec<kCols>::warps;
   constexpr size_t ring = warps * Dec<kCols>::ring * (2 * kStep * D + 16);
   constexpr size_t join = warps * 8 * kCols * ((D + 2) * sizeof(float) + sizeof(float2));
   constexpr size_t smem = std::max(ring, join);
-  const cudaError_t e = allow_smem(kern, smem, allowed);
-  if (e != cudaSuccess) return e;
-  kern<<<dim3(plan.units, a.kv.heads), warps * 32, smem, s>>>(a, plan, rows_aligned(a.q, sizeof(T)),
-                                                                  rows_aligned(a.out, sizeof(T)));
-  return cudaGetLastError();
+  return with_plan(plan, [&](const auto &p) {
+    static std::atomic<uint64_t> allowed{0};
+    auto *kern = attend_decode_kernel<D, kCols, kScores, std::decay_t<decltype(p)>>;
+    const cudaError_t e = allow_smem(kern, smem, allowed);
+    if (e != cudaSuccess) return e;
+    kern<<<dim3(p.units, a.kv.heads), warps * 32, smem, s>>>(a, p, rows_aligned(a.q, 2), rows_aligned(a.out, 2));
+    return cudaGetLastError();
+  });
 }
 
-template <class T, int D>
+template <int D>
 cudaError_t decode_rows(const AttendArgs &a, const Plan &plan, uint32_t rows, cudaStream_t s) {
-  if (rows <= 8) return a.scores ? decode<T, D, 1, true>(a, plan, s) : decode<T, D, 1, false>(a, plan, s);
-  return a.scores ? decode<T, D, 2, true>(a, plan, s) : decode<T, D, 2, false>(a, plan, s);
-}
-
-template <class T>
-cudaError_t decode_dim(const AttendArgs &a, const Plan &plan, uint32_t rows, cudaStream_t s) {
-  switch (a.kv.dim) {
-    case 32: return decode_rows<T, 32>(a, plan, rows, s);
-    case 64: return decode_rows<T, 64>(a, plan, rows, s);
-    case 96: return decode_rows<T, 96>(a, plan, rows, s);
-    default: return decode_rows<T, 128>(a, plan, rows, s);
-  }
+  if (rows <= 8) return a.scores ? decode<D, 1, true>(a, plan, s) : decode<D, 1, false>(a, plan, s);
+  return a.scores ? decode<D, 2, true>(a, plan, s) : decode<D, 2, false>(a, plan, s);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_attend_decode(const AttendArgs &a, const Plan &plan, uint32_t max_rows, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
-  return a.dtype == VG_F16 ? decode_dim<__half>(a, plan, max_rows, s) : decode_dim<__nv_bfloat16>(a, plan, max_rows, s);
+  switch (a.kv.dim) {
+    case 32: return decode_rows<32>(a, plan, max_rows, s);
+    case 64: return decode_rows<64>(a, plan, max_rows, s);
+    case 96: return decode_rows<96>(a, plan, max_rows, s);
+    default: return decode_rows<128>(a, plan, max_rows, s);
+  }
 }
 
 cudaError_t launch_kv_attend_join(const AttendArgs &a, const Plan &plan, uint32_t part_rows, uint32_t max_rows,
                                   cudaStream_t s) {
-  const dim3 grid(max_rows, a.kv.heads, plan.n);
-  const bool vec = rows_aligned(a.out, 2);
-  return launch_chained(a.dtype == VG_F16 ? attend_join_kernel<__half> : attend_join_kernel<__nv_bfloat16>, grid,
-                        kJoinThreads, 0, s, a, plan, part_rows, vec);
+  return with_plan(plan, [&](const auto &p) {
+    return launch_chained(attend_join_kernel<std::decay_t<decltype(p)>>, dim3(max_rows, a.kv.heads, p.n), kJoinThreads,
+                          0, s, a, p, part_rows, rows_aligned(a.out, 2));
+  });
 }
 
 cudaError_t launch_kv_weigh_scores(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
-  return launch_chained(weigh_scores_kernel, dim3(plan.units, a.kv.heads), kWeighTile, 0, s, a, plan);
+  return with_plan(plan, [&](const auto &p) {
+    return launch_chained(weigh_scores_kernel<std::decay_t<decltype(p)>>, dim3(p.units, a.kv.heads), kWeighTile, 0, s,
+                          a, p);
+  });
 }
 
 }  // namespace vg

@@ -100,15 +100,13 @@ cudaError_t allow_smem(Kernel *kern, size_t bytes, std::atomic<uint64_t> &done) 
 }
 
 // The result of one row from its sums: 8 dimensions from c on, and the lse.
-template <class T>
 __device__ __forceinline__ void finish_row(const AttendArgs &a, size_t token, uint32_t hq, uint32_t c, bool ovec,
                                            float mu, float sum, float (&y)[8]) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no token seen: 0
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] *= inv;
-  store8(static_cast<T *>(a.out.p) + static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head +
-             c,
-         ovec, y);
+  store8_16(a.out.p, static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head + c,
+            a.dtype == VG_F16, ovec, y);
   if (c == 0) {
     const float lse2 = sum == 0.0f ? -VG_INF : mu - kPShift + log2f(sum);
     if (a.lse) a.lse[token * a.q_heads + hq] = lse2 * kLn2;

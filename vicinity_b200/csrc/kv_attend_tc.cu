@@ -32,6 +32,7 @@
 #include "umma.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vg {
 
@@ -196,10 +197,10 @@ struct ValueTile {
 // turns its products with key codes times their scale into scores.
 constexpr int kImageThreads = 256;
 
-template <class T>
+template <class P>
 __global__ void __launch_bounds__(kImageThreads) query_tiles_kernel(const __grid_constant__ AttendArgs a,
-                                                                    const __grid_constant__ Plan plan,
-                                                                    const uint32_t blocks, const bool qvec) {
+                                                                    const __grid_constant__ P plan,
+                                                                    const bool qvec) {
   chain_release();
   const uint32_t D = a.kv.dim, head = blockIdx.y;
   uint32_t lo = 0, hi = plan.n;  // the entry that row block blockIdx.x belongs to
@@ -219,9 +220,10 @@ __global__ void __launch_bounds__(kImageThreads) query_tiles_kernel(const __grid
     float x[8] = {};
     if (row < rows && c < D / 8) {
       const uint32_t qi = row / a.group;
-      load8(static_cast<const T *>(a.q.p) + static_cast<int64_t>(ps.row0 + qi) * a.q.token +
+      load8_16(a.q.p,
+               static_cast<int64_t>(ps.row0 + qi) * a.q.token +
                 static_cast<int64_t>(head * a.group + row - qi * a.group) * a.q.head + c * 8,
-            qvec, x);
+               a.dtype == VG_F16, qvec, x);
     }
     float top = 0.0f;
 #pragma unroll
@@ -249,9 +251,9 @@ struct TileSmem {  // offsets from a 1024-byte boundary; kTiles stages of codes
   static constexpr size_t bytes = 1024 + bars + 32 * 8;
 };
 
-template <class T, int D, int kTiles>
+template <int D, int kTiles, class P>
 __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
-    attend_tile_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan, const bool ovec) {
+    attend_tile_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ P plan, const bool ovec) {
   using Smem = TileSmem<D, kTiles>;
   constexpr int kSoftWarps = 4 * kTiles, kMmaWarp = kSoftWarps + 4;
   constexpr uint32_t kColumns = 256 * kTiles;  // per row tile: S (P in its first half) and O
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           for (int d = 0; d < 8; ++d) y[d] = poison != 0.0f ? nan : __uint_as_float(v[8 * (d & 3) + 2 * k + (d >> 2)]);
           const uint32_t c = 4 * b + 8 * k;
           if (whole) {
-            finish_row<T>(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, l, y);
+            finish_row(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, l, y);
           } else {
             float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D + c);
             dst[0] = make_float4(y[0], y[1], y[2], y[3]);
@@ -612,9 +614,9 @@ constexpr size_t weigh_smem() {
   return 1024 + 3 * ((D + 63) / 64) * kKBlockBytes + 2 * kRows * (8 + 4) + kTok * 4 + 128;
 }
 
-template <int D>
+template <int D, class P>
 __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_constant__ AttendArgs a,
-                                                                 const __grid_constant__ Plan plan) {
+                                                                 const __grid_constant__ P plan) {
   extern __shared__ uint8_t weigh_raw[];
   const uint32_t raw = smem_u32(weigh_raw);
   uint8_t *sm = weigh_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -797,31 +799,29 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
 // Shared memory that lets at most two CTAs be on an SM, where each holds half of its TMEM.
 constexpr size_t kTwoPerSm = 80 * 1024;
 
-template <class T, int D, int kTiles>
+template <int D, int kTiles>
 cudaError_t tile(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  auto *kern = attend_tile_kernel<T, D, kTiles>;
   const size_t smem = std::max(TileSmem<D, kTiles>::bytes, kTiles == 1 ? kTwoPerSm : size_t(0));
-  static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e = allow_smem(kern, smem, allowed);
-  if (e != cudaSuccess) return e;
-  return launch_chained(kern, dim3(plan.units, a.kv.heads), kTiles == 2 ? 512 : 288, smem, s, a, plan,
-                        rows_aligned(a.out, sizeof(T)));
-}
-
-template <int D>
-cudaError_t tile_type(const AttendArgs &a, const Plan &plan, uint32_t tiles, cudaStream_t s) {
-  if (a.dtype == VG_F16) return tiles == 1 ? tile<__half, D, 1>(a, plan, s) : tile<__half, D, 2>(a, plan, s);
-  return tiles == 1 ? tile<__nv_bfloat16, D, 1>(a, plan, s) : tile<__nv_bfloat16, D, 2>(a, plan, s);
+  return with_plan(plan, [&](const auto &p) {
+    static std::atomic<uint64_t> allowed{0};
+    auto *kern = attend_tile_kernel<D, kTiles, std::decay_t<decltype(p)>>;
+    const cudaError_t e = allow_smem(kern, smem, allowed);
+    if (e != cudaSuccess) return e;
+    return launch_chained(kern, dim3(p.units, a.kv.heads), kTiles == 2 ? 512 : 288, smem, s, a, p,
+                          rows_aligned(a.out, 2));
+  });
 }
 
 template <int D>
 cudaError_t weigh(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
-  auto *kern = weigh_tile_kernel<D>;
   const size_t smem = std::max(weigh_smem<D>(), kTwoPerSm);
-  static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e = allow_smem(kern, smem, allowed);
-  if (e != cudaSuccess) return e;
-  return launch_chained(kern, dim3(plan.units, a.kv.heads), kThreads, smem, s, a, plan);
+  return with_plan(plan, [&](const auto &p) {
+    static std::atomic<uint64_t> allowed{0};
+    auto *kern = weigh_tile_kernel<D, std::decay_t<decltype(p)>>;
+    const cudaError_t e = allow_smem(kern, smem, allowed);
+    if (e != cudaSuccess) return e;
+    return launch_chained(kern, dim3(p.units, a.kv.heads), kThreads, smem, s, a, p);
+  });
 }
 
 }  // namespace
@@ -829,20 +829,19 @@ cudaError_t weigh(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
 size_t query_tile_bytes(uint32_t dim) { return ((dim + 63) / 64) * kKBlockBytes; }
 
 cudaError_t launch_kv_query_tiles(const AttendArgs &a, const Plan &plan, uint32_t blocks, cudaStream_t s) {
-  const dim3 grid(blocks, a.kv.heads);
-  const bool vec = rows_aligned(a.q, 2);
-  if (a.dtype == VG_F16) query_tiles_kernel<__half><<<grid, kImageThreads, 0, s>>>(a, plan, blocks, vec);
-  else query_tiles_kernel<__nv_bfloat16><<<grid, kImageThreads, 0, s>>>(a, plan, blocks, vec);
-  return cudaGetLastError();
+  return with_plan(plan, [&](const auto &p) {
+    query_tiles_kernel<<<dim3(blocks, a.kv.heads), kImageThreads, 0, s>>>(a, p, rows_aligned(a.q, 2));
+    return cudaGetLastError();
+  });
 }
 
 cudaError_t launch_kv_attend_tiles(const AttendArgs &a, const Plan &plan, uint32_t tiles, cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
   switch (a.kv.dim) {
-    case 32: return tile_type<32>(a, plan, tiles, s);
-    case 64: return tile_type<64>(a, plan, tiles, s);
-    case 96: return tile_type<96>(a, plan, tiles, s);
-    default: return tile_type<128>(a, plan, tiles, s);
+    case 32: return tiles == 1 ? tile<32, 1>(a, plan, s) : tile<32, 2>(a, plan, s);
+    case 64: return tiles == 1 ? tile<64, 1>(a, plan, s) : tile<64, 2>(a, plan, s);
+    case 96: return tiles == 1 ? tile<96, 1>(a, plan, s) : tile<96, 2>(a, plan, s);
+    default: return tiles == 1 ? tile<128, 1>(a, plan, s) : tile<128, 2>(a, plan, s);
   }
 }
 

@@ -85,7 +85,8 @@ __device__ __forceinline__ StoreUnit store_unit(const KvView &kv) {
   const uint32_t u = blockIdx.x / kv.heads;
   return {u >> 1, blockIdx.x - u * kv.heads, static_cast<int>(u & 1)};
 }
-unsigned store_grid(const KvView &kv, const Plan &plan) { return plan.units * 2 * kv.heads; }
+template <class P>
+unsigned store_grid(const KvView &kv, const P &plan) { return plan.units * 2 * kv.heads; }
 
 constexpr int kStoreThreads = 256;
 
@@ -99,8 +100,8 @@ __device__ __forceinline__ uint32_t item_token(uint32_t e, uint32_t per) {
 // are read once into registers (kItems of 16 a thread), their largest magnitude
 // is reduced over the CTA as bits (so infinities and NaN win), and the codes
 // are written; the block's older codes are touched only if its scale grew.
-template <class T, int kItems>
-__global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_constant__ KvView kv, const __grid_constant__ Plan plan,
+template <class T, int kItems, class P>
+__global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_constant__ KvView kv, const __grid_constant__ P plan,
                                                                   const __grid_constant__ Strided k,
     const __grid_constant__ Strided v, const bool kvec,
                                                                   const bool vvec) {
@@ -158,8 +159,8 @@ __global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_c
 }
 
 // One CTA per (tile of tokens, head, K or V): codes times their block's scale.
-template <class T>
-__global__ void __launch_bounds__(kStoreThreads) kv_read_kernel(const __grid_constant__ KvView kv, const __grid_constant__ Plan plan,
+template <class T, class P>
+__global__ void __launch_bounds__(kStoreThreads) kv_read_kernel(const __grid_constant__ KvView kv, const __grid_constant__ P plan,
                                                                 const __grid_constant__ Strided k,
     const __grid_constant__ Strided v, const bool kvec,
                                                                 const bool vvec) {
@@ -230,9 +231,9 @@ __device__ __forceinline__ uint32_t keep_key(float x, bool newest) {
 // enough bins; the two keys that many tokens share, recent ones and weight 0,
 // are counted in registers.  64 rows of 16,384 tokens: SELECT_US; by bisection
 // over a cluster of CTAs, with a barrier a step, 26 us.
-template <bool kOne, uint32_t kHeld>
+template <bool kOne, uint32_t kHeld, class P>
 __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const __grid_constant__ KvView kv,
-                                                                   const __grid_constant__ Plan plan,
+                                                                   const __grid_constant__ P plan,
                                                                    const uint32_t budget, const uint32_t recent,
                                                                    int32_t *kept) {
   __shared__ __align__(16) uint32_t hist[4096];
@@ -385,8 +386,8 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const __grid_
 // One CTA per (destination block, head, K or V): its scale is the largest of
 // its tokens' scales (NaN if one is), and each token's codes are moved, rounded
 // to that scale where their own is smaller.
-template <int kItems>
-__global__ void __launch_bounds__(kStoreThreads) kv_gather_kernel(const __grid_constant__ KvView kv, const __grid_constant__ Plan plan,
+template <int kItems, class P>
+__global__ void __launch_bounds__(kStoreThreads) kv_gather_kernel(const __grid_constant__ KvView kv, const __grid_constant__ P plan,
                                                                   const uint32_t budget, const int32_t *kept) {
   __shared__ float from[128];
   __shared__ int32_t at[128];
@@ -445,10 +446,13 @@ cudaError_t launch_kv_append(const KvView &kv, const Plan &plan, int dtype, cons
                              cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
   const bool kvec = rows_aligned(k, element_size(dtype)), vvec = rows_aligned(v, element_size(dtype));
-  return with_type(dtype, [&](auto t) {
-    return with_items(kv, [&](auto items) {
-      kv_append_kernel<decltype(t), items.value><<<store_grid(kv, plan), kStoreThreads, 0, s>>>(kv, plan, k, v, kvec, vvec);
-      return cudaGetLastError();
+  return with_plan(plan, [&](const auto &p) {
+    return with_type(dtype, [&](auto t) {
+      return with_items(kv, [&](auto items) {
+        kv_append_kernel<decltype(t), items.value>
+            <<<store_grid(kv, p), kStoreThreads, 0, s>>>(kv, p, k, v, kvec, vvec);
+        return cudaGetLastError();
+      });
     });
   });
 }
@@ -457,9 +461,11 @@ cudaError_t launch_kv_read(const KvView &kv, const Plan &plan, int dtype, const 
                            cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
   const bool kvec = rows_aligned(k, element_size(dtype)), vvec = rows_aligned(v, element_size(dtype));
-  return with_type(dtype, [&](auto t) {
-    kv_read_kernel<decltype(t)><<<store_grid(kv, plan), kStoreThreads, 0, s>>>(kv, plan, k, v, kvec, vvec);
-    return cudaGetLastError();
+  return with_plan(plan, [&](const auto &p) {
+    return with_type(dtype, [&](auto t) {
+      kv_read_kernel<decltype(t)><<<store_grid(kv, p), kStoreThreads, 0, s>>>(kv, p, k, v, kvec, vvec);
+      return cudaGetLastError();
+    });
   });
 }
 
@@ -470,20 +476,25 @@ cudaError_t launch_kv_select(const KvView &kv, const Plan &plan, uint32_t budget
   // the fewest tokens a thread that hold the row: short rows cost few rounds
   // of shared-memory additions
   const uint32_t threads = longest <= 256 * 4 ? 256 : kSelectThreads;
-  auto *kern = longest <= threads * 4    ? kv_select_kernel<true, 4>
-               : longest <= threads * 8  ? kv_select_kernel<true, 8>
-               : longest <= threads * 16 ? kv_select_kernel<true, 16>
-                                         : kv_select_kernel<false, 16>;
-  kern<<<dim3(kv.heads, plan.n), threads, 0, s>>>(kv, plan, budget, recent, kept);
-  return cudaGetLastError();
+  return with_plan(plan, [&](const auto &p) {
+    using P = std::decay_t<decltype(p)>;
+    auto *kern = longest <= threads * 4    ? kv_select_kernel<true, 4, P>
+                 : longest <= threads * 8  ? kv_select_kernel<true, 8, P>
+                 : longest <= threads * 16 ? kv_select_kernel<true, 16, P>
+                                           : kv_select_kernel<false, 16, P>;
+    kern<<<dim3(kv.heads, p.n), threads, 0, s>>>(kv, p, budget, recent, kept);
+    return cudaGetLastError();
+  });
 }
 
 cudaError_t launch_kv_gather(const KvView &kv, const Plan &plan, uint32_t budget, const int32_t *kept,
                              cudaStream_t s) {
   if (plan.units == 0) return cudaSuccess;
-  return with_items(kv, [&](auto items) {
-    return launch_chained(kv_gather_kernel<items.value>, store_grid(kv, plan), kStoreThreads, 0, s, kv, plan, budget,
-                          kept);
+  return with_plan(plan, [&](const auto &p) {
+    return with_items(kv, [&](auto items) {
+      return launch_chained(kv_gather_kernel<items.value, std::decay_t<decltype(p)>>, store_grid(kv, p), kStoreThreads,
+                            0, s, kv, p, budget, kept);
+    });
   });
 }
 

@@ -19,7 +19,8 @@ import numpy as np
 from . import _lib
 
 _NAMES = {"float32": _lib.F32, "float16": _lib.F16, "bfloat16": _lib.BF16}
-_CODES: dict = {}  # by the libraries' own dtype objects
+_CODES: dict = {}  # by the libraries' own dtype objects, as _TYPES
+_TYPES: dict = {}
 _SCALINGS = {"none": _lib.ROTARY_PLAIN, "linear": _lib.ROTARY_LINEAR, "by_parts": _lib.ROTARY_BY_PARTS}
 
 
@@ -50,7 +51,10 @@ _HEADS = 32  # bytes of a vg_heads
 
 def _flat(x, name: str, shape: tuple, dtype: str) -> int:
     """Address of a contiguous device array of the given shape and type."""
-    if x.shape != shape or not str(x.dtype).endswith(dtype) or not x.is_contiguous():
+    known = _TYPES.get(x.dtype)
+    if known is None:
+        known = _TYPES[x.dtype] = str(x.dtype).rpartition(".")[2]
+    if known != dtype or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} array of shape {list(shape)}")
     return x.data_ptr()
 
