@@ -635,3 +635,17 @@ def test_many_sequences(seqs):
     m.cache.read([0] * (2 * seqs), lens, k, v)
     assert np.array_equal(_np(k)[:, 0], np.concatenate([h[0].values() for h in m.k]))
     assert np.array_equal(_np(v)[:, 0], np.concatenate([h[0].values() for h in m.v]))
+
+
+def test_streaming_example_runs_them_together():
+    import importlib.util
+
+    from tests.conftest import ROOT
+
+    spec = importlib.util.spec_from_file_location("kv_cache_stream", ROOT / "examples" / "kv_cache_stream.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    # nothing evicted: the outputs differ by the 8-bit codes alone
+    assert example.main(["--prompt", "300", "--steps", "20", "--budget", "600"]) > 0.999
+    # cut down to a quarter: most of the attention is left
+    assert example.main(["--prompt", "1500", "--steps", "60", "--budget", "400"]) > 0.5
