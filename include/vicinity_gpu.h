@@ -407,7 +407,7 @@ int vg_rotary_frequencies(const vg_rotary *r, double *out);
 /* Rotate q and k (k nullable, with k_out) of `tokens` tokens at the given
  * positions (device, int64): (a, b) -> m (a cos t - b sin t, a sin t + b cos t),
  * t = position * frequency, reduced in 64 bits, the rest in f32, rounded once.
- * Head dimensions from dim on are copied.  transpose: -sin, the transposed
+ * Head dimensions (at most 4096) from dim on are copied.  transpose: -sin, the transposed
  * map, which takes the gradient of the outputs to that of the inputs.  An
  * output is its input (same address and strides: in place) or does not
  * overlap any other tensor.  Can be captured into a CUDA graph. */

@@ -649,3 +649,66 @@ def test_streaming_example_runs_them_together():
     assert example.main(["--prompt", "300", "--steps", "20", "--budget", "600"]) > 0.999
     # cut down to a quarter: most of the attention is left
     assert example.main(["--prompt", "1500", "--steps", "60", "--budget", "400"]) > 0.5
+
+
+@pytest.mark.parametrize("which", ["keys", "values"])
+def test_attend_poisoned_keys_or_values_alone(which):
+    # NaN keys make the row NaN, its lse and the weights it gives too; NaN
+    # values the row's output only
+    g = np.random.default_rng(20)
+    for counts in ([1, 1], [30, 50], [200, 1]):
+        m = Mirror(2, 640, 1, 64, 16)
+        m.fill(g, [150, 96])
+        good = _rand(g, 32, 1, 64, dtype="f32")
+        bad = torch.full((32, 1, 64), math.nan, device="cuda")
+        m.append([16, 16], bad if which == "keys" else good, good if which == "keys" else bad)
+        m.fill(g, counts)
+        q = _rand(g, sum(counts), 4, 64, dtype="bf16")
+        m.attend(counts, q, "bf16", accumulate=True)
+        m.attend(counts, q, "bf16", causal=False)
+
+
+def test_weights_without_stored_scores():
+    # the scores of 16 rows over 2.2 million tokens of 8 heads (1.1 GB) are not
+    # kept but computed again: the same weights as from two halves of the rows
+    from vicinity_b200 import KVCache
+
+    n, heads, d = 2_200_000, 8, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache = KVCache(1, n, heads, d, block_tokens=128)
+    k = torch.randn(n, heads, d, generator=g, device="cuda").to(torch.bfloat16)
+    cache.append(k, k, [n])
+    del k
+    q = torch.randn(1, heads, 16, d, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.as_tensor(cache.weights, device="cuda")
+    out = torch.empty(1, heads * 16, d, dtype=torch.bfloat16, device="cuda")
+    cache.attend(q.view(1, -1, d), [1], out, accumulate=True)
+    whole = w[0].clone()
+    w.zero_()
+    halves = []
+    for part in (q[:, :, :8], q[:, :, 8:]):
+        o = torch.empty(1, heads * 8, d, dtype=torch.bfloat16, device="cuda")
+        cache.attend(part.reshape(1, -1, d), [1], o, accumulate=True)
+        halves.append(o.view(1, heads, 8, d))
+    # scores up to about 30 in binary logarithms: |err| <= 2 (d + 16) u 30 + 64 u 22, each way
+    rel = 2 * (2 * (d + 16) * U * 30 + 64 * U * 22)
+    assert ((whole - w[0]).abs() <= rel * w[0] + 1e-12).all()
+    assert abs(float(whole.double().sum()) - heads * 16) <= 1e-2
+    assert torch.allclose(out.view(1, heads, 16, d).float(), torch.cat(halves, 2).float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_rotary_wide_heads():
+    # one pair of a very wide head, many heads: the largest items per CTA
+    from vicinity_b200 import Rotary
+
+    g = np.random.default_rng(21)
+    q = _rand(g, 600, 70, 4096, dtype="bf16")
+    r = Rotary(2)
+    pos = torch.arange(600).cuda()
+    out = torch.empty_like(q)
+    r.apply(pos, q, out_q=out)
+    assert torch.equal(out[..., 2:], q[..., 2:])
+    want = ref.rotary(_np(q[..., :2]), np.arange(600), r.frequencies())
+    assert (np.abs(_np(out[..., :2]) - want) <= _rotary_bound(q[..., :2], want, r.frequencies(), False, 1.0, "bf16")).all()
+    with pytest.raises(ValueError, match="at most 4096"):
+        r.apply(pos[:1], torch.zeros(1, 1, 4104, device="cuda"))

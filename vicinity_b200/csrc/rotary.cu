@@ -127,11 +127,14 @@ cudaError_t launch_rotary(const RotaryTable &tab, int dtype, uint32_t dim, const
   // a CTA takes about 256 sines for its tokens and all heads; with few tokens,
   // one token and a share of the heads, so that the GPU is filled
   a.tokens_per_cta = std::max(1u, 256u / tab.pairs);
-  a.heads_per_cta = a.heads;
+  // (at most 2^24 items a CTA: they are counted in 32 bits)
+  a.heads_per_cta = std::min(a.heads, std::max(1u, (1u << 24) / (a.tokens_per_cta * std::max(1u, a.items))));
   if (tokens < a.tokens_per_cta * kFillCtas) {
     a.tokens_per_cta = 1;
     const uint32_t parts = static_cast<uint32_t>(std::max<size_t>(1, kFillCtas / tokens));
-    a.heads_per_cta = std::max(std::max(1u, kRotaryThreads / 2 / std::max(1u, a.items)), (a.heads + parts - 1) / parts);
+    a.heads_per_cta = std::min(
+        a.heads_per_cta,
+        std::max(std::max(1u, kRotaryThreads / 2 / std::max(1u, a.items)), (a.heads + parts - 1) / parts));
   }
   const dim3 grid(static_cast<uint32_t>((tokens + a.tokens_per_cta - 1) / a.tokens_per_cta),
                   (a.heads + a.heads_per_cta - 1) / a.heads_per_cta);
@@ -216,8 +219,8 @@ int vg_rotary_apply(const vg_rotary *r, int dtype, size_t head_dim, const int64_
   return guarded([&]() -> int {
     if (!r) return fail(VG_ERR_INVALID_PARAMETER, "null rotary table");
     VG_TRY(check_dtype(dtype));
-    if (head_dim < 2 * r->table.pairs || head_dim > 65536)
-      return fail(VG_ERR_DIMENSION_MISMATCH, "head_dim must be at least the rotated dimensions, at most 65536");
+    if (head_dim < 2 * r->table.pairs || head_dim > 4096)
+      return fail(VG_ERR_DIMENSION_MISMATCH, "head_dim must be at least the rotated dimensions, at most 4096");
     if (tokens > 0x7fffffffull) return fail(VG_ERR_INVALID_PARAMETER, "at most 2^31 - 1 tokens");
     if (!k != !k_out) return fail(VG_ERR_INVALID_PARAMETER, "k and k_out go together");
     VG_TRY(check_device(device));
