@@ -32,12 +32,21 @@ struct RotaryArgs {
   bool transpose;
 };
 
+template <int N>
+__device__ __forceinline__ void sines(const float *p, float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    const float4 v = reinterpret_cast<const float4 *>(p)[i];
+    x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+  }
+}
+
 // An item is 8 pairs (halves), 4 pairs (adjacent) or 8 copied elements with
 // vec, one pair or one element without.
 template <class T, bool kVec, bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryTable tab,
                                                                 const __grid_constant__ RotaryArgs a) {
-  extern __shared__ float2 cs[];  // [tokens_per_cta][pairs] (m cos, m sin)
+  extern __shared__ __align__(16) float cs[];  // [tokens_per_cta][2][pairs]: m cos, m sin
   const uint32_t t0 = blockIdx.x * a.tokens_per_cta, nt = min(a.tokens_per_cta, a.tokens - t0);
   const uint32_t h0 = blockIdx.y * a.heads_per_cta, nh = min(a.heads_per_cta, a.heads - h0);
   for (uint32_t e = threadIdx.x; e < nt * tab.pairs; e += kRotaryThreads) {
@@ -47,7 +56,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     float s, c;
     sincospif(static_cast<float>(2.0 * turn), &s, &c);
     s *= tab.magnitude;
-    cs[e] = make_float2(c * tab.magnitude, a.transpose ? -s : s);
+    cs[e + t * tab.pairs] = c * tab.magnitude;
+    cs[e + (t + 1) * tab.pairs] = a.transpose ? -s : s;
   }
   __syncthreads();
   const uint32_t n = nt * nh * a.items;
@@ -59,7 +69,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     const int64_t hh = is_q ? h : h - a.q_heads;
     const T *src = static_cast<const T *>(in.p) + static_cast<int64_t>(t0 + t) * in.token + hh * in.head;
     T *dst = static_cast<T *>(out.p) + static_cast<int64_t>(t0 + t) * out.token + hh * out.head;
-    const float2 *f = cs + t * tab.pairs;
+    const float *fc = cs + 2 * t * tab.pairs, *fs = fc + tab.pairs;
     if (item >= a.pair_items) {
       const uint32_t d = 2 * tab.pairs + (item - a.pair_items) * (kVec ? 8 : 1);
       if (kVec) {
@@ -70,33 +80,35 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
         dst[d] = src[d];
       }
     } else if (kVec && kInterleaved) {
-      float x[8], y[8];
+      float x[8], y[8], c[4], s[4];
       load8(src + item * 8, true, x);
+      sines<4>(fc + item * 4, c);
+      sines<4>(fs + item * 4, s);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 w = f[item * 4 + j];
-        y[2 * j] = x[2 * j] * w.x - x[2 * j + 1] * w.y;
-        y[2 * j + 1] = x[2 * j] * w.y + x[2 * j + 1] * w.x;
+        y[2 * j] = x[2 * j] * c[j] - x[2 * j + 1] * s[j];
+        y[2 * j + 1] = x[2 * j] * s[j] + x[2 * j + 1] * c[j];
       }
       store8(dst + item * 8, true, y);
     } else if (kVec) {
-      float x[8], y[8], u[8], v[8];
+      float x[8], y[8], u[8], v[8], c[8], s[8];
       load8(src + item * 8, true, x);
       load8(src + tab.pairs + item * 8, true, y);
+      sines<8>(fc + item * 8, c);
+      sines<8>(fs + item * 8, s);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 w = f[item * 8 + j];
-        u[j] = x[j] * w.x - y[j] * w.y;
-        v[j] = x[j] * w.y + y[j] * w.x;
+        u[j] = x[j] * c[j] - y[j] * s[j];
+        v[j] = x[j] * s[j] + y[j] * c[j];
       }
       store8(dst + item * 8, true, u);
       store8(dst + tab.pairs + item * 8, true, v);
     } else {
       const uint32_t ia = kInterleaved ? 2 * item : item, ib = kInterleaved ? 2 * item + 1 : item + tab.pairs;
-      const float2 w = f[item];
+      const float c = fc[item], s = fs[item];
       const float x = to_f32(src[ia]), y = to_f32(src[ib]);
-      dst[ia] = from_f32<T>(x * w.x - y * w.y);
-      dst[ib] = from_f32<T>(x * w.y + y * w.x);
+      dst[ia] = from_f32<T>(x * c - y * s);
+      dst[ib] = from_f32<T>(x * s + y * c);
     }
   }
 }
