@@ -383,52 +383,61 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const __grid_
   }
 }
 
-// One CTA per (destination block, head, K or V): its scale is the largest of
-// its tokens' scales (NaN if one is), and each token's codes are moved, rounded
-// to that scale where their own is smaller.
+// One CTA per (destination block, head): per keys and values the block's scale
+// is the largest of its tokens' scales (NaN if one is), and each token's codes
+// are moved, rounded to that scale where their own is smaller.  Bound by memory
+// behind a chain of three loads (place, scale, codes); keys and values together
+// have twice the bytes in flight behind it.
 template <int kItems, class P>
-__global__ void __launch_bounds__(kStoreThreads) kv_gather_kernel(const __grid_constant__ KvView kv, const __grid_constant__ P plan,
+__global__ void __launch_bounds__(kStoreThreads) kv_gather_kernel(const __grid_constant__ KvView kv,
+                                                                  const __grid_constant__ P plan,
                                                                   const uint32_t budget, const int32_t *kept) {
-  __shared__ float from[128];
+  __shared__ float from[2][128];
   __shared__ int32_t at[128];
-  __shared__ uint32_t top;
-  const StoreUnit u = store_unit(kv);
-  const uint32_t entry = plan_find(plan, u.unit);
+  __shared__ uint32_t top[2];
+  const uint32_t unit = blockIdx.x / kv.heads, head = blockIdx.x - unit * kv.heads;
+  const uint32_t entry = plan_find(plan, unit);
   const PlanSeq &ps = plan.s[entry];
   const uint32_t per = kv.dim / 16;
-  const uint32_t b = u.unit - ps.unit0, blk0 = b << kv.block_shift;
+  const uint32_t b = unit - ps.unit0, blk0 = b << kv.block_shift;
   const uint32_t n = min(kv.block, min(ps.len, budget) - blk0);
   const size_t nb = kv.stride >> kv.block_shift;
-  const size_t rs = static_cast<size_t>(ps.seq) * kv.heads + u.head;
-  const size_t rd = static_cast<size_t>(ps.row0) * kv.heads + u.head;
-  const uint4 *src = reinterpret_cast<const uint4 *>((u.which ? kv.codes[1] : kv.codes[0]) + rs * kv.stride * kv.dim);
-  uint4 *dst = reinterpret_cast<uint4 *>((u.which ? kv.codes[1] : kv.codes[0]) + (rd * kv.stride + blk0) * kv.dim);
-  if (threadIdx.x == 0) top = 0;
+  const size_t rs = static_cast<size_t>(ps.seq) * kv.heads + head;
+  const size_t rd = static_cast<size_t>(ps.row0) * kv.heads + head;
+  if (threadIdx.x < 2) top[threadIdx.x] = 0;
   __syncthreads();
   chain_wait();  // the selection
-  if (threadIdx.x < n) {
-    const int32_t t = kept[(static_cast<size_t>(entry) * kv.heads + u.head) * budget + blk0 + threadIdx.x];
-    at[threadIdx.x] = t;
-    const float s = (u.which ? kv.scales[1] : kv.scales[0])[rs * nb + (static_cast<uint32_t>(t) >> kv.block_shift)];
-    from[threadIdx.x] = s;
-    atomicMax(&top, __float_as_uint(s) & 0x7fffffffu);  // positive: ordered by their bits, NaN last
+  const uint32_t token = threadIdx.x & 127, which = threadIdx.x >> 7;
+  if (token < n) {
+    const int32_t t = kept[(static_cast<size_t>(entry) * kv.heads + head) * budget + blk0 + token];
+    const float s = (which ? kv.scales[1] : kv.scales[0])[rs * nb + (static_cast<uint32_t>(t) >> kv.block_shift)];
+    at[token] = t;  // both halves of the CTA write the same
+    from[which][token] = s;
+    atomicMax(&top[which], __float_as_uint(s) & 0x7fffffffu);  // positive: ordered by their bits, NaN last
   }
   __syncthreads();
-  const float s_new = __uint_as_float(top), inv = inverse(s_new);
-  uint4 w[kItems];
+  uint4 w[2][kItems];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     const uint32_t e = threadIdx.x + i * kStoreThreads, t = item_token(e, per);
-    if (e < n * per) w[i] = __ldg(src + static_cast<size_t>(at[t]) * per + (e - t * per));
+    if (e >= n * per) continue;
+    const size_t src = (rs * kv.stride + at[t]) * per + (e - t * per);
+    w[0][i] = __ldg(reinterpret_cast<const uint4 *>(kv.codes[0]) + src);
+    w[1][i] = __ldg(reinterpret_cast<const uint4 *>(kv.codes[1]) + src);
   }
 #pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const uint32_t e = threadIdx.x + i * kStoreThreads;
-    if (e >= n * per) continue;
-    const float ratio = from[item_token(e, per)] * inv;
-    dst[e] = ratio < 1.0f ? rescaled(w[i], ratio) : w[i];
+  for (int c = 0; c < 2; ++c) {
+    const float s_new = __uint_as_float(top[c]), inv = inverse(s_new);
+    uint4 *dst = reinterpret_cast<uint4 *>(kv.codes[c]) + (rd * kv.stride + blk0) * per;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t e = threadIdx.x + i * kStoreThreads;
+      if (e >= n * per) continue;
+      const float ratio = from[c][item_token(e, per)] * inv;
+      dst[e] = ratio < 1.0f ? rescaled(w[c][i], ratio) : w[c][i];
+    }
+    if (threadIdx.x == 0) kv.scales[c][rd * nb + b] = s_new;
   }
-  if (threadIdx.x == 0) (u.which ? kv.scales[1] : kv.scales[0])[rd * nb + b] = s_new;
 }
 
 // f(the number of items of 16 elements that a thread takes of a block)
@@ -492,8 +501,8 @@ cudaError_t launch_kv_gather(const KvView &kv, const Plan &plan, uint32_t budget
   if (plan.units == 0) return cudaSuccess;
   return with_plan(plan, [&](const auto &p) {
     return with_items(kv, [&](auto items) {
-      return launch_chained(kv_gather_kernel<items.value, std::decay_t<decltype(p)>>, store_grid(kv, p), kStoreThreads,
-                            0, s, kv, p, budget, kept);
+      return launch_chained(kv_gather_kernel<items.value, std::decay_t<decltype(p)>>, p.units * kv.heads,
+                            kStoreThreads, 0, s, kv, p, budget, kept);
     });
   });
 }
