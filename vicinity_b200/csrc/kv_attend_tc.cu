@@ -296,8 +296,10 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
       mbar_init(vfull + i, 4);
       mbar_init(vempty + i, 1);
       mbar_init(sfull + i, 1);
-      mbar_init(pfull + 2 * i, 4);
-      mbar_init(pfull + 2 * i + 1, 4);
+      // the warps of a row tile that have rows
+      const uint32_t from = rb * kUnitRows + i * kRows, some = rows > from ? min(4u, (rows - from + 31) / 32) : 4u;
+      mbar_init(pfull + 2 * i, some);
+      mbar_init(pfull + 2 * i + 1, some);
       mbar_init(pvdone + i, 1);
     }
     *abort_flag = 0;
@@ -426,8 +428,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     const uint32_t qi = row / a.group;
     const uint32_t lim = valid ? tokens_seen(ps, qi, a.causal) : 0xffffffffu;
     const uint32_t warp_lim = __reduce_min_sync(VG_FULL_MASK, lim);
-    const uint32_t my_tiles = x < row_tiles ? tiles : 0;  // a row tile past the unit's rows has nothing to do
-    const float f_row = x >= row_tiles ? 0.0f : a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
+    const uint32_t my_tiles = row - lane < rows ? tiles : 0;  // a warp without rows has nothing to do
+    const float f_row = my_tiles == 0 ? 0.0f : a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t pS = tmem + x * kTok + lane_base, pO = tmem + (kTiles + x) * kTok + lane_base;
     float mu = -VG_INF, l = 0.0f;
@@ -636,6 +638,8 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
   const PlanSeq &ps = plan.s[plan_find(plan, unit)];
   const uint32_t t0 = (unit - ps.unit0) * kTok;
   const uint32_t rows = ps.count * a.group, nrb = (rows + kRows - 1) / kRows;
+  // rows of block b, in whole groups of 32: the columns of its products
+  auto columns = [&](uint32_t b) { return min(static_cast<uint32_t>(kRows), (rows - b * kRows + 31) / 32 * 32); };
   const size_t r = static_cast<size_t>(ps.seq) * kv.heads + head;
   // the first row block with a row that sees the tile's first token
   uint32_t rb0 = 0;
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
           break;
         }
         tc_fence_after();
-        umma_rows(tmem + st * kRows, dK, dQ + st * (kQBytes >> 4), f16_idesc(kRows), D / 16);
+        umma_rows(tmem + st * kRows, dK, dQ + st * (kQBytes >> 4), f16_idesc(columns(rb0 + i)), D / 16);
         umma_commit(qempty + st);
         umma_commit(sfull + st);
         if (i + 2 < n) {
@@ -754,12 +758,13 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
       if (ok) ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(sfull + eg, (i >> 1) & 1));
       tc_fence_after();
       f32x2 sum2 = 0;
+      const int groups = static_cast<int>(columns(b)) / 32;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < groups; ++c) {
         uint32_t v[32];
         tmem_ld32_nowait(pS + c * 32, v);
         tmem_wait_ld32(v);
-        if (c == 3) {  // in registers: the accumulator is free
+        if (c + 1 == groups) {  // in registers: the accumulator is free
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(sempty + eg);
