@@ -136,9 +136,13 @@ struct KeyTile {
     for (int i = 0; i < kItems; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(codes) + tid + i * kWorkers);
   }
   __device__ __forceinline__ void store(uint8_t *tile, uint32_t tid) const {
+    // where a step of kWorkers items is whole tokens, a thread's chunk stays
+    constexpr bool kWhole = kWorkers % (D / 16) == 0;
+    const uint32_t tok0 = tid / (D / 16), c0 = tid % (D / 16);
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const uint32_t e = tid + i * kWorkers, tok = e / (D / 16), c = e % (D / 16);
+      const uint32_t e = tid + i * kWorkers;
+      const uint32_t tok = kWhole ? tok0 : e / (D / 16), c = kWhole ? c0 : e % (D / 16);
       const uint32_t x[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -146,7 +150,9 @@ struct KeyTile {
         // order: eight lanes of a token meet eight different bank groups
         const uint32_t hh = (c & 4u) ? 1 - h : h;
         const uint32_t a = hh ? x[2] : x[0], b = hh ? x[3] : x[1];
-        *reinterpret_cast<uint4 *>(tile + tile_byte(kTok, tok, 2 * c + hh)) =
+        // (16 and more tokens further: a multiple of 8 rows, the same swizzle)
+        uint8_t *dst = tile + tile_byte(kTok, tok, 2 * c + hh) + (kWhole ? i * (kWorkers / (D / 16)) * 128 : 0);
+        *reinterpret_cast<uint4 *>(dst) =
             make_uint4(half2_of<0x4140>(a), half2_of<0x4342>(a), half2_of<0x4140>(b), half2_of<0x4342>(b));
       }
     }
@@ -161,19 +167,23 @@ struct KeyTile {
 template <int D>
 struct ValueTile {
   static constexpr int kItems = (kTok / 8) * (D / 4) / 128;
+  static constexpr bool kWhole = 128 % (D / 4) == 0;  // as for the keys
   uint32_t w[kItems][8];
   __device__ __forceinline__ void load(const int8_t *codes, uint32_t tid) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const uint32_t e = tid + i * 128, u = e / (D / 4), c = e % (D / 4);
+      const uint32_t e = tid + i * 128, u = kWhole ? tid / (D / 4) : e / (D / 4), c = kWhole ? tid % (D / 4) : e % (D / 4);
+      const uint32_t *p = reinterpret_cast<const uint32_t *>(codes) + u * 8 * (D / 4) + c + (kWhole ? i * 128 * 8 : 0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[i][k] = __ldg(reinterpret_cast<const uint32_t *>(codes) + (u * 8 + k) * (D / 4) + c);
+      for (int k = 0; k < 8; ++k) w[i][k] = __ldg(p + k * (D / 4));
     }
   }
   __device__ __forceinline__ void store(uint8_t *tile, uint32_t tid) const {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const uint32_t e = tid + i * 128, u = e / (D / 4), c = e % (D / 4);
+      const uint32_t e = tid + i * 128;
+      const uint32_t u = (kWhole ? tid / (D / 4) + i * (128 / (D / 4)) : e / (D / 4));
+      const uint32_t c = kWhole ? tid % (D / 4) : e % (D / 4);
       uint32_t out[4][4];  // [dimension][token pair]
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
