@@ -61,9 +61,10 @@ __device__ __forceinline__ uint4 codes16(const Raw16<T> &x, float inv, bool exot
                     pack4(r[12], r[13], r[14], r[15]));
 }
 
-// The value of byte i of a word of codes
+// The value of byte i of a word of codes: biased by 128 it is the last byte of
+// 2^23 + 128 + code (the conversion instruction has a quarter of the rate).
 __device__ __forceinline__ float code_at(uint32_t c, int i) {
-  return static_cast<float>(static_cast<int>(c << (24 - 8 * i)) >> 24);
+  return __uint_as_float(__byte_perm(c ^ 0x80808080u, 0x4b000000u, 0x7540 | i)) - 8388736.0f;
 }
 
 // Codes rounded to a larger scale; ratio = 2^-k (0 where every code vanishes).
