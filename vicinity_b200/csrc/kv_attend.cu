@@ -33,6 +33,8 @@ namespace {
 // The order of the dimensions inside a product is free, so a lane takes whole
 // words of a token: dim / 4 consecutive key dimensions, dim / 8 consecutive
 // value dimensions.
+// 131,101 tokens x 8 heads x 128, 4 rows a head (268 MB): 50 us, 5.4 TB/s; the
+// copies alone take 46, the rest is the start and the end of the CTAs.
 constexpr int kStep = 16;  // tokens per step: one scale each for keys and values (blocks are multiples of 16)
 
 // byte offset of (token, byte of its row) in a stage: 16-byte chunks XORed so
@@ -346,7 +348,8 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
 // ---- joining the chunks of a sequence -------------------------------------------
 
 // One CTA per (row, head, sequence): 32-byte slices of the row's partial sums,
-// groups of threads taking every kGroups-th chunk.
+// groups of threads taking every kGroups-th chunk.  Latency: about 4 us.  (By
+// the last CTA of the first kernel instead of a launch: 14 us for 74 chunks.)
 constexpr int kJoinThreads = 256;
 
 template <class P>
@@ -413,7 +416,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   }
 }
 
-// Weights from stored scores: a thread takes one token of one head.
+// Weights from stored scores: a thread takes one token of one head.  Storing
+// and reading 4 bytes a row and token replaces reading the keys again.
 template <class P>
 __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_constant__ AttendArgs a,
                                                                   const __grid_constant__ P plan) {

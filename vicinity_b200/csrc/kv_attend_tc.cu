@@ -3,9 +3,14 @@
 //
 // The rows of a key/value head are its queries times the query heads that share
 // it; a tile is 128 rows (the lanes of the TMEM accumulator) by 128 tokens.
-// Bound by the exponentials and the products: 4 dim multiply-adds' worth of
-// tensor work and one ex2 per (row, token), the codes being read from L2 by
-// every row block.  See kv_attend.cu for the scaling of scores and
+// Bound by the two products, 4 dim flops per (row, token), and as much by one
+// ex2 each; the codes are read from L2 by every row block.  1,024 queries x 32
+// heads x 128 over 16,384 tokens (266 GFLOP): 321 us, 0.83 PFLOP/s, tensor and
+// exponential pipes 55 % busy.  Product and softmax of a row tile follow each
+// other, two tiles take turns, and what is left is the time between a product's
+// end and the start of what waits for it; a third tile has no room in TMEM.
+// Their weights (133 GFLOP and the exponentials again): 208 us, the exponential
+// pipe 78 % busy.  See kv_attend.cu for the scaling of scores and
 // probabilities.
 //
 // attend_tile_kernel, one CTA per (sequence, head, kTiles row tiles, chunk of

@@ -101,10 +101,13 @@ __device__ __forceinline__ uint32_t item_token(uint32_t e, uint32_t per) {
 // are read once into registers (kItems of 16 a thread), their largest magnitude
 // is reduced over the CTA as bits (so infinities and NaN win), and the codes
 // are written; the block's older codes are touched only if its scale grew.
+// 16,384 tokens x 8 heads x 128, keys and values in bf16: 22 us, 4.5 TB/s (the
+// time between a CTA's loads and its stores is not covered by others' loads).
 template <class T, int kItems, class P>
-__global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_constant__ KvView kv, const __grid_constant__ P plan,
+__global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_constant__ KvView kv,
+                                                                  const __grid_constant__ P plan,
                                                                   const __grid_constant__ Strided k,
-    const __grid_constant__ Strided v, const bool kvec,
+                                                                  const __grid_constant__ Strided v, const bool kvec,
                                                                   const bool vvec) {
   __shared__ uint32_t part[kStoreThreads / 32];
   const StoreUnit u = store_unit(kv);
@@ -160,10 +163,12 @@ __global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_c
 }
 
 // One CTA per (tile of tokens, head, K or V): codes times their block's scale.
+// Bound by memory: the same 16,384 tokens into bf16 19 us, 5.3 TB/s.
 template <class T, class P>
-__global__ void __launch_bounds__(kStoreThreads) kv_read_kernel(const __grid_constant__ KvView kv, const __grid_constant__ P plan,
+__global__ void __launch_bounds__(kStoreThreads) kv_read_kernel(const __grid_constant__ KvView kv,
+                                                                const __grid_constant__ P plan,
                                                                 const __grid_constant__ Strided k,
-    const __grid_constant__ Strided v, const bool kvec,
+                                                                const __grid_constant__ Strided v, const bool kvec,
                                                                 const bool vvec) {
   const StoreUnit u = store_unit(kv);
   const PlanSeq &ps = plan.s[plan_find(plan, u.unit)];
@@ -230,8 +235,8 @@ __device__ __forceinline__ uint32_t keep_key(float x, bool newest) {
 // histograms in shared memory with their scans, or fewer -- the search stops
 // when a bin is kept whole.  12 bits spread weights of a few exponents over
 // enough bins; the two keys that many tokens share, recent ones and weight 0,
-// are counted in registers.  64 rows of 16,384 tokens: SELECT_US; by bisection
-// over a cluster of CTAs, with a barrier a step, 26 us.
+// are counted in registers.  64 rows of 16,384 tokens: 14 us (4 MB: the memory
+// would take 1); by bisection over a cluster of CTAs, with a barrier a step, 26.
 template <bool kOne, uint32_t kHeld, class P>
 __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const __grid_constant__ KvView kv,
                                                                    const __grid_constant__ P plan,
@@ -388,7 +393,8 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const __grid_
 // is the largest of its tokens' scales (NaN if one is), and each token's codes
 // are moved, rounded to that scale where their own is smaller.  Bound by memory
 // behind a chain of three loads (place, scale, codes); keys and values together
-// have twice the bytes in flight behind it.
+// have twice the bytes in flight behind it.  8 sequences x 8 heads x 2,048
+// tokens: 13 us, 5.0 TB/s.
 template <int kItems, class P>
 __global__ void __launch_bounds__(kStoreThreads) kv_gather_kernel(const __grid_constant__ KvView kv,
                                                                   const __grid_constant__ P plan,
