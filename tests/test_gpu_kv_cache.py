@@ -712,3 +712,120 @@ def test_rotary_wide_heads():
     assert (np.abs(_np(out[..., :2]) - want) <= _rotary_bound(q[..., :2], want, r.frequencies(), False, 1.0, "bf16")).all()
     with pytest.raises(ValueError, match="at most 4096"):
         r.apply(pos[:1], torch.zeros(1, 1, 4104, device="cuda"))
+
+
+# ---- the whole range of scales ------------------------------------------------
+
+
+def _attention64(q, k, v, causal, scale):
+    """q [n, g, d] over k, v [len, d] of one head, in 64 bits on the GPU: (out, lse, weights, sum p |v|, max scale sum |q k|)."""
+    n, L = q.shape[0], k.shape[0]
+    q, k, v = q.double(), k.double(), v.double()
+    s = scale * torch.einsum("ngd,ld->ngl", q, k)
+    if causal:
+        seen = torch.arange(L, device="cuda") < L - n + 1 + torch.arange(n, device="cuda")[:, None]
+        s = torch.where(seen[:, None], s, -math.inf)
+    p = torch.softmax(s, -1)
+    top = abs(scale) * torch.einsum("ngd,ld->ngl", q.abs(), k.abs()).amax(-1)
+    return p @ v, torch.logsumexp(s, -1), p.sum((0, 1)), p @ v.abs(), top
+
+
+# queries times query heads per key/value head: both forms of the decoding
+# kernel, one row tile, two
+ROWS = [(1, 2), (3, 5), (20, 3), (150, 1)]
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_zero_keys_and_values_over_a_long_sequence(n, group, causal):
+    # equal scores: lse is the logarithm of the tokens seen and each gets the
+    # same weight, whatever scale a block of zeros has
+    from vicinity_b200 import KVCache
+
+    L, d = 200_000, 32
+    cache = KVCache(1, L, 1, d, block_tokens=128)
+    zero = torch.zeros(L, 1, d, dtype=torch.bfloat16, device="cuda")
+    cache.append(zero, zero, [L])
+    q = torch.randn(n, group, d, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(torch.bfloat16)
+    out, lse = torch.full_like(q, 7.0), torch.empty(n, group, device="cuda")
+    cache.attend(q, [n], out, lse=lse, causal=causal, accumulate=True)
+    w = torch.as_tensor(cache.weights, device="cuda")[0, 0, :L].double()
+    seen = (L - n + 1 + torch.arange(n, device="cuda") if causal else torch.full((n,), L, device="cuda")).double()
+    assert (out == 0).all()
+    assert ((lse.double() - seen.log()[:, None]).abs() <= 16 * U * (1 + math.log(L))).all()
+    each = (torch.arange(L, device="cuda") < seen[:, None]).double() / seen[:, None]
+    want = group * each.sum(0)
+    assert ((w - want).abs() <= (32 * U * (1 + math.log(L)) + 4 * U) * want).all()
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("zeros_first", [True, False])
+def test_attend_a_long_run_of_zeros_beside_values(n, group, zeros_first):
+    from vicinity_b200 import KVCache
+
+    Z, V, d = 70_000, 700, 64
+    g = torch.Generator(device="cuda").manual_seed(6)
+    cache = KVCache(1, Z + V, 1, d, block_tokens=16)
+    zero = torch.zeros(Z, 1, d, dtype=torch.bfloat16, device="cuda")
+    k, v = (torch.randn(V, 1, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    for a, b in [(zero, zero), (k, v)] if zeros_first else [(k, v), (zero, zero)]:
+        cache.append(a, b, [a.shape[0]])
+    q = (2 * torch.randn(n, group, d, generator=g, device="cuda")).to(torch.bfloat16)
+    out, lse = torch.full_like(q, 7.0), torch.empty(n, group, device="cuda")
+    cache.attend(q, [n], out, lse=lse, accumulate=True)
+    w = torch.as_tensor(cache.weights, device="cuda")[0, 0, :Z + V].double()
+    kk, vv = (torch.empty(Z + V, 1, d, device="cuda") for _ in range(2))
+    cache.read([0], [Z + V], kk, vv)
+    want, want_lse, want_w, size, top = _attention64(q, kk[:, 0], vv[:, 0], True, d ** -0.5)
+    e = (d + 16) * U * top
+    assert ((lse.double() - want_lse).abs() <= e + 16 * U * (1 + want_lse.abs())).all()
+    soft = 2 * e + 32 * U * (1 + want_lse.abs())
+    tol = 1.01 * ROUND["bf16"] * want.abs() + (2.0 ** -11 + soft)[..., None] * size
+    tol += (Z + V) * 2.0 ** -36 * float(vv.abs().max())
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((w - want_w).abs() <= (soft.max() + 4 * U) * want_w + 1e-12).all()
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("length", [200, 3000])
+def test_attend_values_of_all_magnitudes(length, n, group):
+    # runs of tokens whose values are 0, or up to 2^120 apart, with keys of one
+    # magnitude: the denominators do not depend on the values
+    g = np.random.default_rng(length + n)
+    for sizes in ([0.0, 2.0 ** 60], [2.0 ** 60, 0.0], [2.0 ** 100, 2.0 ** -90, 1.0, 0.0],
+                  [0.0, 2.0 ** 20, 0.0, 2.0 ** 110, 2.0 ** -110], [2.0 ** -95], [2.0 ** 118, 0.0, 2.0 ** -60]):
+        m = Mirror(1, length, 1, 64, 16)
+        ends = [length * (i + 1) // len(sizes) for i in range(len(sizes))]
+        for a, b, size in zip([0] + ends, ends, sizes):
+            m.append([b - a], _rand(g, b - a, 1, 64, dtype="bf16"), _rand(g, b - a, 1, 64, dtype="bf16", scale=size))
+        q = _rand(g, n, group, 64, dtype="bf16", scale=2.0)
+        m.attend([n], q, "bf16", accumulate=True)
+        m.attend([n], q, "bf16", causal=False)
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+def test_attend_a_long_run_of_zeros_within_a_chunk(n, group):
+    # as many heads as CTAs run at once, so that none is cut: a CTA's own sums
+    # pass 32,768 tokens of zeros before the values come
+    from vicinity_b200 import KVCache
+
+    Z, V, d, heads = 39_000, 300, 32, 296
+    g = torch.Generator(device="cuda").manual_seed(7)
+    cache = KVCache(1, Z + V, heads, d, block_tokens=64)
+    zero = torch.zeros(1, 1, d, dtype=torch.bfloat16, device="cuda").expand(Z, heads, d)
+    cache.append(zero, zero, [Z])
+    k, v = (torch.randn(V, heads, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    cache.append(k, v, [V])
+    q = torch.randn(n, heads * group, d, generator=g, device="cuda").to(torch.bfloat16)
+    out, lse = torch.full_like(q, 7.0), torch.empty(n, heads * group, device="cuda")
+    cache.attend(q, [n], out, lse=lse)
+    kk, vv = (torch.empty(Z + V, heads, d, device="cuda") for _ in range(2))
+    cache.read([0], [Z + V], kk, vv)
+    for h in (0, 100, 295):
+        at = slice(h * group, (h + 1) * group)
+        want, want_lse, _, size, top = _attention64(q[:, at], kk[:, h], vv[:, h], True, d ** -0.5)
+        e = (d + 16) * U * top
+        assert ((lse[:, at].double() - want_lse).abs() <= e + 16 * U * (1 + want_lse.abs())).all()
+        tol = 1.01 * ROUND["bf16"] * want.abs() + (2.0 ** -11 + 2 * e + 32 * U * (1 + want_lse.abs()))[..., None] * size
+        tol += (Z + V) * 2.0 ** -36 * float(vv.abs().max())
+        assert ((out[:, at].double() - want).abs() <= tol).all()

@@ -1,11 +1,15 @@
 // Attention over a key/value cache held in 8 bits.
 //
-// Scores are x = log2(e) scale q.k and the reference of a row's exponentials is
+// Scores are x = log2(e) scale q.k and the reference mu of a row's exponentials is
 // the running maximum of x + log2(value scale): with P = 2^(x + log2 vs - mu) the
 // sum of P times the value codes needs no other factor, and the denominator is
-// the sum of P / vs (powers of two: exact).  Codes are exact in binary16, and a
-// query row is scaled by a power of two into its range, so both products run on
-// the tensor cores in binary16 with f32 sums; only P is rounded, to 11 bits.
+// the sum of P / vs (powers of two: exact), held relative to the running maximum
+// nu of x alone.  Codes are exact in binary16, and a query row is scaled by a
+// power of two into its range, so both products run on the tensor cores in
+// binary16 with f32 sums; only P is rounded, to 11 bits: in more the second
+// product would take two binary16 parts, twice the products of a kernel that
+// is bound by them, for an error that an output in 16 bits does not show (f16
+// outputs differ from the exact ones by 2.1e-4 of their norm, 2.0e-4 without).
 #include "chain.cuh"
 #include "common.cuh"
 #include "elements.cuh"
@@ -69,12 +73,6 @@ __device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint3
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t *>(st + swz<D>(tok, at + 4 * i));
   }
-}
-
-// Factor of a partial sum with reference ml.x in one with reference m >= ml.x;
-// 0 for one that has seen nothing, 1 where its sums are NaN without a reference.
-__device__ __forceinline__ float part_weight(float2 ml, float m) {
-  return ml.x == -VG_INF ? (ml.y == ml.y ? 0.0f : 1.0f) : exp2_approx(ml.x - m);
 }
 
 // transposes an 8 x 8 matrix of binary16 (lane 4 r + c holds columns 2 c, 2 c + 1 of row r)
@@ -186,10 +184,10 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
   for (int g = 0; g < kCols; ++g)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
-  float mu[2 * kCols], l[2 * kCols];
+  float mu[2 * kCols], nu[2 * kCols], l[2 * kCols];
 #pragma unroll
   for (int h = 0; h < 2 * kCols; ++h) {
-    mu[h] = -VG_INF;
+    mu[h] = nu[h] = kUnseen;
     l[h] = 0.0f;
   }
 
@@ -239,18 +237,18 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
     }
     bool raise = false;
 #pragma unroll
-    for (int h = 0; h < 2 * kCols; ++h)
-      raise |= fmaf(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h], lv) > mu[h] + kLazy;
+    for (int h = 0; h < 2 * kCols; ++h) {
+      const float x = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) * f[h];
+      raise |= x + lv > mu[h] + kLazy || x > nu[h] + kLazy;
+    }
     if (__any_sync(VG_FULL_MASK, raise)) {
 #pragma unroll
       for (int h = 0; h < 2 * kCols; ++h) {
-        float m = fmaf(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h], lv);
+        float x = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) * f[h];
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
-        m = fmaxf(m, mu[h]);
-        const float c = m == -VG_INF ? 1.0f : exp2_approx(mu[h] - m);
-        mu[h] = m;
-        l[h] *= c;
+        for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(VG_FULL_MASK, x, w));
+        const float c = raise_reference(mu[h], x + lv);
+        l[h] *= raise_reference(nu[h], x);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           o[h >> 1][i][h & 1] *= c;
@@ -264,10 +262,11 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
       float p[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float ref = lv + kPShift - (mu[2 * g + h] == -VG_INF ? 0.0f : mu[2 * g + h]);
+        const PowerRefs refs(mu[2 * g + h], nu[2 * g + h]);
+        const float ref = refs.exponent(lv);
         p[h] = exp2_approx(fmaf(s[g][h], f[2 * g + h], ref));
         p[2 + h] = exp2_approx(fmaf(s[g][2 + h], f[2 * g + h], ref));
-        l[2 * g + h] = fmaf(p[h] + p[2 + h], per_v, l[2 * g + h]);
+        l[2 * g + h] = fmaf(p[h] + p[2 + h], refs.share(per_v), l[2 * g + h]);
         if (scale.y != scale.y) {  // the values read as NaN: so does every row that sees one of them
           if (t + n < lim[2 * g + h]) p[h] = scale.y;
           if (t + n + 8 < lim[2 * g + h]) p[2 + h] = scale.y;
@@ -307,7 +306,7 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
   // [warp][row][D], rows padded so that a lane's pairs of dimensions spread over the banks
   constexpr int kPad = D + 2;
   float *so = reinterpret_cast<float *>(dec_smem);
-  float2 *sml = reinterpret_cast<float2 *>(so + kDecWarps * kRowsMax * kPad);  // [warp][row]
+  float4 *sml = reinterpret_cast<float4 *>(so + kDecWarps * kRowsMax * kPad);  // [warp][row]
 #pragma unroll
   for (int h = 0; h < 2 * kCols; ++h) {
     const uint32_t row = 8 * (h >> 1) + 2 * j + (h & 1);
@@ -315,32 +314,35 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
       *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[h >> 1][i][h & 1], o[h >> 1][i][2 + (h & 1)]);
-    if (n == 0) sml[warp * kRowsMax + row] = make_float2(mu[h], l[h]);
+    if (n == 0) sml[warp * kRowsMax + row] = make_float4(mu[h], nu[h], l[h], 0.0f);
   }
   __syncthreads();
   const bool whole = ps.len <= a.chunk;
   for (uint32_t e = threadIdx.x; e < rows * (D / 8); e += kDecWarps * 32) {
     const uint32_t row = e / (D / 8), c = e % (D / 8) * 8;
-    float m = -VG_INF, sum = 0.0f, y[8] = {};
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, sml[w * kRowsMax + row].x);
+    float m = kUnseen, mn = kUnseen, sum = 0.0f, y[8] = {};
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
-      const float2 ml = sml[w * kRowsMax + row];
-      const float f = part_weight(ml, m);
-      sum += f * ml.y;
+      m = fmaxf(m, sml[w * kRowsMax + row].x);
+      mn = fmaxf(mn, sml[w * kRowsMax + row].y);
+    }
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float4 ml = sml[w * kRowsMax + row];
+      const float f = exp2_approx(ml.x - m);
+      sum += exp2_approx(ml.y - mn) * ml.z;
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kRowsMax + row) * kPad + c + i];
     }
     if (whole) {
       const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
+      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, mn, sum, y);
     } else {
       const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kDecodeRows + row;
       float *dst = a.part_o + at * D + c;
       *reinterpret_cast<float4 *>(dst) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4 *>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
-      if (c == 0) a.part_ml[at] = make_float2(m, sum);
+      if (c == 0) a.part_ml[at] = make_float4(m, mn, sum, 0.0f);
     }
   }
 }
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
                                                                    const __grid_constant__ P plan,
                                                                    const uint32_t part_rows, const bool ovec) {
   __shared__ float weight[kMaxSplits];
-  __shared__ float red[kJoinThreads / 32];
+  __shared__ float2 red[kJoinThreads / 32];
   __shared__ float acc[kJoinThreads * 8];
   chain_release();
   chain_wait();
@@ -371,27 +373,36 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   const size_t first =
       ((static_cast<size_t>(ps.unit0) + block * ns) * a.kv.heads + head) * part_rows + row % part_rows;
   const int warp = threadIdx.x >> 5;
-  float m = -VG_INF;
-  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) m = fmaxf(m, a.part_ml[first + i * step].x);
+  float m = kUnseen, mn = kUnseen;
+  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
+    const float4 ml = a.part_ml[first + i * step];
+    m = fmaxf(m, ml.x);
+    mn = fmaxf(mn, ml.y);
+  }
 #pragma unroll
-  for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
-  if (lane_id() == 0) red[warp] = m;
+  for (int w = 16; w > 0; w >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
+    mn = fmaxf(mn, __shfl_xor_sync(VG_FULL_MASK, mn, w));
+  }
+  if (lane_id() == 0) red[warp] = make_float2(m, mn);
   __syncthreads();
-  for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, red[w]);
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    m = fmaxf(m, red[w].x);
+    mn = fmaxf(mn, red[w].y);
+  }
   __syncthreads();
   float sum = 0.0f;
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
-    const float2 ml = a.part_ml[first + i * step];
-    const float f = part_weight(ml, m);
-    weight[i] = f;
-    sum += f * ml.y;
+    const float4 ml = a.part_ml[first + i * step];
+    weight[i] = exp2_approx(ml.x - m);
+    sum += exp2_approx(ml.y - mn) * ml.z;
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(VG_FULL_MASK, sum, w);
-  if (lane_id() == 0) red[warp] = sum;
+  if (lane_id() == 0) red[warp].x = sum;
   __syncthreads();
   sum = 0.0f;
-  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[w];
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[w].x;
   const uint32_t per = D / 8, groups = kJoinThreads / per, g = threadIdx.x / per, c = threadIdx.x % per * 8;
   float y[8] = {};
   if (g < groups) {
@@ -412,7 +423,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += acc[(w * per + threadIdx.x) * 8 + i];
     const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, sum, y);
+    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, mn, sum, y);
   }
 }
 
@@ -449,7 +460,7 @@ template <int D, int kCols, bool kScores>
 cudaError_t decode(const AttendArgs &a, const Plan &plan, cudaStream_t s) {
   constexpr int warps = Dec<kCols>::warps;
   constexpr size_t ring = warps * Dec<kCols>::ring * (2 * kStep * D + 16);
-  constexpr size_t join = warps * 8 * kCols * ((D + 2) * sizeof(float) + sizeof(float2));
+  constexpr size_t join = warps * 8 * kCols * ((D + 2) * sizeof(float) + sizeof(float4));
   constexpr size_t smem = std::max(ring, join);
   return with_plan(plan, [&](const auto &p) {
     static std::atomic<uint64_t> allowed{0};

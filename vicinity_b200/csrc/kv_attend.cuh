@@ -16,10 +16,17 @@ namespace vg {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 #define VG_INF __int_as_float(0x7f800000)
 
-// Probabilities are held as 2^(x - mu + kPShift) in binary16: mu may lag the
-// running maximum by kLazy (fewer rescalings), so they are at most 2^15 and
-// vanish below 2^-38 of the largest.
-constexpr float kPShift = 13.0f, kLazy = 2.0f;
+// A row has two references, whole numbers that may lag by kLazy (fewer
+// rescalings): mu of x + log2(value scale) and nu of the scores x themselves.
+// Probabilities are P = 2^(x + log2 vs - mu + kPShift) in binary16: at most
+// 2^15, and they vanish below 2^-37 of the largest.  The denominator is the
+// sum of 2^(x - nu) = P 2^(mu - nu - kPShift) / vs in f32, which no value scale
+// can overflow.  Where vs is so small beside the row's others that P would
+// vanish in f32 too, its exponent is held at x - nu - kFar: 0 in binary16 all the
+// same, but still there for the denominator.  Both start at kUnseen, the lowest
+// number: below every score but -inf, and differences stay defined.
+constexpr float kUnseen = -3.402823466e38f;
+constexpr float kPShift = 13.0f, kLazy = 2.0f, kFar = 32.0f, kFarFactor = 4294967296.0f;
 
 // 2 ulp; 0 below 2^-126 (the form that keeps subnormal results is four instructions)
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -82,6 +89,27 @@ __device__ __forceinline__ float inverse_scale(float s) {
   return s == s ? __uint_as_float(0x7f000000u - __float_as_uint(s)) : 1.0f;
 }
 
+// What P of a block of value scale 2^lv takes: its exponents are x plus the
+// first, its share of the denominator is P times the second.
+struct PowerRefs {
+  float mu, nu, ratio;
+  __device__ __forceinline__ PowerRefs(float m, float n) {
+    mu = m;
+    nu = n;
+    ratio = exp2_approx(m - n - kPShift);
+  }
+  __device__ __forceinline__ float exponent(float lv) const { return fmaxf(lv + (kPShift - mu), -kFar - nu); }
+  __device__ __forceinline__ float share(float per_v) const { return fminf(per_v * ratio, kFarFactor); }
+};
+
+// Takes a reference up to `top` where that is larger; returns what sums that refer to it shrink by.
+__device__ __forceinline__ float raise_reference(float &ref, float top) {
+  const float to = fmaxf(ref, ceilf(top));
+  const float c = exp2_approx(ref - to);
+  ref = to;
+  return c;
+}
+
 // Cached tokens that query qi of a sequence sees.
 __device__ __forceinline__ uint32_t tokens_seen(const PlanSeq &ps, uint32_t qi, bool causal) {
   const uint32_t behind = ps.count - 1 - qi;
@@ -101,14 +129,15 @@ cudaError_t allow_smem(Kernel *kern, size_t bytes, std::atomic<uint64_t> &done) 
 
 // The result of one row from its sums: 8 dimensions from c on, and the lse.
 __device__ __forceinline__ void finish_row(const AttendArgs &a, size_t token, uint32_t hq, uint32_t c, bool ovec,
-                                           float mu, float sum, float (&y)[8]) {
+                                           float mu, float nu, float sum, float (&y)[8]) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no token seen: 0
+  const float ratio = sum == 0.0f ? 0.0f : exp2_approx(mu - nu - kPShift);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] *= inv;
+  for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * ratio;
   store8_16(a.out.p, static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head + c,
             a.dtype == VG_F16, ovec, y);
   if (c == 0) {
-    const float lse2 = sum == 0.0f ? -VG_INF : mu - kPShift + log2f(sum);
+    const float lse2 = sum == 0.0f ? -VG_INF : nu + log2f(sum);
     if (a.lse) a.lse[token * a.q_heads + hq] = lse2 * kLn2;
     if (a.lse2) a.lse2[token * a.q_heads + hq] = lse2;
   }

@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     const float f_row = my_tiles == 0 ? 0.0f : a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t pS = tmem + x * kTok + lane_base, pO = tmem + (kTiles + x) * kTok + lane_base;
-    float mu = -VG_INF, l = 0.0f;
+    float mu = kUnseen, nu = kUnseen, l = 0.0f;
     float poison = 0.0f;  // whether the row has seen values (1) or keys (2) that read as NaN
     // products of 32 tokens from `from` on that the row does not see
     auto hide = [&](uint32_t *v, uint32_t from) {
@@ -465,26 +465,25 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
       for (int k = 0; k < 32; ++k)
         if (from + k >= lim) v[k] = 0xff800000u;
     };
-    // largest score plus log2 of the value scale of 32 products; the factors
-    // are above 0, so that -inf stays -inf
-    auto largest = [&](const uint32_t *v, const float4 *tab, float m) {
+    // largest score (n) and score plus log2 of the value scale (m) of 32
+    // products; the factors are above 0, so that -inf stays -inf
+    auto largest = [&](const uint32_t *v, const float4 *tab, float &m, float &n) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float4 e = tab[g];
         float top = -VG_INF;
 #pragma unroll
         for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(v[16 * g + k]));
-        m = fmaxf(m, fmaf(top, fmaxf(f_row * e.x, 1e-37f), e.y));
+        const float x = top * fmaxf(f_row * e.x, 1e-37f);
+        n = fmaxf(n, x);
+        m = fmaxf(m, x + e.y);
       }
-      return m;
     };
-    // takes the reference up to m where it lags too far: the sums so far shrink
-    auto raise = [&](float m, bool sums) {
-      if (!__any_sync(VG_FULL_MASK, m > mu + kLazy)) return;
-      m = fmaxf(m, mu);
-      const float c = m == -VG_INF ? 1.0f : exp2_approx(mu - m);
-      mu = m;
-      l *= c;
+    // takes the references up to m and n where they lag too far: the sums so far shrink
+    auto raise = [&](float m, float n, bool sums) {
+      if (!__any_sync(VG_FULL_MASK, m > mu + kLazy || n > nu + kLazy)) return;
+      l *= raise_reference(nu, n);
+      const float c = raise_reference(mu, m);
       if (!sums) return;
 #pragma unroll 1
       for (int b = 0; b < D; b += 16) {
@@ -499,11 +498,11 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     };
     // P of 32 tokens from `from` on, into the denominator and binary16 pairs
     auto powers = [&](const uint32_t *v, const float4 *tab, uint32_t from, uint32_t (&p)[16]) {
-      const float base = kPShift - (mu == -VG_INF ? 0.0f : mu);
+      const PowerRefs refs(mu, nu);
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float4 e = tab[g];
-        const float f = fmaxf(f_row * e.x, 1e-37f), ref = base + e.y;
+        const float f = fmaxf(f_row * e.x, 1e-37f), ref = refs.exponent(e.y);
         const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
         f32x2 sum2[2] = {0, 0};
 #pragma unroll
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           p[8 * g + k] = pack_half2(y.x, y.y);
         }
         const float2 sum = f2_unpack(f2_add(sum2[0], sum2[1]));
-        l = fmaf(sum.x + sum.y, e.z, l);
+        l = fmaf(sum.x + sum.y, refs.share(e.z), l);
         if (e.w != 0.0f && from + 16 * g < lim) poison = fmaxf(poison, e.w);
       }
     };
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
       }
       tc_fence_after();
       const bool edge = t + kTok > warp_lim;
-      float m = -VG_INF;
+      float m = -VG_INF, n = -VG_INF;
       if constexpr (kTiles == 2) {
         uint32_t v[kTok];
 #pragma unroll
@@ -548,8 +547,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           for (int c = 0; c < 4; ++c) hide(v + c * 32, t + c * 32);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) m = largest(v + c * 32, tab + 2 * c, m);
-        raise(m, i != 0);
+        for (int c = 0; c < 4; ++c) largest(v + c * 32, tab + 2 * c, m, n);
+        raise(m, n, i != 0);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t p[16];
@@ -564,9 +563,9 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           tmem_ld32_nowait(pS + c * 32, v);
           tmem_wait_ld32(v);
           if (edge) hide(v, t + c * 32);
-          m = largest(v, tab + 2 * c, m);
+          largest(v, tab + 2 * c, m, n);
         }
-        raise(m, i != 0);
+        raise(m, n, i != 0);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t v[32], p[16];
@@ -604,7 +603,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           for (int d = 0; d < 8; ++d) y[d] = poison != 0.0f ? nan : __uint_as_float(v[8 * (d & 3) + 2 * k + (d >> 2)]);
           const uint32_t c = 4 * b + 8 * k;
           if (whole) {
-            finish_row(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, l, y);
+            finish_row(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, nu, l,
+                       y);
           } else {
             float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D + c);
             dst[0] = make_float4(y[0], y[1], y[2], y[3]);
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           }
         }
       }
-      if (!whole && valid) a.part_ml[at] = make_float2(mu, l);
+      if (!whole && valid) a.part_ml[at] = make_float4(mu, nu, l, 0.0f);
     } else {
       give_up(3);
     }

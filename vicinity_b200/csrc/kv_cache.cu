@@ -199,9 +199,9 @@ int weigh_tiles(AttendArgs &a, Plan &plan, cudaStream_t s) {
 
 int reserve_parts(vg_kv_cache *kv, AttendArgs &a, const Plan &plan, uint32_t part_rows) {
   const size_t rows = static_cast<size_t>(plan.units) * kv->view.heads * part_rows;
-  VG_CU(kv->ws_part.reserve(rows * (kv->view.dim * sizeof(float) + sizeof(float2))));
+  VG_CU(kv->ws_part.reserve(rows * (kv->view.dim * sizeof(float) + sizeof(float4))));
   a.part_o = kv->ws_part.as<float>();
-  a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * kv->view.dim);
+  a.part_ml = reinterpret_cast<float4 *>(a.part_o + rows * kv->view.dim);
   return VG_OK;
 }
 
