@@ -829,3 +829,15 @@ def test_attend_a_long_run_of_zeros_within_a_chunk(n, group):
         tol = 1.01 * ROUND["bf16"] * want.abs() + (2.0 ** -11 + 2 * e + 32 * U * (1 + want_lse.abs()))[..., None] * size
         tol += (Z + V) * 2.0 ** -36 * float(vv.abs().max())
         assert ((out[:, at].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+def test_attend_largest_keys_smallest_queries(n, group):
+    # keys near the largest scale and queries near the smallest numbers: their
+    # scores are ordinary, in the attention and in the weights
+    g = np.random.default_rng(30 + n)
+    m = Mirror(1, 400, 2, 64, 32)
+    for size in (124, 100, 124):
+        m.append([130], _rand(g, 130, 2, 64, dtype="bf16", scale=2.0 ** size), _rand(g, 130, 2, 64, dtype="bf16"))
+    q = _rand(g, n, 2 * group, 64, dtype="bf16", scale=2.0 ** -122)
+    m.attend([n], q, "bf16", accumulate=True)

@@ -794,8 +794,10 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const float4 w = reinterpret_cast<const float4 *>(my_f)[c * 16 + k];
-          const f32x2 x = f2_mul(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), ks2);
-          float2 p = f2_unpack(f2_fma(x, f2_pack(w.x, w.y), f2_pack(w.z, w.w)));
+          // the factors first: a product times the largest scales passes f32
+          const f32x2 f = f2_mul(f2_pack(w.x, w.y), ks2);
+          float2 p = f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), f,
+                                      f2_pack(w.z, w.w)));
           p.x = exp2_approx(p.x);
           p.y = exp2_approx(p.y);
           if (edge) {
