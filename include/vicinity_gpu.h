@@ -490,7 +490,8 @@ int vg_kv_read(vg_kv_cache *kv, const uint32_t *starts, const uint32_t *counts, 
 /* Set or copy out a whole sequence: codes int8 [num_kv_heads][length][head_dim],
  * scales f32 [num_kv_heads][ceil(length / block_tokens)], weights (nullable)
  * f32 [num_kv_heads][length]; host or device memory, contiguous.  `length`
- * of an export is the sequence's.  Scales are powers of two (or NaN).  These
+ * of an export is the sequence's.  Scales are powers of two in [2^-100, 2^120]
+ * or NaN: VG_ERR_INVALID_PARAMETER, with nothing loaded, for any other.  These
  * return when the copy is done. */
 int vg_kv_load(vg_kv_cache *kv, size_t seq, size_t length, const int8_t *k_codes, const float *k_scales,
                const int8_t *v_codes, const float *v_scales, const float *weights, void *stream);

@@ -841,3 +841,32 @@ def test_attend_largest_keys_smallest_queries(n, group):
         m.append([130], _rand(g, 130, 2, 64, dtype="bf16", scale=2.0 ** size), _rand(g, 130, 2, 64, dtype="bf16"))
     q = _rand(g, n, 2 * group, 64, dtype="bf16", scale=2.0 ** -122)
     m.attend([n], q, "bf16", accumulate=True)
+
+
+@pytest.mark.parametrize("where", ["host", "device"])
+def test_load_refuses_scales_that_are_none(where):
+    # scales are powers of two in [2^-100, 2^120], or NaN
+    from vicinity_b200 import KVCache
+
+    g = np.random.default_rng(31)
+    c = KVCache(2, 100, 2, 32, block_tokens=16)
+
+    def load(ks, vs):
+        a = [g.integers(-127, 128, (2, 70, 32)).astype(np.int8), ks, g.integers(-127, 128, (2, 70, 32)).astype(np.int8), vs]
+        c.load(0, *(a if where == "host" else [torch.from_numpy(x).cuda() for x in a]))
+
+    good = np.float32(2.0) ** g.integers(-100, 121, (2, 5)).astype(np.float32)
+    good[0, 0], good[0, 1], good[1, 4] = 2.0 ** -100, 2.0 ** 120, np.nan
+    load(good, good[::-1].copy())
+    before = c.export(0)
+    for bad in (0.0, -0.0, -1.0, 3.0, 1.0 / 127, 2.0 ** -101, 2.0 ** 121, 2.0 ** -130, math.inf, -math.inf,
+                float(np.nextafter(np.float32(1), np.float32(2)))):
+        for at in ((0, 0), (1, 4)):
+            scales = good.copy()
+            scales[at] = bad
+            for pair in ((scales, good), (good, scales)):
+                with pytest.raises(ValueError, match="scales"):
+                    load(*pair)
+    assert c.lengths.tolist() == [70, 0]
+    for a, b in zip(before, c.export(0)):
+        assert np.array_equal(a, b, equal_nan=a.dtype == np.float32)

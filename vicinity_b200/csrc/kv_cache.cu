@@ -529,6 +529,26 @@ int vg_kv_read(vg_kv_cache *kv, const uint32_t *starts, const uint32_t *counts, 
 
 namespace {
 
+// Scales of a host or device array as the kernels take them: their exponents
+// are used as they are.
+int check_scales(const float *scales, size_t n, const char *name, cudaStream_t s) {
+  std::vector<uint32_t> bits(std::min<size_t>(n, size_t(1) << 18));
+  for (size_t at = 0; at < n; at += bits.size()) {
+    const size_t m = std::min(n - at, bits.size());
+    VG_CU(cudaMemcpyAsync(bits.data(), scales + at, m * sizeof(float), cudaMemcpyDefault, s));
+    VG_CU(cudaStreamSynchronize(s));
+    for (size_t i = 0; i < m; ++i) {
+      const uint32_t b = bits[i], e = b >> 23;  // the sign would be the exponent's ninth bit
+      const bool nan = (b & 0x7fffffffu) > 0x7f800000u;
+      if (!nan && ((b & 0x7fffffu) || e < 127 + kMinScaleExp || e > 127 + kMaxScaleExp))
+        return fail(VG_ERR_INVALID_PARAMETER,
+                    std::string(name) + " must be scales: powers of two in [2^-100, 2^120], or NaN (entry " +
+                        std::to_string(at + i) + ")");
+    }
+  }
+  return VG_OK;
+}
+
 // One row of a host or device array to or from the cache.
 int copy_row(void *dst, const void *src, size_t bytes, cudaStream_t s) {
   VG_CU(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDefault, s));
@@ -555,6 +575,7 @@ int vg_kv_load(vg_kv_cache *kv, size_t seq, size_t length, const int8_t *k_codes
     const int8_t *codes[2] = {k_codes, v_codes};
     const float *scales[2] = {k_scales, v_scales};
     const size_t nb = w.stride >> w.block_shift, used = (length + w.block - 1) >> w.block_shift;
+    for (int i = 0; i < 2; ++i) VG_TRY(check_scales(scales[i], w.heads * used, i ? "v_scales" : "k_scales", s));
     for (size_t h = 0; length && h < w.heads; ++h) {
       const size_t r = seq * w.heads + h;
       for (int i = 0; i < 2; ++i) {

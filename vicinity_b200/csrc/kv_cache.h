@@ -19,6 +19,7 @@
 namespace vg {
 
 constexpr uint32_t kKvPad = 128;
+constexpr int kMinScaleExp = -100, kMaxScaleExp = 120;  // scales are 2^e, or NaN
 // Sequences per launch: the plan travels as a kernel argument, 8 KB or, up to
 // kSmallPlan of them, half a KB (which takes 1.2 us less to launch).
 constexpr int kPlanSeqs = 256, kSmallPlan = 16;

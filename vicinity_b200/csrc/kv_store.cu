@@ -18,16 +18,14 @@ namespace vg {
 
 namespace {
 
-constexpr int kMinExp = -100, kMaxExp = 120;
-
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-// The smallest 2^e, e in [kMinExp, kMaxExp], with 127 * 2^e >= |x|, from the
+// The smallest 2^e, e in [kMinScaleExp, kMaxScaleExp], with 127 * 2^e >= |x|, from the
 // bits of |x|: |x| = m 2^(x-126), m in [0.5, 1); 127/128 has mantissa 0x7e0000.
 __device__ __forceinline__ float scale_of(uint32_t absbits) {
   if (absbits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);  // not finite: the block reads as NaN
   const int e = static_cast<int>(absbits >> 23) - 126 - 7 + ((absbits & 0x7fffffu) > 0x7e0000u ? 1 : 0);
-  return pow2(min(max(e, kMinExp), kMaxExp));
+  return pow2(min(max(e, kMinScaleExp), kMaxScaleExp));
 }
 
 // 1 / s of a scale (a power of two: exact; NaN stays NaN)
@@ -131,7 +129,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_c
     const uint32_t e = threadIdx.x + i * kStoreThreads, t = item_token(e, per);
     if (e < total) x[i].load(src + static_cast<int64_t>(t) * in.token + (e - t * per) * 16, vec);
   }
-  const float s_old = lo > blk0 ? *scale : pow2(kMinExp);
+  const float s_old = lo > blk0 ? *scale : pow2(kMinScaleExp);
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kItems; ++i)
@@ -147,7 +145,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv_append_kernel(const __grid_c
   const float s_top = scale_of(top);
   const float s_new = s_old != s_old || s_top != s_top ? s_old + s_top : fmaxf(s_old, s_top);
   const float inv = inverse(s_new);
-  const bool exotic = !(s_new < pow2(kMaxExp));
+  const bool exotic = !(s_new < pow2(kMaxScaleExp));
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     const uint32_t e = threadIdx.x + i * kStoreThreads;
