@@ -870,3 +870,31 @@ def test_load_refuses_scales_that_are_none(where):
     assert c.lengths.tolist() == [70, 0]
     for a, b in zip(before, c.export(0)):
         assert np.array_equal(a, b, equal_nan=a.dtype == np.float32)
+
+
+def test_misaligned_addresses_are_refused():
+    # through the C entry points: an array must lie on a multiple of its element
+    import ctypes as C
+
+    from vicinity_b200 import KVCache, Rotary, _lib
+
+    lib, bad = _lib.load(), _lib.VG_ERR_INVALID_PARAMETER
+    c = KVCache(2, 64, 1, 32, block_tokens=16)
+    k = torch.zeros(5, 1, 32, dtype=torch.bfloat16, device="cuda")
+    c.append(k, k, [5, 0])
+    room = torch.zeros(64, dtype=torch.int64, device="cuda")
+    counts, src, dst = ((C.c_uint32 * n)(*x) for n, x in ((2, (5, 0)), (1, (0,)), (1, (1,))))
+    at = lambda x: (C.c_int64 * 4)(x, 1, 32, 32)  # noqa: E731
+    q, out = at(k.data_ptr()), at(k.clone().data_ptr())
+    for off in (1, 2, 3):
+        assert lib.vg_kv_attend(c._h, counts, _lib.BF16, q, out, room.data_ptr() + off, 1.0, 0, None) == bad
+        assert "lse" in _lib.last_error()
+        assert lib.vg_kv_evict(c._h, 1, src, dst, 4, 1, room.data_ptr() + off, None) == bad
+        assert "kept" in _lib.last_error()
+    r = Rotary(32)
+    for off in (1, 2, 4, 7):
+        assert lib.vg_rotary_apply(r._h, _lib.BF16, 32, room.data_ptr() + off, 5, q, out, None, None, 0, 0, None) == bad
+        assert "positions" in _lib.last_error()
+    odd = at(k.data_ptr() + 1)
+    assert lib.vg_kv_append(c._h, counts, _lib.BF16, odd, q, None) == bad
+    assert c.lengths.tolist() == [5, 0]

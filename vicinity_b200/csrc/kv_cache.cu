@@ -411,7 +411,7 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     if (out->num_heads != q->num_heads) return fail(VG_ERR_DIMENSION_MISMATCH, "out must have the heads of q");
     if (rows * (q->num_heads / kv->params.num_kv_heads) > 0x7fffffffull)
       return fail(VG_ERR_INVALID_PARAMETER, "too many queries in one call");
-    if (lse) VG_TRY(check_device_memory(lse, kv->device, "lse"));
+    if (lse) VG_TRY(check_device_memory(lse, sizeof(float), kv->device, "lse"));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Work work(kv, stream);
     VG_TRY(work.begin());
@@ -461,7 +461,7 @@ int vg_kv_evict(vg_kv_cache *kv, size_t n, const uint32_t *src, const uint32_t *
       }
     if (n == 0) return VG_OK;
     DeviceGuard g(kv->device);
-    if (kept) VG_TRY(check_device_memory(kept, kv->device, "kept"));
+    if (kept) VG_TRY(check_device_memory(kept, sizeof(int32_t), kv->device, "kept"));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Work work(kv, stream);
     VG_TRY(work.begin());

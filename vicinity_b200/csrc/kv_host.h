@@ -42,7 +42,10 @@ inline int check_dtype(int dtype) {
   return VG_OK;
 }
 
-inline int check_device_memory(const void *p, int device, const char *name) {
+// An array of elements of `size` bytes.
+inline int check_device_memory(const void *p, size_t size, int device, const char *name) {
+  if (reinterpret_cast<uintptr_t>(p) % size)
+    return fail(VG_ERR_INVALID_PARAMETER, std::string(name) + " is not aligned to its elements");
   cudaPointerAttributes a{};
   const bool known = p && cudaPointerGetAttributes(&a, p) == cudaSuccess;
   if (!known) cudaGetLastError();
@@ -61,8 +64,6 @@ inline int check_heads(const vg_heads *t, const char *name, size_t tokens, size_
     return fail(VG_ERR_INVALID_PARAMETER, std::string(name) + " must have 1 to 65535 heads");
   if (t->token_stride < 0 || t->head_stride < 0)
     return fail(VG_ERR_INVALID_PARAMETER, std::string(name) + " has a negative stride");
-  if (reinterpret_cast<uintptr_t>(t->data) % element_size(dtype))
-    return fail(VG_ERR_INVALID_PARAMETER, std::string(name) + " is not aligned to its elements");
   // the last element's byte offset has to fit in 63 bits
   const __int128 reach = static_cast<__int128>(t->token_stride) * (tokens - 1) +
                          static_cast<__int128>(t->head_stride) * (t->num_heads - 1) + dim;
@@ -76,7 +77,7 @@ inline int check_heads(const vg_heads *t, const char *name, size_t tokens, size_
     if (!heads_in_token && !tokens_in_head)
       return fail(VG_ERR_INVALID_PARAMETER, std::string(name) + " is written to: its rows must not overlap");
   }
-  return check_device_memory(t->data, device, name);
+  return check_device_memory(t->data, element_size(dtype), device, name);
 }
 
 inline Strided strided(const vg_heads &t) { return Strided{t.data, t.token_stride, t.head_stride}; }

@@ -239,7 +239,7 @@ int vg_rotary_apply(const vg_rotary *r, int dtype, size_t head_dim, const int64_
     VG_TRY(check_device(device));
     if (tokens == 0) return VG_OK;
     DeviceGuard g(device);
-    VG_TRY(check_device_memory(positions, device, "positions"));
+    VG_TRY(check_device_memory(positions, sizeof(int64_t), device, "positions"));
     const vg_heads *in[2] = {q, k}, *out[2] = {q_out, k_out};
     const char *names[2][2] = {{"q", "q_out"}, {"k", "k_out"}};
     for (int i = 0; i < (k ? 2 : 1); ++i) {
