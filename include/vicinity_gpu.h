@@ -360,7 +360,10 @@ int vg_flat_search_ip_noalloc(const float *db, size_t n, const float *queries,
  *
  * The functions of this section enqueue their work on `stream` (a cudaStream_t
  * of the handle's device, NULL = legacy default stream) and return without
- * waiting for it.  Tensors are device memory that stays valid until that work
+ * waiting for it.  (A call of vg_kv_attend or vg_kv_evict that needs more
+ * working memory than any before allocates it and waits for the device; single
+ * tokens take what their sequences need at full capacity, so that a decoding
+ * loop does so once or twice.)  Tensors are device memory that stays valid until that work
  * is done; counts, lengths and sequence lists are host memory, read before
  * the call returns.  A vg_kv_cache is externally synchronised on the host;
  * work on its contents is ordered by the handle, also across streams.  Its

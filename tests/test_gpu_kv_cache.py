@@ -898,3 +898,36 @@ def test_misaligned_addresses_are_refused():
     odd = at(k.data_ptr() + 1)
     assert lib.vg_kv_append(c._h, counts, _lib.BF16, odd, q, None) == bad
     assert c.lengths.tolist() == [5, 0]
+
+
+def test_growing_sequences_need_no_new_memory():
+    # a decoding loop with weights: lengths pass multiples of 16 and of the
+    # chunks, the working memory stays what the first step took
+    g = np.random.default_rng(33)
+    m = Mirror(5, 1500, 2, 64, 32)
+    m.fill(g, [900, 13, 0, 601, 310])
+    before = None
+    for _ in range(150):
+        k = _rand(g, 5, 2, 64, dtype="bf16")
+        m.cache.append(k, k, [1] * 5)
+        q = _rand(g, 5, 8, 64, dtype="bf16")
+        m.cache.attend(q, [1] * 5, torch.empty_like(q), accumulate=True)
+        now = int(m.cache.info().device_bytes)
+        assert before in (None, now)
+        before = now
+
+
+def test_growing_prompts_need_new_memory_rarely():
+    # chunks of a prompt against all before them: working memory at least doubles where it grows
+    g = np.random.default_rng(34)
+    m = Mirror(2, 6000, 2, 64, 64)
+    q = _rand(g, 200, 4, 64, dtype="bf16")
+    held = [int(m.cache.info().device_bytes)]
+    for step in range(29):
+        counts = [100, 100] if step % 2 else [200, 0]
+        k = _rand(g, 200, 2, 64, dtype="bf16")
+        m.cache.append(k, k, counts)
+        m.cache.attend(q, counts, torch.empty_like(q), accumulate=True)
+        held.append(int(m.cache.info().device_bytes))
+    # one step in which every buffer is made, and a doubling of the partial sums' at most every other length
+    assert len(set(held)) <= 7, sorted(set(held))

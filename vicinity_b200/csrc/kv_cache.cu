@@ -138,7 +138,7 @@ int set_units(Plan &plan, Units &&units_of) {
 // units of one chunk of it.  Costs are in tokens of a unit: a unit's start and
 // end take about 1 us, a join 4 us, where the decoding kernel's take 3 to 4 us per
 // 512 tokens.
-constexpr uint32_t kUnitCost = 128, kJoinCost = 512;
+constexpr uint32_t kUnitCost = 128, kJoinCost = 512, kMaxWaves = 4;
 
 template <class PerChunk>
 uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, PerChunk &&per_chunk) {
@@ -156,7 +156,7 @@ uint32_t pick_chunk(const Plan &plan, uint64_t slots, uint32_t quantum, PerChunk
   };
   uint32_t best = whole;
   uint64_t cost = cost_of(whole);
-  for (uint32_t w = 1; w <= 4; ++w) {
+  for (uint32_t w = 1; w <= kMaxWaves; ++w) {
     uint32_t lo = least, hi = whole;  // the smallest chunk that makes at most w waves
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo) / 2;
@@ -176,6 +176,18 @@ constexpr size_t kScoreBytes = size_t(1) << 30;  // stored scores of one launch,
 constexpr uint64_t kSlots = 148 * 2;             // CTAs that run at once, of the decoding and the tile kernel
 constexpr uint32_t kDecodeQuantum = 32;
 
+// Working memory of `bytes`.  To replace a buffer waits for the device, so what
+// grows with the sequences is made for the longest they can get (`most`, where
+// that is known), and anything else at least doubles.
+int reserve(DevBuf &b, size_t bytes, size_t most = 0) {
+  if (bytes <= b.cap) return VG_OK;
+  if (b.reserve(std::max({bytes, most, 2 * b.cap})) != cudaSuccess) {
+    cudaGetLastError();  // no room for more than is needed
+    VG_CU(b.reserve(bytes));
+  }
+  return VG_OK;
+}
+
 // Query tiles of a plan's rows, for the tile kernels.
 int query_tiles(vg_kv_cache *kv, AttendArgs &a, Plan &plan, cudaStream_t s) {
   uint64_t blocks = 0;
@@ -184,7 +196,7 @@ int query_tiles(vg_kv_cache *kv, AttendArgs &a, Plan &plan, cudaStream_t s) {
     blocks += ceil_div(plan.s[i].count * a.group, kTileRows);
   }
   const size_t n = blocks * kv->view.heads, bytes = query_tile_bytes(kv->view.dim);
-  VG_CU(kv->ws_tiles.reserve(n * (bytes + kTileRows * sizeof(float))));
+  VG_TRY(reserve(kv->ws_tiles, n * (bytes + kTileRows * sizeof(float))));
   a.q_tiles = kv->ws_tiles.as<uint8_t>();
   a.q_factor = reinterpret_cast<float *>(a.q_tiles + n * bytes);
   VG_CU(launch_kv_query_tiles(a, plan, static_cast<uint32_t>(blocks), s));
@@ -197,9 +209,11 @@ int weigh_tiles(AttendArgs &a, Plan &plan, cudaStream_t s) {
   return VG_OK;
 }
 
-int reserve_parts(vg_kv_cache *kv, AttendArgs &a, const Plan &plan, uint32_t part_rows) {
+// max_ctas: what a plan that is cut can have at any lengths, where it is known.
+int reserve_parts(vg_kv_cache *kv, AttendArgs &a, const Plan &plan, uint32_t part_rows, size_t max_ctas = 0) {
   const size_t rows = static_cast<size_t>(plan.units) * kv->view.heads * part_rows;
-  VG_CU(kv->ws_part.reserve(rows * (kv->view.dim * sizeof(float) + sizeof(float4))));
+  const size_t row_bytes = kv->view.dim * sizeof(float) + sizeof(float4);
+  VG_TRY(reserve(kv->ws_part, rows * row_bytes, max_ctas * part_rows * row_bytes));
   a.part_o = kv->ws_part.as<float>();
   a.part_ml = reinterpret_cast<float4 *>(a.part_o + rows * kv->view.dim);
   return VG_OK;
@@ -211,19 +225,23 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
   for (uint32_t i = 0; i < plan.n; ++i) max_rows = std::max(max_rows, plan.s[i].count * a.group);
   a.chunk = pick_chunk(plan, kSlots, kDecodeQuantum, [&](const PlanSeq &) { return uint64_t(kv->view.heads); });
   bool split = false;
-  size_t scores = 0;
+  size_t scores = 0, most = 0, chunks = 0;  // the latter two: of sequences at their capacity
+  const uint32_t cap = static_cast<uint32_t>(kv->params.capacity);
   for (uint32_t i = 0; i < plan.n; ++i) {
     PlanSeq &e = plan.s[i];
     split |= e.len > a.chunk;
     e.aux = scores;
-    scores += static_cast<size_t>(kv->view.heads) * ((e.count * a.group + 1) & ~1u) *
-              (static_cast<size_t>(ceil_div(e.len, 16)) * 16);
+    const size_t rows = static_cast<size_t>(kv->view.heads) * ((e.count * a.group + 1) & ~1u);
+    scores += rows * (static_cast<size_t>(ceil_div(e.len, 16)) * 16);
+    most += rows * (static_cast<size_t>(ceil_div(cap, 16)) * 16);
+    chunks += static_cast<size_t>(kv->view.heads) * ceil_div(cap, kDecodeQuantum);
   }
   VG_TRY(set_units(plan, [&](const PlanSeq &e) { return std::max(1u, ceil_div(e.len, a.chunk)); }));
-  if (split) VG_TRY(reserve_parts(kv, a, plan, kDecodeRows));
+  if (split) VG_TRY(reserve_parts(kv, a, plan, kDecodeRows, std::min<size_t>(kMaxWaves * kSlots, chunks)));
   const bool keep = a.lse2 && scores * sizeof(float) <= kScoreBytes;
   if (keep) {
-    VG_CU(kv->ws_scores.reserve(std::max<size_t>(scores, 1) * sizeof(float)));
+    VG_TRY(reserve(kv->ws_scores, std::max<size_t>(scores, 1) * sizeof(float),
+                   std::min(most * sizeof(float), kScoreBytes)));
     a.scores = kv->ws_scores.as<float>();
   }
   VG_CU(launch_kv_attend_decode(a, plan, max_rows, s));
@@ -427,7 +445,7 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     a.lse = lse;
     a.error = kv->d_err;
     if (flags & VG_KV_ACCUMULATE) {
-      VG_CU(kv->ws_lse.reserve(rows * a.q_heads * sizeof(float)));
+      VG_TRY(reserve(kv->ws_lse, rows * a.q_heads * sizeof(float)));
       a.lse2 = kv->ws_lse.as<float>();
     }
     // by the rows of a key/value head: 16 in the decoding kernel, one row tile, more
@@ -467,7 +485,7 @@ int vg_kv_evict(vg_kv_cache *kv, size_t n, const uint32_t *src, const uint32_t *
     VG_TRY(work.begin());
     const size_t row = kv->params.num_kv_heads * budget;
     if (!kept) {
-      VG_CU(kv->ws_kept.reserve(n * row * sizeof(int32_t)));
+      VG_TRY(reserve(kv->ws_kept, n * row * sizeof(int32_t)));
       kept = kv->ws_kept.as<int32_t>();
     }
     Plan plan;
