@@ -931,3 +931,20 @@ def test_growing_prompts_need_new_memory_rarely():
         held.append(int(m.cache.info().device_bytes))
     # one step in which every buffer is made, and a doubling of the partial sums' at most every other length
     assert len(set(held)) <= 7, sorted(set(held))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("d,rot", [(128, 128), (96, 64), (50, 26)])
+def test_rotary_in_place_within_a_fused_tensor(d, rot, layout):
+    # queries and keys as slices of one projection, rotated where they lie
+    from vicinity_b200 import Rotary
+
+    g = np.random.default_rng(37)
+    t = 3001
+    x = _rand(g, t, 7, d, dtype="bf16")
+    pos = torch.arange(5, 5 + t).cuda()
+    r = Rotary(rot, layout=layout)
+    want = x.clone()
+    r.apply(pos, x[:, :4], x[:, 4:6], out_q=want[:, :4], out_k=want[:, 4:6])
+    r.apply(pos, x[:, :4], x[:, 4:6])
+    assert torch.equal(x, want)

@@ -25,14 +25,15 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// vec: p is 16-byte aligned
+// vec: p is 16-byte aligned.  Plain loads: an output may be its input, and then
+// the memory is not read-only while the kernel runs.
 template <class T>
 __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
-  T e[8];
+  alignas(16) T e[8];
   if (vec) {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4 *>(e)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+      reinterpret_cast<uint4 *>(e)[i] = reinterpret_cast<const uint4 *>(p)[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = p[i];
