@@ -463,7 +463,8 @@ int vg_kv_append(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
  * head h reads key/value head h / g.  Query j of n sees the first
  * length - n + j + 1 tokens with VG_KV_CAUSAL (the queries are the last
  * tokens appended), every token without; a query that sees none gives 0 and
- * an lse of -inf.  out = softmax(scale q.K) V in `dtype` (VG_F16 or VG_BF16),
+ * an lse of -inf.  out = softmax(scale q.K) V in `dtype` (VG_F16 or VG_BF16;
+ * out is q, at the same address and strides, or does not overlap it),
  * lse (nullable, f32 [queries][q heads], contiguous) the natural log of the
  * softmax's denominator.  VG_KV_ACCUMULATE adds to every cached token's
  * weight (per key/value head) its probabilities summed over the call's

@@ -948,3 +948,39 @@ def test_rotary_in_place_within_a_fused_tensor(d, rot, layout):
     r.apply(pos, x[:, :4], x[:, 4:6], out_q=want[:, :4], out_k=want[:, 4:6])
     r.apply(pos, x[:, :4], x[:, 4:6])
     assert torch.equal(x, want)
+
+
+def test_attend_in_place():
+    # out may be q, in every form of the kernels
+    from vicinity_b200 import KVCache
+
+    g = np.random.default_rng(35)
+    m = Mirror(4, 3000, 2, 64, 32)
+    m.fill(g, [3000, 40, 700, 500])
+    for counts in ([1, 1, 1, 1], [4, 0, 16, 1], [20, 300, 1, 64]):
+        q = _rand(g, sum(counts), 8, 64, dtype="bf16")
+        want, w = torch.empty_like(q), torch.as_tensor(m.cache.weights, device="cuda")
+        w.zero_()
+        m.cache.attend(q, counts, want, accumulate=True)
+        want_w = w.clone()
+        w.zero_()
+        m.cache.attend(q, counts, q, accumulate=True)
+        assert torch.equal(q, want) and torch.equal(w, want_w)
+    # the same memory in another order is refused
+    q = _rand(g, 8, 8, 64, dtype="bf16")
+    with pytest.raises(ValueError, match="strides of q"):
+        m.cache.attend(q, [2] * 4, q.transpose(0, 1))
+    # more scores than are kept: they are computed again from the queries
+    n, heads, d = 2_200_000, 8, 32
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    cache = KVCache(1, n, heads, d, block_tokens=128)
+    k = torch.randn(n, heads, d, generator=gen, device="cuda").to(torch.bfloat16)
+    cache.append(k, k, [n])
+    del k
+    q = torch.randn(1, heads * 16, d, generator=gen, device="cuda").to(torch.bfloat16)
+    want, w = torch.empty_like(q), torch.as_tensor(cache.weights, device="cuda")
+    cache.attend(q, [1], want, accumulate=True)
+    want_w = w.clone()
+    w.zero_()
+    cache.attend(q, [1], q, accumulate=True)
+    assert torch.equal(q, want) and torch.equal(w, want_w)

@@ -243,6 +243,8 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
     VG_TRY(reserve(kv->ws_scores, std::max<size_t>(scores, 1) * sizeof(float),
                    std::min(most * sizeof(float), kScoreBytes)));
     a.scores = kv->ws_scores.as<float>();
+  } else if (a.lse2) {  // before the attention: its outputs may take the queries' place
+    VG_TRY(query_tiles(kv, a, plan, s));
   }
   VG_CU(launch_kv_attend_decode(a, plan, max_rows, s));
   if (split) VG_CU(launch_kv_attend_join(a, plan, kDecodeRows, max_rows, s));
@@ -250,7 +252,6 @@ int attend_decode(vg_kv_cache *kv, AttendArgs a, Plan &plan, cudaStream_t s) {
     VG_TRY(set_units(plan, [](const PlanSeq &e) { return ceil_div(e.len, kWeighTile); }));
     VG_CU(launch_kv_weigh_scores(a, plan, s));
   } else if (a.lse2) {
-    VG_TRY(query_tiles(kv, a, plan, s));
     VG_TRY(weigh_tiles(a, plan, s));
   }
   return VG_OK;
@@ -427,6 +428,9 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     if (q->num_heads % kv->params.num_kv_heads)
       return fail(VG_ERR_DIMENSION_MISMATCH, "the query heads must be a multiple of the cache's key/value heads");
     if (out->num_heads != q->num_heads) return fail(VG_ERR_DIMENSION_MISMATCH, "out must have the heads of q");
+    if (out->data == q->data && ((rows > 1 && out->token_stride != q->token_stride) ||
+                                 (q->num_heads > 1 && out->head_stride != q->head_stride)))
+      return fail(VG_ERR_INVALID_PARAMETER, "out in place must have the strides of q");
     if (rows * (q->num_heads / kv->params.num_kv_heads) > 0x7fffffffull)
       return fail(VG_ERR_INVALID_PARAMETER, "too many queries in one call");
     if (lse) VG_TRY(check_device_memory(lse, sizeof(float), kv->device, "lse"));
