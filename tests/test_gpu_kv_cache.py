@@ -984,3 +984,41 @@ def test_attend_in_place():
     w.zero_()
     cache.attend(q, [1], q, accumulate=True)
     assert torch.equal(q, want) and torch.equal(w, want_w)
+
+
+def test_weights_are_ordered_across_streams():
+    # each call on a stream of its own, appends, attention and eviction: the
+    # state is that of the same calls on one stream, bit for bit
+    g = np.random.default_rng(36)
+    one, many = (Mirror(4, 4000, 2, 128, 64) for _ in range(2))
+    lens = [3600, 1, 777, 0]
+    n = sum(lens)
+    k, v = (_rand(g, n, 2, 128, dtype="bf16") for _ in range(2))
+    more = [_rand(g, 40 * 3, 2, 128, dtype="bf16") for _ in range(6)]
+    queries = [_rand(g, 3 * c, 8, 128, dtype="bf16") for c in (1, 100, 2, 1, 40, 1)]
+    outs = [[torch.empty_like(q) for q in queries] for _ in range(2)]
+    torch.cuda.synchronize()
+    for m, out, streams in ((one, outs[0], None), (many, outs[1], [torch.cuda.Stream() for _ in range(20)])):
+        at = iter(streams) if streams else None
+        stream = (lambda: next(at).cuda_stream) if streams else (lambda: None)
+        m.cache.append(k, v, lens, stream=stream())
+        for x, q, o in zip(more, queries, out):
+            m.cache.append(x, x, [40] * 3 + [0], stream=stream())
+            m.cache.attend(q, [q.shape[0] // 3] * 3 + [0], o, accumulate=True, stream=stream())
+        total = torch.as_tensor(m.cache.weights, device="cuda")
+        m.cache.evict([0], [3], 700, 50, stream=stream())
+        torch.cuda.synchronize()
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    lengths = one.cache.lengths
+    assert lengths.tolist() == many.cache.lengths.tolist() == [3840, 241, 1017, 700]
+    for s in range(4):
+        for a, b in zip(one.cache.export(s), many.cache.export(s)):
+            assert np.array_equal(a, b)
+    # every query gives each of its heads' tokens one unit in all, within the
+    # weights' bound: 2 (d + 16) u 10 + 32 u 10 for scores of sum |q k| below 10
+    # (a query that sees no token gives nothing)
+    for s in range(3):
+        rows = 4 * sum(min(q.shape[0] // 3, lens[s] + 40 * (i + 1)) for i, q in enumerate(queries))
+        w = total[s, :, :int(lengths[s])].double().sum(-1)
+        assert ((w - rows).abs() <= rows * 2.5e-4).all()
