@@ -1022,3 +1022,25 @@ def test_weights_are_ordered_across_streams():
         rows = 4 * sum(min(q.shape[0] // 3, lens[s] + 40 * (i + 1)) for i, q in enumerate(queries))
         w = total[s, :, :int(lengths[s])].double().sum(-1)
         assert ((w - rows).abs() <= rows * 2.5e-4).all()
+
+
+def test_load_and_export_of_rows_past_2_gb():
+    # a head's codes lie further apart than a strided copy reaches
+    from vicinity_b200 import KVCache
+
+    g = np.random.default_rng(38)
+    small, large = (KVCache(2, cap, 2, 128, block_tokens=64) for cap in (500, (1 << 24) + 100))
+    k = _rand(g, 300, 2, 128, dtype="bf16")
+    for c in (small, large):
+        c.append(k, k, [0, 300])
+    q = _rand(g, 1, 4, 128, dtype="bf16")
+    for c in (small, large):
+        c.attend(q, [0, 1], torch.empty_like(q), accumulate=True)
+    state = small.export(1)
+    for a, b in zip(state, large.export(1)):
+        assert np.array_equal(a, b)
+    large.load(0, *state)
+    for a, b in zip(state, large.export(0)):
+        assert np.array_equal(a, b)
+    large.load(0, *state[:4])      # without weights: zeros
+    assert not large.export(0)[4].any()
