@@ -1044,3 +1044,25 @@ def test_load_and_export_of_rows_past_2_gb():
         assert np.array_equal(a, b)
     large.load(0, *state[:4])      # without weights: zeros
     assert not large.export(0)[4].any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,group", ROWS)
+def test_attend_a_single_token_gives_its_value(n, group, dtype):
+    # the largest probability of a row is not rounded: a query that sees one
+    # token gets its value, code times scale, to the last bit
+    from vicinity_b200 import KVCache
+
+    g = np.random.default_rng(39 + n)
+    cache = KVCache(1, n, 2, 64, block_tokens=16)
+    k, v = (_rand(g, n, 2, 64, dtype="bf16", scale=s) for s in (3.0, 0.3))
+    q = _rand(g, n, 2 * group, 64, dtype=dtype, scale=2.0)
+    for length in (1, n):      # the first query of a prompt sees the first token alone
+        cache.truncate([0])
+        cache.append(k[:length], v[:length], [length])
+        kk, vv = (torch.empty(length, 2, 64, dtype=q.dtype, device="cuda") for _ in range(2))
+        cache.read([0], [length], kk, vv)
+        out = torch.full_like(q, 7.0)
+        cache.attend(q, [n], out)
+        row = n - length       # those before it see nothing
+        assert torch.equal(out[row], vv[0].repeat_interleave(group, 0))

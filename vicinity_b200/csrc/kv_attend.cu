@@ -8,8 +8,8 @@
 // power of two into its range, so both products run on the tensor cores in
 // binary16 with f32 sums; only P is rounded, to 11 bits: in more the second
 // product would take two binary16 parts, twice the products of a kernel that
-// is bound by them, for an error that an output in 16 bits does not show (f16
-// outputs differ from the exact ones by 2.1e-4 of their norm, 2.0e-4 without).
+// is bound by them, for an error that an output in 16 bits hardly shows: f16
+// outputs err by 2.1e-4 to 2.3e-4 of their norm against 2.05e-4 to 2.1e-4 in f32.
 #include "chain.cuh"
 #include "common.cuh"
 #include "elements.cuh"
@@ -184,10 +184,11 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
   for (int g = 0; g < kCols; ++g)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.0f;
-  float mu[2 * kCols], nu[2 * kCols], l[2 * kCols];
+  float nu[2 * kCols], lift[2 * kCols], l[2 * kCols];
 #pragma unroll
   for (int h = 0; h < 2 * kCols; ++h) {
-    mu[h] = nu[h] = kUnseen;
+    nu[h] = kUnseen;
+    lift[h] = 0.0f;
     l[h] = 0.0f;
   }
 
@@ -238,8 +239,8 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
     bool raise = false;
 #pragma unroll
     for (int h = 0; h < 2 * kCols; ++h) {
-      const float x = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) * f[h];
-      raise |= x + lv > mu[h] + kLazy || x > nu[h] + kLazy;
+      const float above = fmaf(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h], -nu[h]);
+      raise |= fmaxf(above, above + (lv - lift[h])) > kLazy;
     }
     if (__any_sync(VG_FULL_MASK, raise)) {
 #pragma unroll
@@ -247,8 +248,7 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
         float x = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) * f[h];
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(VG_FULL_MASK, x, w));
-        const float c = raise_reference(mu[h], x + lv);
-        l[h] *= raise_reference(nu[h], x);
+        const float c = raise_references(nu[h], lift[h], x, x + lv, l[h]);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           o[h >> 1][i][h & 1] *= c;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
       float p[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const PowerRefs refs(mu[2 * g + h], nu[2 * g + h]);
+        const PowerRefs refs(nu[2 * g + h], lift[2 * g + h]);
         const float ref = refs.exponent(lv);
         p[h] = exp2_approx(fmaf(s[g][h], f[2 * g + h], ref));
         p[2 + h] = exp2_approx(fmaf(s[g][2 + h], f[2 * g + h], ref));
@@ -314,35 +314,36 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
       *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[h >> 1][i][h & 1], o[h >> 1][i][2 + (h & 1)]);
-    if (n == 0) sml[warp * kRowsMax + row] = make_float4(mu[h], nu[h], l[h], 0.0f);
+    if (n == 0) sml[warp * kRowsMax + row] = make_float4(nu[h], lift[h], l[h], 0.0f);
   }
   __syncthreads();
   const bool whole = ps.len <= a.chunk;
   for (uint32_t e = threadIdx.x; e < rows * (D / 8); e += kDecWarps * 32) {
     const uint32_t row = e / (D / 8), c = e % (D / 8) * 8;
-    float m = kUnseen, mn = kUnseen, sum = 0.0f, y[8] = {};
+    float m = kUnseen, n = kUnseen, sum = 0.0f, y[8] = {};  // mu and nu of all
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
-      m = fmaxf(m, sml[w * kRowsMax + row].x);
-      mn = fmaxf(mn, sml[w * kRowsMax + row].y);
+      const float4 ml = sml[w * kRowsMax + row];
+      m = fmaxf(m, ml.x + ml.y);
+      n = fmaxf(n, ml.x);
     }
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
       const float4 ml = sml[w * kRowsMax + row];
-      const float f = exp2_approx(ml.x - m);
-      sum += exp2_approx(ml.y - mn) * ml.z;
+      const float f = exp2_approx(ml.x + ml.y - m);
+      sum += exp2_approx(ml.x - n) * ml.z;
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kRowsMax + row) * kPad + c + i];
     }
     if (whole) {
       const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, mn, sum, y);
+      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, n, m - n, sum, y);
     } else {
       const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kDecodeRows + row;
       float *dst = a.part_o + at * D + c;
       *reinterpret_cast<float4 *>(dst) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4 *>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
-      if (c == 0) a.part_ml[at] = make_float4(m, mn, sum, 0.0f);
+      if (c == 0) a.part_ml[at] = make_float4(n, m - n, sum, 0.0f);
     }
   }
 }
@@ -373,29 +374,29 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   const size_t first =
       ((static_cast<size_t>(ps.unit0) + block * ns) * a.kv.heads + head) * part_rows + row % part_rows;
   const int warp = threadIdx.x >> 5;
-  float m = kUnseen, mn = kUnseen;
+  float m = kUnseen, n = kUnseen;  // mu and nu of all
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
     const float4 ml = a.part_ml[first + i * step];
-    m = fmaxf(m, ml.x);
-    mn = fmaxf(mn, ml.y);
+    m = fmaxf(m, ml.x + ml.y);
+    n = fmaxf(n, ml.x);
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) {
     m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
-    mn = fmaxf(mn, __shfl_xor_sync(VG_FULL_MASK, mn, w));
+    n = fmaxf(n, __shfl_xor_sync(VG_FULL_MASK, n, w));
   }
-  if (lane_id() == 0) red[warp] = make_float2(m, mn);
+  if (lane_id() == 0) red[warp] = make_float2(m, n);
   __syncthreads();
   for (int w = 0; w < kJoinThreads / 32; ++w) {
     m = fmaxf(m, red[w].x);
-    mn = fmaxf(mn, red[w].y);
+    n = fmaxf(n, red[w].y);
   }
   __syncthreads();
   float sum = 0.0f;
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
     const float4 ml = a.part_ml[first + i * step];
-    weight[i] = exp2_approx(ml.x - m);
-    sum += exp2_approx(ml.y - mn) * ml.z;
+    weight[i] = exp2_approx(ml.x + ml.y - m);
+    sum += exp2_approx(ml.x - n) * ml.z;
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(VG_FULL_MASK, sum, w);
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += acc[(w * per + threadIdx.x) * 8 + i];
     const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, m, mn, sum, y);
+    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, n, m - n, sum, y);
   }
 }
 

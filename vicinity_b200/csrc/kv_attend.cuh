@@ -16,15 +16,17 @@ namespace vg {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 #define VG_INF __int_as_float(0x7f800000)
 
-// A row has two references, whole numbers that may lag by kLazy (fewer
-// rescalings): mu of x + log2(value scale) and nu of the scores x themselves.
+// A row has two references, which may lag by kLazy (fewer rescalings): nu of
+// the scores x and mu = nu + lift of x + log2(value scale), lift a whole number.
 // Probabilities are P = 2^(x + log2 vs - mu + kPShift) in binary16: at most
-// 2^15, and they vanish below 2^-37 of the largest.  The denominator is the
-// sum of 2^(x - nu) = P 2^(mu - nu - kPShift) / vs in f32, which no value scale
-// can overflow.  Where vs is so small beside the row's others that P would
-// vanish in f32 too, its exponent is held at x - nu - kFar: 0 in binary16 all the
-// same, but still there for the denominator.  Both start at kUnseen, the lowest
-// number: below every score but -inf, and differences stay defined.
+// 2^15, and they vanish below 2^-38 of the largest, which is a power of two when
+// the references move to it (a row that one token dominates has its value, not
+// rounded twice).  The denominator is the sum of 2^(x - nu) =
+// P 2^(lift - kPShift) / vs in f32, which no value scale can overflow.  Where vs
+// is so small beside the row's others that P would vanish in f32 too, its
+// exponent is held at x - nu - kFar: 0 in binary16 all the same, but still there
+// for the denominator.  nu starts at kUnseen, the lowest number: below every
+// score but -inf, and differences stay defined.
 constexpr float kUnseen = -3.402823466e38f;
 constexpr float kPShift = 13.0f, kLazy = 2.0f, kFar = 32.0f, kFarFactor = 4294967296.0f;
 
@@ -92,21 +94,26 @@ __device__ __forceinline__ float inverse_scale(float s) {
 // What P of a block of value scale 2^lv takes: its exponents are x plus the
 // first, its share of the denominator is P times the second.
 struct PowerRefs {
-  float mu, nu, ratio;
-  __device__ __forceinline__ PowerRefs(float m, float n) {
-    mu = m;
-    nu = n;
-    ratio = exp2_approx(m - n - kPShift);
+  float nu, lift, ratio;
+  __device__ __forceinline__ PowerRefs(float nu_, float lift_) {
+    nu = nu_;
+    lift = lift_;
+    ratio = exp2_approx(lift - kPShift);
   }
-  __device__ __forceinline__ float exponent(float lv) const { return fmaxf(lv + (kPShift - mu), -kFar - nu); }
+  __device__ __forceinline__ float exponent(float lv) const { return fmaxf(lv + (kPShift - lift), -kFar) - nu; }
   __device__ __forceinline__ float share(float per_v) const { return fminf(per_v * ratio, kFarFactor); }
 };
 
-// Takes a reference up to `top` where that is larger; returns what sums that refer to it shrink by.
-__device__ __forceinline__ float raise_reference(float &ref, float top) {
-  const float to = fmaxf(ref, ceilf(top));
-  const float c = exp2_approx(ref - to);
-  ref = to;
+// Takes mu up to m, the largest x + log2 vs, and nu to within 1/2 of n, the
+// largest x, where these are larger: the denominator l shrinks, the sum of
+// values has to shrink by the result.
+__device__ __forceinline__ float raise_references(float &nu, float &lift, float n, float m, float &l) {
+  const float top = fmaxf(nu + lift, m), less = rintf(fmaxf(nu, n) - top);
+  const float to = top + less, by = nu - to;
+  const float c = exp2_approx(by + (lift + less));
+  l *= exp2_approx(by);
+  nu = to;
+  lift = -less;
   return c;
 }
 
@@ -129,9 +136,9 @@ cudaError_t allow_smem(Kernel *kern, size_t bytes, std::atomic<uint64_t> &done) 
 
 // The result of one row from its sums: 8 dimensions from c on, and the lse.
 __device__ __forceinline__ void finish_row(const AttendArgs &a, size_t token, uint32_t hq, uint32_t c, bool ovec,
-                                           float mu, float nu, float sum, float (&y)[8]) {
+                                           float nu, float lift, float sum, float (&y)[8]) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no token seen: 0
-  const float ratio = sum == 0.0f ? 0.0f : exp2_approx(mu - nu - kPShift);
+  const float ratio = sum == 0.0f ? 0.0f : exp2_approx(lift - kPShift);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * ratio;
   store8_16(a.out.p, static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head + c,

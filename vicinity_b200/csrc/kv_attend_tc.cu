@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     const float f_row = my_tiles == 0 ? 0.0f : a.q_factor[(q_at + static_cast<size_t>(x) * kv.heads) * kRows + wr];
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t pS = tmem + x * kTok + lane_base, pO = tmem + (kTiles + x) * kTok + lane_base;
-    float mu = kUnseen, nu = kUnseen, l = 0.0f;
+    float nu = kUnseen, lift = 0.0f, l = 0.0f;
     float poison = 0.0f;  // whether the row has seen values (1) or keys (2) that read as NaN
     // products of 32 tokens from `from` on that the row does not see
     auto hide = [&](uint32_t *v, uint32_t from) {
@@ -481,9 +481,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     };
     // takes the references up to m and n where they lag too far: the sums so far shrink
     auto raise = [&](float m, float n, bool sums) {
-      if (!__any_sync(VG_FULL_MASK, m > mu + kLazy || n > nu + kLazy)) return;
-      l *= raise_reference(nu, n);
-      const float c = raise_reference(mu, m);
+      if (!__any_sync(VG_FULL_MASK, fmaxf(n, m - lift) > nu + kLazy)) return;
+      const float c = raise_references(nu, lift, n, m, l);
       if (!sums) return;
 #pragma unroll 1
       for (int b = 0; b < D; b += 16) {
@@ -498,7 +497,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
     };
     // P of 32 tokens from `from` on, into the denominator and binary16 pairs
     auto powers = [&](const uint32_t *v, const float4 *tab, uint32_t from, uint32_t (&p)[16]) {
-      const PowerRefs refs(mu, nu);
+      const PowerRefs refs(nu, lift);
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float4 e = tab[g];
@@ -603,8 +602,8 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           for (int d = 0; d < 8; ++d) y[d] = poison != 0.0f ? nan : __uint_as_float(v[8 * (d & 3) + 2 * k + (d >> 2)]);
           const uint32_t c = 4 * b + 8 * k;
           if (whole) {
-            finish_row(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, mu, nu, l,
-                       y);
+            finish_row(a, static_cast<size_t>(ps.row0) + qi, head * a.group + row - qi * a.group, c, ovec, nu, lift,
+                       l, y);
           } else {
             float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * D + c);
             dst[0] = make_float4(y[0], y[1], y[2], y[3]);
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           }
         }
       }
-      if (!whole && valid) a.part_ml[at] = make_float4(mu, nu, l, 0.0f);
+      if (!whole && valid) a.part_ml[at] = make_float4(nu, lift, l, 0.0f);
     } else {
       give_up(3);
     }

@@ -120,7 +120,7 @@ struct AttendArgs {
   // than one unit leaves [unit][head][row of 16 or 128] partial sums
   uint32_t chunk;
   float *part_o;    // [..][dim]
-  float4 *part_ml;  // [..] (references mu and nu, denominator, -)
+  float4 *part_ml;  // [..] (references nu and mu - nu, denominator, -)
   // Scores x of the call's rows, for the weights (nullable): entry e has
   // [heads][len rounded up to 16][rows rounded up to 2] from scores + plan.s[e].aux
   float *scores;
