@@ -1066,3 +1066,51 @@ def test_attend_a_single_token_gives_its_value(n, group, dtype):
         cache.attend(q, [n], out)
         row = n - length       # those before it see nothing
         assert torch.equal(out[row], vv[0].repeat_interleave(group, 0))
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("size", [5, 12, 20, 50])
+def test_attend_very_large_scores(size, n, group):
+    # scores of 2^(2 size + 3), up to far more than f32 resolves to whole numbers:
+    # tokens that tie for the largest share the attention, others get none.
+    # Everything is a power of two, so the scores are exact and add nothing to
+    # the bounds, which are those of small scores.
+    from vicinity_b200 import KVCache
+
+    g = np.random.default_rng(40 + size)
+    L, d = 3000, 64
+    sign = np.where(g.random((1, 1, d)) < 0.5, -1.0, 1.0)
+    k = np.where(g.random((L, 1, d)) < 0.5, -1.0, 1.0) * 2.0 ** size     # far below the ties, below
+    k[7::64] = -2 * sign * 2.0 ** size                                      # every other block has another scale
+    tie = np.setdiff1d(g.choice(L, 40, replace=False), np.arange(7, L, 64))
+    k[tie] = sign * 2.0 ** size
+    v = g.standard_normal((L, 1, d))
+    v[:L // 4] *= 2.0 ** 30
+    v[L // 4:L // 2] = 0.0
+    v[L // 2:3 * L // 4] *= 2.0 ** -40
+    q = np.broadcast_to(sign * 2.0 ** size, (n, group, d)) * 2.0 ** -(np.arange(n) % 3)[:, None, None]
+    kt, vt, qt = (torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(torch.bfloat16).cuda() for x in (k, v, q))
+    third = tie[(tie >= L // 2) & (tie < 3 * L // 4)]
+    soft = 32 * U * (1 + math.log(L))
+    for ties in (tie, tie[tie >= L // 2], third[:1]):
+        for negative in (False, True):
+            keys = kt.clone()
+            keys[np.setdiff1d(tie, ties)] *= -1
+            if negative:      # the ties' scores too, the others' further below
+                keys = -4 * kt.abs() * torch.from_numpy(sign).to(kt)
+                keys[ties] = -kt[ties]
+            cache = KVCache(1, L, 1, d, block_tokens=32)
+            cache.append(keys, vt, [L])
+            kr, vr = (torch.empty(L, 1, d, device="cuda") for _ in range(2))
+            cache.read([0], [L], kr, vr)
+            assert torch.equal(kr, keys.float())
+            want, want_lse, want_w, size_of, _ = _attention64(qt, kr[:, 0], vr[:, 0], False, 0.125)
+            assert ((want_w > 0.9 * n * group / len(ties)).sum() == len(ties)) and want_w.sum() > (1 - 1e-9) * n * group
+            out, lse = torch.full_like(qt, 7.0), torch.empty(n, group, device="cuda")
+            cache.attend(qt, [n], out, lse=lse, scale=0.125, causal=False, accumulate=True)
+            w = torch.as_tensor(cache.weights, device="cuda")[0, 0, :L].double()
+            assert ((lse.double() - want_lse).abs() <= 16 * U * (1 + want_lse.abs())).all()
+            tol = 1.01 * ROUND["bf16"] * want.abs() + (2.0 ** -11 + soft) * size_of
+            tol += L * 2.0 ** -36 * float(vr[ties].abs().max())
+            assert ((out.double() - want).abs() <= tol).all()
+            assert ((w - want_w).abs() <= (soft + 4 * U) * want_w + 1e-12).all()

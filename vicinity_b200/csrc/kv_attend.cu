@@ -75,6 +75,13 @@ __device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint3
   }
 }
 
+// References of joined partial sums: the largest nu, and the largest lift, so
+// that none of their factors is above 1.
+__device__ __forceinline__ void join_references(float &nu, float &lift, float4 part) {
+  nu = fmaxf(nu, part.x);
+  lift = fmaxf(lift, part.y);
+}
+
 // transposes an 8 x 8 matrix of binary16 (lane 4 r + c holds columns 2 c, 2 c + 1 of row r)
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -239,16 +246,16 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
     bool raise = false;
 #pragma unroll
     for (int h = 0; h < 2 * kCols; ++h) {
-      const float above = fmaf(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h], -nu[h]);
+      const float above = __fmul_rn(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h]) - nu[h];
       raise |= fmaxf(above, above + (lv - lift[h])) > kLazy;
     }
     if (__any_sync(VG_FULL_MASK, raise)) {
 #pragma unroll
       for (int h = 0; h < 2 * kCols; ++h) {
-        float x = fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]) * f[h];
+        float x = __fmul_rn(fmaxf(s[h >> 1][h & 1], s[h >> 1][2 + (h & 1)]), f[h]);
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(VG_FULL_MASK, x, w));
-        const float c = raise_references(nu[h], lift[h], x, x + lv, l[h]);
+        const float c = raise_references(nu[h], lift[h], x, lv, l[h]);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           o[h >> 1][i][h & 1] *= c;
@@ -263,9 +270,9 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const PowerRefs refs(nu[2 * g + h], lift[2 * g + h]);
-        const float ref = refs.exponent(lv);
-        p[h] = exp2_approx(fmaf(s[g][h], f[2 * g + h], ref));
-        p[2 + h] = exp2_approx(fmaf(s[g][2 + h], f[2 * g + h], ref));
+        const float shift = refs.shift(lv);
+        p[h] = exp2_approx(__fmul_rn(s[g][h], f[2 * g + h]) - nu[2 * g + h] + shift);
+        p[2 + h] = exp2_approx(__fmul_rn(s[g][2 + h], f[2 * g + h]) - nu[2 * g + h] + shift);
         l[2 * g + h] = fmaf(p[h] + p[2 + h], refs.share(per_v), l[2 * g + h]);
         if (scale.y != scale.y) {  // the values read as NaN: so does every row that sees one of them
           if (t + n < lim[2 * g + h]) p[h] = scale.y;
@@ -320,30 +327,26 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
   const bool whole = ps.len <= a.chunk;
   for (uint32_t e = threadIdx.x; e < rows * (D / 8); e += kDecWarps * 32) {
     const uint32_t row = e / (D / 8), c = e % (D / 8) * 8;
-    float m = kUnseen, n = kUnseen, sum = 0.0f, y[8] = {};  // mu and nu of all
+    float top_nu = kUnseen, top_lift = 0.0f, sum = 0.0f, y[8] = {};
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) join_references(top_nu, top_lift, sml[w * kRowsMax + row]);
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
       const float4 ml = sml[w * kRowsMax + row];
-      m = fmaxf(m, ml.x + ml.y);
-      n = fmaxf(n, ml.x);
-    }
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      const float4 ml = sml[w * kRowsMax + row];
-      const float f = exp2_approx(ml.x + ml.y - m);
-      sum += exp2_approx(ml.x - n) * ml.z;
+      const float f = exp2_approx(ml.x - top_nu + (ml.y - top_lift));
+      sum += exp2_approx(ml.x - top_nu) * ml.z;
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += f * so[(w * kRowsMax + row) * kPad + c + i];
     }
     if (whole) {
       const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, n, m - n, sum, y);
+      finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, top_nu, top_lift, sum, y);
     } else {
       const size_t at = (static_cast<size_t>(unit) * kv.heads + head) * kDecodeRows + row;
       float *dst = a.part_o + at * D + c;
       *reinterpret_cast<float4 *>(dst) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4 *>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
-      if (c == 0) a.part_ml[at] = make_float4(n, m - n, sum, 0.0f);
+      if (c == 0) a.part_ml[at] = make_float4(top_nu, top_lift, sum, 0.0f);
     }
   }
 }
@@ -374,29 +377,25 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   const size_t first =
       ((static_cast<size_t>(ps.unit0) + block * ns) * a.kv.heads + head) * part_rows + row % part_rows;
   const int warp = threadIdx.x >> 5;
-  float m = kUnseen, n = kUnseen;  // mu and nu of all
-  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
-    const float4 ml = a.part_ml[first + i * step];
-    m = fmaxf(m, ml.x + ml.y);
-    n = fmaxf(n, ml.x);
-  }
+  float nu = kUnseen, lift = 0.0f;
+  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) join_references(nu, lift, a.part_ml[first + i * step]);
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(VG_FULL_MASK, m, w));
-    n = fmaxf(n, __shfl_xor_sync(VG_FULL_MASK, n, w));
+    nu = fmaxf(nu, __shfl_xor_sync(VG_FULL_MASK, nu, w));
+    lift = fmaxf(lift, __shfl_xor_sync(VG_FULL_MASK, lift, w));
   }
-  if (lane_id() == 0) red[warp] = make_float2(m, n);
+  if (lane_id() == 0) red[warp] = make_float2(nu, lift);
   __syncthreads();
   for (int w = 0; w < kJoinThreads / 32; ++w) {
-    m = fmaxf(m, red[w].x);
-    n = fmaxf(n, red[w].y);
+    nu = fmaxf(nu, red[w].x);
+    lift = fmaxf(lift, red[w].y);
   }
   __syncthreads();
   float sum = 0.0f;
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
     const float4 ml = a.part_ml[first + i * step];
-    weight[i] = exp2_approx(ml.x + ml.y - m);
-    sum += exp2_approx(ml.x - n) * ml.z;
+    weight[i] = exp2_approx(ml.x - nu + (ml.y - lift));
+    sum += exp2_approx(ml.x - nu) * ml.z;
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(VG_FULL_MASK, sum, w);
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += acc[(w * per + threadIdx.x) * 8 + i];
     const uint32_t qi = row / a.group, hq = head * a.group + row - qi * a.group;
-    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, n, m - n, sum, y);
+    finish_row(a, static_cast<size_t>(ps.row0) + qi, hq, c, ovec, nu, lift, sum, y);
   }
 }
 
@@ -440,7 +439,7 @@ __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_c
   const uint32_t rows = ps.count * a.group, stride = (rows + 1) & ~1u;
   const float *sc =
       a.scores + ps.aux + (static_cast<size_t>(head) * ((ps.len + kStep - 1) / kStep * kStep) + t) * stride;
-  const float *lse = a.lse2 + static_cast<size_t>(ps.row0) * a.q_heads + head * a.group;
+  const float2 *lse = a.lse2 + static_cast<size_t>(ps.row0) * a.q_heads + head * a.group;
   float sum = 0.0f;
   for (uint32_t row = 0; row < rows; row += 2) {
     const float2 x = *reinterpret_cast<const float2 *>(sc + row);
@@ -449,7 +448,8 @@ __global__ void __launch_bounds__(kWeighTile) weigh_scores_kernel(const __grid_c
       if (row + h >= rows) break;
       const uint32_t qi = (row + h) / a.group;
       const float y = h ? x.y : x.x;
-      const float p = exp2_approx(y - lse[static_cast<size_t>(qi) * a.q_heads + row + h - qi * a.group]);
+      const float2 ref = lse[static_cast<size_t>(qi) * a.q_heads + row + h - qi * a.group];
+      const float p = exp2_approx(y - ref.x - ref.y);
       sum += y == -VG_INF ? 0.0f : p;  // not seen
     }
   }

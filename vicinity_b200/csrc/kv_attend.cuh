@@ -28,6 +28,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // for the denominator.  nu starts at kUnseen, the lowest number: below every
 // score but -inf, and differences stay defined.
 constexpr float kUnseen = -3.402823466e38f;
+// Scores beyond this (in binary logarithms) take their reference off before
+// anything else is added, in two roundings instead of one multiply-add.
+constexpr float kLargeScore = 1024.0f;
 constexpr float kPShift = 13.0f, kLazy = 2.0f, kFar = 32.0f, kFarFactor = 4294967296.0f;
 
 // 2 ulp; 0 below 2^-126 (the form that keeps subnormal results is four instructions)
@@ -91,8 +94,8 @@ __device__ __forceinline__ float inverse_scale(float s) {
   return s == s ? __uint_as_float(0x7f000000u - __float_as_uint(s)) : 1.0f;
 }
 
-// What P of a block of value scale 2^lv takes: its exponents are x plus the
-// first, its share of the denominator is P times the second.
+// What P of a block of value scale 2^lv takes: what is added to its scores, and
+// what P is multiplied by for its share of the denominator.
 struct PowerRefs {
   float nu, lift, ratio;
   __device__ __forceinline__ PowerRefs(float nu_, float lift_) {
@@ -100,16 +103,19 @@ struct PowerRefs {
     lift = lift_;
     ratio = exp2_approx(lift - kPShift);
   }
-  __device__ __forceinline__ float exponent(float lv) const { return fmaxf(lv + (kPShift - lift), -kFar) - nu; }
+  // added to x - nu, and to x itself (unless a score is so large that the rest is lost in it)
+  __device__ __forceinline__ float shift(float lv) const { return fmaxf(lv + (kPShift - lift), -kFar); }
+  __device__ __forceinline__ float exponent(float lv) const { return shift(lv) - nu; }
   __device__ __forceinline__ float share(float per_v) const { return fminf(per_v * ratio, kFarFactor); }
 };
 
-// Takes mu up to m, the largest x + log2 vs, and nu to within 1/2 of n, the
-// largest x, where these are larger: the denominator l shrinks, the sum of
-// values has to shrink by the result.
-__device__ __forceinline__ float raise_references(float &nu, float &lift, float n, float m, float &l) {
-  const float top = fmaxf(nu + lift, m), less = rintf(fmaxf(nu, n) - top);
-  const float to = top + less, by = nu - to;
+// Takes nu to within 1/2 of n, the largest x, and mu up to the largest
+// x + log2 vs, which is n + over, where these are larger: the denominator l
+// shrinks, the sum of values has to shrink by the result.  All in differences
+// from the largest score, which stay exact however large the scores are.
+__device__ __forceinline__ float raise_references(float &nu, float &lift, float n, float over, float &l) {
+  const float at = fmaxf(nu, n), top = fmaxf((nu - at) + lift, (n - at) + over), less = rintf(-top);
+  const float to = at + (top + less), by = nu - to;
   const float c = exp2_approx(by + (lift + less));
   l *= exp2_approx(by);
   nu = to;
@@ -144,9 +150,9 @@ __device__ __forceinline__ void finish_row(const AttendArgs &a, size_t token, ui
   store8_16(a.out.p, static_cast<int64_t>(token) * a.out.token + static_cast<int64_t>(hq) * a.out.head + c,
             a.dtype == VG_F16, ovec, y);
   if (c == 0) {
-    const float lse2 = sum == 0.0f ? -VG_INF : nu + log2f(sum);
-    if (a.lse) a.lse[token * a.q_heads + hq] = lse2 * kLn2;
-    if (a.lse2) a.lse2[token * a.q_heads + hq] = lse2;
+    const float rest = log2f(sum);  // -inf: no token seen
+    if (a.lse) a.lse[token * a.q_heads + hq] = (nu + rest) * kLn2;
+    if (a.lse2) a.lse2[token * a.q_heads + hq] = sum == 0.0f ? make_float2(0.0f, VG_INF) : make_float2(nu, rest);
   }
 }
 

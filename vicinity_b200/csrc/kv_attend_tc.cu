@@ -474,16 +474,32 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         float top = -VG_INF;
 #pragma unroll
         for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(v[16 * g + k]));
-        const float x = top * fmaxf(f_row * e.x, 1e-37f);
+        const float x = __fmul_rn(top, fmaxf(f_row * e.x, 1e-37f));
         n = fmaxf(n, x);
         m = fmaxf(m, x + e.y);
       }
     };
-    // takes the references up to m and n where they lag too far: the sums so far shrink
-    auto raise = [&](float m, float n, bool sums) {
-      if (!__any_sync(VG_FULL_MASK, fmaxf(n, m - lift) > nu + kLazy)) return;
-      const float c = raise_references(nu, lift, n, m, l);
-      if (!sums) return;
+    // Large scores: 32 products become scores less nu; over: the largest of
+    // these plus log2 of the value scale
+    auto subtract = [&](uint32_t *v, const float4 *tab, float &over) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 e = tab[g];
+        const float f = fmaxf(f_row * e.x, 1e-37f);
+        float top = -VG_INF;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float x = __fmul_rn(__uint_as_float(v[16 * g + k]), f) - nu;
+          v[16 * g + k] = __float_as_uint(x);
+          top = fmaxf(top, x);
+        }
+        over = fmaxf(over, top + e.y);
+      }
+    };
+    // whether a reference that goes to n would be large
+    auto any_large = [](float n) { return __any_sync(VG_FULL_MASK, fabsf(n) > kLargeScore && n != -VG_INF); };
+    // the sums of values so far shrink
+    auto shrink = [&](float c) {
 #pragma unroll 1
       for (int b = 0; b < D; b += 16) {
         uint32_t v[16];
@@ -495,13 +511,21 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         tmem_st16(pO + b, v);
       }
     };
-    // P of 32 tokens from `from` on, into the denominator and binary16 pairs
-    auto powers = [&](const uint32_t *v, const float4 *tab, uint32_t from, uint32_t (&p)[16]) {
-      const PowerRefs refs(nu, lift);
+    // whether the references lag too far behind n and m
+    auto lag = [&](float m, float n) { return __any_sync(VG_FULL_MASK, fmaxf(n, m - lift) > nu + kLazy); };
+    // takes them there
+    auto raise = [&](float m, float n, bool sums) {
+      const float c = raise_references(nu, lift, n, m - n, l);
+      if (sums) shrink(c);
+    };
+    // P of 32 tokens from `from` on, into the denominator and binary16 pairs;
+    // large: v holds scores less nu
+    auto powers = [&](const uint32_t *v, const float4 *tab, uint32_t from, auto large, uint32_t (&p)[16]) {
+      const PowerRefs refs(large.value ? 0.0f : nu, lift);
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float4 e = tab[g];
-        const float f = fmaxf(f_row * e.x, 1e-37f), ref = refs.exponent(e.y);
+        const float f = large.value ? 1.0f : fmaxf(f_row * e.x, 1e-37f), ref = refs.exponent(e.y);
         const f32x2 f2 = f2_pack(f, f), ref2 = f2_pack(ref, ref);
         f32x2 sum2[2] = {0, 0};
 #pragma unroll
@@ -524,15 +548,48 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
       __syncwarp();
       if (lane == 0) mbar_arrive(pfull + 2 * x + h);
     };
-    bool ok = true;
-    for (uint32_t i = 0; i < my_tiles; ++i) {
+    // A tile with large scores: S is read for the largest, again for what lies
+    // over the new nu, and again for P.
+    auto large_tile = [&](const float4 *tab, uint32_t t, bool edge, bool sums) {
+      float m = -VG_INF, n = -VG_INF, low = 0.0f, over = 0.0f;
+#pragma unroll 1
+      for (int step = 0; step < 12; ++step) {
+        const int c = step & 3;
+        uint32_t v[32], p[16];
+        tmem_ld32_nowait(pS + c * 32, v);
+        tmem_wait_ld32(v);
+        if (edge) hide(v, t + c * 32);
+        if (step < 4) {
+          largest(v, tab + 2 * c, m, n);
+          if (step < 3) continue;
+          const float was = nu;
+          nu = fmaxf(nu, n);
+          l *= exp2_approx(was - nu);
+          low = over = lift + (was - nu);
+          continue;
+        }
+        subtract(v, tab + 2 * c, over);
+        if (step < 7) continue;
+        if (step == 7) {
+          lift = over;
+          if (sums) shrink(exp2_approx(low - over));
+          continue;
+        }
+        powers(v, tab + 2 * c, t + c * 32, std::true_type{}, p);
+        tmem_st16(pS + c * 16, p);
+        if (c & 1) half_done(c >> 1);
+      }
+    };
+    bool ok = true, large = false;
+    auto ready = [&](uint32_t i) {
+      ok = __all_sync(VG_FULL_MASK, mbar_wait(tfull + (i & 1), (i >> 1) & 1) && mbar_wait(sfull + x, i & 1));
+      tc_fence_after();
+      return ok;
+    };
+    uint32_t i = 0;
+    for (; i < my_tiles && ready(i); ++i) {
       const uint32_t t = t0 + i * kTok;
       const float4 *tab = table + (i & 1) * 8;
-      if (!__all_sync(VG_FULL_MASK, mbar_wait(tfull + (i & 1), (i >> 1) & 1) && mbar_wait(sfull + x, i & 1))) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
       const bool edge = t + kTok > warp_lim;
       float m = -VG_INF, n = -VG_INF;
       if constexpr (kTiles == 2) {
@@ -547,11 +604,14 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) largest(v + c * 32, tab + 2 * c, m, n);
-        raise(m, n, i != 0);
+        if (lag(m, n)) {
+          if ((large = any_large(n))) break;
+          raise(m, n, i != 0);
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t p[16];
-          powers(v + c * 32, tab + 2 * c, t + c * 32, p);
+          powers(v + c * 32, tab + 2 * c, t + c * 32, std::false_type{}, p);
           tmem_st16(pS + c * 16, p);
           if (c & 1) half_done(c >> 1);
         }
@@ -564,19 +624,27 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
           if (edge) hide(v, t + c * 32);
           largest(v, tab + 2 * c, m, n);
         }
-        raise(m, n, i != 0);
+        if (lag(m, n)) {
+          if ((large = any_large(n))) break;
+          raise(m, n, i != 0);
+        }
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t v[32], p[16];
           tmem_ld32_nowait(pS + c * 32, v);
           tmem_wait_ld32(v);
           if (edge) hide(v, t + c * 32);
-          powers(v, tab + 2 * c, t + c * 32, p);
+          powers(v, tab + 2 * c, t + c * 32, std::false_type{}, p);
           tmem_st16(pS + c * 16, p);  // over S of tokens that have been read
           if (c & 1) half_done(c >> 1);
         }
       }
     }
+    // From the first tile on that would take a reference there.  (A loop of its
+    // own: as a branch of the one above, its code alone takes 1,024 queries over
+    // 16,384 tokens from 314 to 336 us.)
+    for (; large && i < my_tiles && ready(i); ++i)
+      large_tile(table + (i & 1) * 8, t0 + i * kTok, t0 + (i + 1) * kTok > warp_lim, i != 0);
     if (ok && my_tiles) {
       ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(pvdone + x, (my_tiles - 1) & 1));
       tc_fence_after();
@@ -634,7 +702,7 @@ __global__ void __launch_bounds__(kTiles == 2 ? 512 : 288, 3 - kTiles)
 //   warp 8      copies query tiles (two in flight), issues K Q^T
 template <int D>
 constexpr size_t weigh_smem() {
-  return 1024 + 3 * ((D + 63) / 64) * kKBlockBytes + 2 * kRows * (8 + 4) + kTok * 4 + 128;
+  return 1024 + 3 * ((D + 63) / 64) * kKBlockBytes + 2 * kRows * (8 + 8 + 4) + kTok * 4 + 8 * 4 + 128;
 }
 
 template <int D, class P>
@@ -646,9 +714,11 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
   constexpr uint32_t kQBytes = ((D + 63) / 64) * kKBlockBytes;
   uint8_t *sK = sm, *sQ = sm + kQBytes;  // two query tiles
   float4 *row_f = reinterpret_cast<float4 *>(sQ + 2 * kQBytes);      // [2][64] (factor, factor, -lse, -lse) of a row pair
-  uint32_t *row_lim = reinterpret_cast<uint32_t *>(row_f + 2 * 64);  // [2][128]
+  float4 *row_ref = row_f + 2 * 64;                                  // [2][64] lse of a row pair: (score, score, rest, rest)
+  uint32_t *row_lim = reinterpret_cast<uint32_t *>(row_ref + 2 * 64);  // [2][128]
   float *half = reinterpret_cast<float *>(row_lim + 2 * kRows);      // [128]
-  uint64_t *bars = reinterpret_cast<uint64_t *>(half + kTok);
+  int *row_large = reinterpret_cast<int *>(half + kTok);             // [2][4] whether 32 rows have large scores
+  uint64_t *bars = reinterpret_cast<uint64_t *>(row_large + 8);
   uint64_t *kfull = bars, *qfull = bars + 1, *qempty = bars + 3, *sfull = bars + 5, *sempty = bars + 7, *drain = bars + 9;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -751,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
     const uint32_t pS = tmem + eg * kRows + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float ks = t < ps.len ? kv.scales[0][r * (kv.stride >> kv.block_shift) + (t >> kv.block_shift)] : 0.0f;
     const f32x2 ks2 = f2_pack(ks, ks);
-    float *my_f = reinterpret_cast<float *>(row_f + eg * 64);
+    float *my_f = reinterpret_cast<float *>(row_f + eg * 64), *my_ref = reinterpret_cast<float *>(row_ref + eg * 64);
     uint32_t *my_lim = row_lim + eg * kRows;
     float total = 0.0f;
     bool ok = true;
@@ -759,22 +829,27 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
       const uint32_t b = rb0 + i;
       {
         const uint32_t row = b * kRows + wl, qi = row / a.group;
-        float lse = VG_INF;  // rows past the end, or that see nothing: probability 0
+        float2 lse = make_float2(0.0f, VG_INF);  // rows past the end, or that see nothing: probability 0
         uint32_t lim = 0;
         if (row < rows) {
           lim = tokens_seen(ps, qi, a.causal);
           lse = a.lse2[(static_cast<size_t>(ps.row0) + qi) * a.q_heads + head * a.group + row - qi * a.group];
-          if (lse == -VG_INF) lse = VG_INF;
         }
         const float f = a.q_factor[(static_cast<size_t>(ps.block0 + b) * kv.heads + head) * kRows + wl];
+        const bool large = __any_sync(VG_FULL_MASK, fabsf(lse.x) > kLargeScore);
         named_sync(1 + eg, 128);  // the previous block's have been read
         my_f[(wl >> 1) * 4 + (wl & 1)] = f;
-        my_f[(wl >> 1) * 4 + 2 + (wl & 1)] = -lse;
+        my_f[(wl >> 1) * 4 + 2 + (wl & 1)] = -(lse.x + lse.y);
+        my_ref[(wl >> 1) * 4 + (wl & 1)] = lse.x;
+        my_ref[(wl >> 1) * 4 + 2 + (wl & 1)] = lse.y;
+        if (lane == 0) row_large[eg * 4 + (wl >> 5)] = large;
         my_lim[wl] = lim;
         named_sync(1 + eg, 128);
       }
       // rows are in the order of their queries: the first one sees least
       const bool edge = my_lim[0] < t0 + kTok;
+      const int4 any = *reinterpret_cast<const int4 *>(row_large + eg * 4);
+      const bool large = any.x | any.y | any.z | any.w;
       // after a wait that gave up the loop goes on, without waits, to keep the barriers in step
       if (ok) ok = __all_sync(VG_FULL_MASK, mbar_wait_sleep(sfull + eg, (i >> 1) & 1));
       tc_fence_after();
@@ -790,13 +865,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
           __syncwarp();
           if (lane == 0) mbar_arrive(sempty + eg);
         }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float4 w = reinterpret_cast<const float4 *>(my_f)[c * 16 + k];
-          // the factors first: a product times the largest scales passes f32
-          const f32x2 f = f2_mul(f2_pack(w.x, w.y), ks2);
-          float2 p = f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), f,
-                                      f2_pack(w.z, w.w)));
+        auto add = [&](int k, float2 p) {  // of rows 2 k and 2 k + 1: powers, where they are seen
           p.x = exp2_approx(p.x);
           p.y = exp2_approx(p.y);
           if (edge) {
@@ -804,6 +873,29 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
             if (t >= my_lim[c * 32 + 2 * k + 1]) p.y = 0.0f;
           }
           sum2 = f2_add(sum2, f2_pack(p.x, p.y));
+        };
+        if (large) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float4 w = reinterpret_cast<const float4 *>(my_f)[c * 16 + k];
+            const float4 ref = reinterpret_cast<const float4 *>(my_ref)[c * 16 + k];
+            const f32x2 x = f2_mul(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])),
+                                   f2_mul(f2_pack(w.x, w.y), ks2));
+            float2 p = f2_unpack(f2_sub(f2_sub(x, f2_pack(ref.x, ref.y)), f2_pack(ref.z, ref.w)));
+            // the product's sum may differ from the attention's in its last bit: not above 1 (and NaN stays)
+            p.x = p.x > 0.0f ? 0.0f : p.x;
+            p.y = p.y > 0.0f ? 0.0f : p.y;
+            add(k, p);
+          }
+          continue;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float4 w = reinterpret_cast<const float4 *>(my_f)[c * 16 + k];
+          // the factors first: a product times the largest scales passes f32
+          const f32x2 f = f2_mul(f2_pack(w.x, w.y), ks2);
+          add(k, f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), f,
+                                  f2_pack(w.z, w.w))));
         }
       }
       const float2 sum = f2_unpack(sum2);

@@ -449,8 +449,8 @@ int vg_kv_attend(vg_kv_cache *kv, const uint32_t *counts, int dtype, const vg_he
     a.lse = lse;
     a.error = kv->d_err;
     if (flags & VG_KV_ACCUMULATE) {
-      VG_TRY(reserve(kv->ws_lse, rows * a.q_heads * sizeof(float)));
-      a.lse2 = kv->ws_lse.as<float>();
+      VG_TRY(reserve(kv->ws_lse, rows * a.q_heads * sizeof(float2)));
+      a.lse2 = kv->ws_lse.as<float2>();
     }
     // by the rows of a key/value head: 16 in the decoding kernel, one row tile, more
     const auto no_units = [](size_t, PlanSeq &) { return 0u; };

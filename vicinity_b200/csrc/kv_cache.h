@@ -115,7 +115,8 @@ struct AttendArgs {
   float scale;      // softmax scale
   bool causal;
   float *lse;       // [rows][q_heads] natural log (nullable)
-  float *lse2;      // [rows][q_heads] log2, for the weights (nullable)
+  // [rows][q_heads] log2 for the weights, as a score and the rest; (0, inf) where no token is seen (nullable)
+  float2 *lse2;
   // Splitting over the tokens: a unit takes `chunk` tokens; a sequence of more
   // than one unit leaves [unit][head][row of 16 or 128] partial sums
   uint32_t chunk;
