@@ -368,7 +368,16 @@ int vg_flat_search_ip_noalloc(const float *db, size_t n, const float *queries,
  * the call returns.  A vg_kv_cache is externally synchronised on the host;
  * work on its contents is ordered by the handle, also across streams.  Its
  * functions cannot be captured into a CUDA graph (lengths and launch shapes
- * are host state): VG_ERR_UNSUPPORTED. */
+ * are host state): VG_ERR_UNSUPPORTED.
+ *
+ * Errors.  A refused argument leaves everything as it was.  VG_ERR_CUDA and
+ * VG_ERR_OUT_OF_MEMORY may come after some sequences have been served: then
+ * outputs and weights of the call are not defined, lengths are unchanged.
+ * Waits inside the attention kernels are bounded; one that gives up is a fault
+ * of the engine, is known once the stream's work is done, and is reported by the
+ * next call on the cache that takes a stream (of vg_kv_export, for one), and
+ * by all after it, as VG_ERR_CUDA: the results since then are not valid, and
+ * the cache can only be destroyed. */
 
 /* Element types of tensors. */
 enum { VG_F32 = 0, VG_F16 = 1, VG_BF16 = 2 };
@@ -441,7 +450,10 @@ int vg_kv_get_info(const vg_kv_cache *kv, vg_kv_info *out);
 /* Tokens held by each sequence, [num_seqs]. */
 int vg_kv_lengths(const vg_kv_cache *kv, uint32_t *out);
 /* Drop the tokens of every sequence from lengths[s] on (at most the present
- * length; 0 empties it).  Host only: no device work. */
+ * length; 0 empties it).  Host only: no device work.  The block that a
+ * sequence is cut in keeps its scale, and its other tokens the codes that were
+ * rounded to it: a scale raised by dropped tokens, or a NaN they brought, stays
+ * until the sequence is cut at or before the block's start. */
 int vg_kv_truncate(vg_kv_cache *kv, const uint32_t *lengths);
 /* The accumulated weights, device f32 [num_seqs][num_kv_heads][weight_stride],
  * owned by the cache. */

@@ -37,7 +37,7 @@ namespace {
 // The order of the dimensions inside a product is free, so a lane takes whole
 // words of a token: dim / 4 consecutive key dimensions, dim / 8 consecutive
 // value dimensions.
-// 131,101 tokens x 8 heads x 128, 4 rows a head (268 MB): 50 us, 5.4 TB/s; the
+// 131,101 tokens x 8 heads x 128, 4 rows a head (268 MB): 49 us, 5.5 TB/s; the
 // copies alone take 46, the rest is the start and the end of the CTAs.
 constexpr int kStep = 16;  // tokens per step: one scale each for keys and values (blocks are multiples of 16)
 

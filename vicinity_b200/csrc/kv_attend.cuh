@@ -33,7 +33,7 @@ constexpr float kUnseen = -3.402823466e38f;
 constexpr float kLargeScore = 1024.0f;
 constexpr float kPShift = 13.0f, kLazy = 2.0f, kFar = 32.0f, kFarFactor = 4294967296.0f;
 
-// 2 ulp; 0 below 2^-126 (the form that keeps subnormal results is four instructions)
+// 2 ulp; 0 below 2^-126
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -5,12 +5,12 @@
 // it; a tile is 128 rows (the lanes of the TMEM accumulator) by 128 tokens.
 // Bound by the two products, 4 dim flops per (row, token), and as much by one
 // ex2 each; the codes are read from L2 by every row block.  1,024 queries x 32
-// heads x 128 over 16,384 tokens (266 GFLOP): 321 us, 0.83 PFLOP/s, tensor and
-// exponential pipes 55 % busy.  Product and softmax of a row tile follow each
+// heads x 128 over 16,384 tokens (266 GFLOP): 314 us after 9 for the query tiles,
+// 0.85 PFLOP/s, tensor and exponential pipes 54 % busy.  Product and softmax of a row tile follow each
 // other, two tiles take turns, and what is left is the time between a product's
 // end and the start of what waits for it; a third tile has no room in TMEM.
-// Their weights (133 GFLOP and the exponentials again): 208 us, the exponential
-// pipe 78 % busy.  See kv_attend.cu for the scaling of scores and
+// Their weights (133 GFLOP and the exponentials again): 210 us, the exponential
+// pipe 74 % busy.  See kv_attend.cu for the scaling of scores and
 // probabilities.
 //
 // attend_tile_kernel, one CTA per (sequence, head, kTiles row tiles, chunk of

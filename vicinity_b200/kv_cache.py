@@ -1,9 +1,10 @@
 """Key/value cache held in 8 bits, rotary positions, attention and eviction.
 
 The Python side of the cache section of ``include/vicinity_gpu.h``, which
-states the semantics.  Tensors are device arrays of any library whose objects
-have ``data_ptr()``, ``shape``, ``stride()`` and ``dtype`` (PyTorch tensors do),
-with f32, f16 or bf16 elements; outputs are the caller's.  Work is enqueued on
+states the semantics.  Tensors are device arrays of PyTorch, or of any library
+whose objects have ``data_ptr()``, ``shape``, ``stride()``, ``dtype``,
+``is_contiguous()`` and ``device.index`` as PyTorch's, with f32, f16 or bf16
+elements; outputs are the caller's.  Work is enqueued on
 ``stream`` (a cudaStream_t handle, None = the legacy default stream) and the
 calls return without waiting for it, so a tensor has to stay alive, and be
 ready, in that stream's order.
@@ -213,7 +214,8 @@ class KVCache:
         return c, c.buffer_info()[0], sum(c)
 
     def truncate(self, lengths) -> None:
-        """Keep the first ``lengths[s]`` tokens of every sequence; 0 empties it."""
+        """Keep the first ``lengths[s]`` tokens of every sequence; 0 empties it.
+        A block that is cut keeps its scale."""
         c, ptr, _ = self._counts(lengths, "lengths")
         _lib.check(self._lib.vg_kv_truncate(self._h, ptr))
 
@@ -232,7 +234,7 @@ class KVCache:
         [sum(counts), heads, head_dim] in f16 or bf16, into ``out`` (and the log
         of the denominators into ``lse``, f32 [sum(counts), heads]).  ``scale``
         defaults to head_dim ** -0.5.  ``accumulate`` adds the probabilities to
-        ``weights``."""
+        ``weights``.  ``out`` may be ``q``."""
         c, ptr, n = self._counts(counts)
         dt = _dtype(q)
         hq = _heads(q, "q", n, self.head_dim, dt)
@@ -277,7 +279,7 @@ class KVCache:
 
     def load(self, seq: int, k_codes, k_scales, v_codes, v_scales, weights=None, stream=None) -> None:
         """Set a sequence from host or device arrays as ``export`` returns them
-        (weights default to 0)."""
+        (weights default to 0).  Scales are powers of two in [2^-100, 2^120] or NaN."""
         n = int(k_codes.shape[1])
         codes, scales, w = self._shapes(n)
         if seq < 0:
