@@ -1114,3 +1114,38 @@ def test_attend_very_large_scores(size, n, group):
             tol += L * 2.0 ** -36 * float(vr[ties].abs().max())
             assert ((out.double() - want).abs() <= tol).all()
             assert ((w - want_w).abs() <= (soft + 4 * U) * want_w + 1e-12).all()
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("length", [300, 3000])
+@pytest.mark.parametrize("huge", [80, 118])
+def test_attend_tiny_values_beside_huge_ones_that_get_nothing(huge, length, n, group):
+    # runs of tokens that no query looks at (2^-500 of the others' probability)
+    # hold huge values: what is left of the tiny ones is not lost beside them
+    g = torch.Generator(device="cuda").manual_seed(huge + length)
+    from vicinity_b200 import KVCache
+
+    for run in (16, 112, length // 32 * 16):     # whole blocks: no token shares a huge scale
+        far = (torch.arange(length, device="cuda") // run % 2 == 1)
+        for flip in (False, True):
+            far = far ^ flip
+            k = torch.randn(length, 1, 64, generator=g, device="cuda")
+            k[..., 0] = torch.where(far, -200.0, 0.0)[:, None]
+            v = torch.randn(length, 1, 64, generator=g, device="cuda")
+            v *= torch.where(far, 2.0 ** huge, 2.0 ** -60)[:, None, None]
+            q = torch.randn(n, group, 64, generator=g, device="cuda")
+            q[..., 0] = 16.0
+            k, v, q = (x.to(torch.bfloat16) for x in (k, v, q))
+            cache = KVCache(1, length, 1, 64, block_tokens=16)
+            cache.append(k, v, [length])
+            kk, vv = (torch.empty(length, 1, 64, device="cuda") for _ in range(2))
+            cache.read([0], [length], kk, vv)
+            out, lse = torch.full_like(q, 7.0), torch.empty(n, group, device="cuda")
+            cache.attend(q, [n], out, lse=lse, causal=False)
+            want, want_lse, _, size, top = _attention64(q, kk[:, 0], vv[:, 0], False, 64 ** -0.5)
+            e = (64 + 16) * U * top
+            soft = 32 * U * (1 + want_lse.abs()) + 2 * e
+            assert ((lse.double() - want_lse).abs() <= e + 16 * U * (1 + want_lse.abs())).all()
+            tol = 1.01 * ROUND["bf16"] * want.abs() + (2.0 ** -11 + soft)[..., None] * size
+            tol += length * 2.0 ** -36 * float(vv[~far].abs().max())
+            assert ((out.double() - want).abs() <= tol).all()

@@ -75,11 +75,11 @@ __device__ __forceinline__ void row_words(const uint8_t *st, uint32_t tok, uint3
   }
 }
 
-// References of joined partial sums: the largest nu, and the largest lift, so
-// that none of their factors is above 1.
-__device__ __forceinline__ void join_references(float &nu, float &lift, float4 part) {
-  nu = fmaxf(nu, part.x);
-  lift = fmaxf(lift, part.y);
+// References of joined partial sums: the larger nu, and the lift from there to the larger mu.
+__device__ __forceinline__ void join_references(float &nu, float &lift, float nu2, float lift2) {
+  const float at = fmaxf(nu, nu2);
+  lift = fmaxf(nu - at + lift, nu2 - at + lift2);
+  nu = at;
 }
 
 // transposes an 8 x 8 matrix of binary16 (lane 4 r + c holds columns 2 c, 2 c + 1 of row r)
@@ -327,9 +327,15 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
   const bool whole = ps.len <= a.chunk;
   for (uint32_t e = threadIdx.x; e < rows * (D / 8); e += kDecWarps * 32) {
     const uint32_t row = e / (D / 8), c = e % (D / 8) * 8;
-    float top_nu = kUnseen, top_lift = 0.0f, sum = 0.0f, y[8] = {};
+    // the largest nu, and the lift from there to the largest mu
+    float top_nu = kUnseen, top_lift = kUnseen, sum = 0.0f, y[8] = {};
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) join_references(top_nu, top_lift, sml[w * kRowsMax + row]);
+    for (int w = 0; w < kDecWarps; ++w) top_nu = fmaxf(top_nu, sml[w * kRowsMax + row].x);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float4 ml = sml[w * kRowsMax + row];
+      top_lift = fmaxf(top_lift, ml.x - top_nu + ml.y);
+    }
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
       const float4 ml = sml[w * kRowsMax + row];
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(Dec<kCols>::warps * 32, 2)
 // ---- joining the chunks of a sequence -------------------------------------------
 
 // One CTA per (row, head, sequence): 32-byte slices of the row's partial sums,
-// groups of threads taking every kGroups-th chunk.  Latency: about 4 us.  (By
+// groups of threads taking every kGroups-th chunk.  Latency: about 5 us.  (By
 // the last CTA of the first kernel instead of a launch: 14 us for 74 chunks.)
 constexpr int kJoinThreads = 256;
 
@@ -378,18 +384,18 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
       ((static_cast<size_t>(ps.unit0) + block * ns) * a.kv.heads + head) * part_rows + row % part_rows;
   const int warp = threadIdx.x >> 5;
   float nu = kUnseen, lift = 0.0f;
-  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) join_references(nu, lift, a.part_ml[first + i * step]);
+  for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
+    const float4 ml = a.part_ml[first + i * step];
+    join_references(nu, lift, ml.x, ml.y);
+  }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) {
-    nu = fmaxf(nu, __shfl_xor_sync(VG_FULL_MASK, nu, w));
-    lift = fmaxf(lift, __shfl_xor_sync(VG_FULL_MASK, lift, w));
+    const float nu2 = __shfl_xor_sync(VG_FULL_MASK, nu, w), lift2 = __shfl_xor_sync(VG_FULL_MASK, lift, w);
+    join_references(nu, lift, nu2, lift2);
   }
   if (lane_id() == 0) red[warp] = make_float2(nu, lift);
   __syncthreads();
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    nu = fmaxf(nu, red[w].x);
-    lift = fmaxf(lift, red[w].y);
-  }
+  for (int w = 0; w < kJoinThreads / 32; ++w) join_references(nu, lift, red[w].x, red[w].y);
   __syncthreads();
   float sum = 0.0f;
   for (uint32_t i = threadIdx.x; i < ns; i += kJoinThreads) {
