@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh_tile_kernel(const __grid_co
   constexpr uint32_t kQBytes = ((D + 63) / 64) * kKBlockBytes;
   uint8_t *sK = sm, *sQ = sm + kQBytes;  // two query tiles
   float4 *row_f = reinterpret_cast<float4 *>(sQ + 2 * kQBytes);      // [2][64] (factor, factor, -lse, -lse) of a row pair
-  float4 *row_ref = row_f + 2 * 64;                                  // [2][64] lse of a row pair: (score, score, rest, rest)
+  float4 *row_ref = row_f + 2 * 64;  // [2][64] lse of a row pair: (score, score, rest, rest)
   uint32_t *row_lim = reinterpret_cast<uint32_t *>(row_ref + 2 * 64);  // [2][128]
   float *half = reinterpret_cast<float *>(row_lim + 2 * kRows);      // [128]
   int *row_large = reinterpret_cast<int *>(half + kTok);             // [2][4] whether 32 rows have large scores
